@@ -18,12 +18,18 @@ Supported contract:
   * ``head_dim`` a power of two ``<= 128``
   * ``attn_mask is None`` and ``dropout_p == 0`` (causal masking via ``is_causal``)
   * ``scale`` optional (defaults to ``1/sqrt(head_dim)``)
+
+Beside it stand two entry points with contracts of their own, forward and backward, over
+the same kind of kernels: :func:`cross_attention` (keys of another length, padded batches,
+shared key heads) and :func:`relative_attention` (a bias learned by relative position, over
+a sequence itself or over a cache).
 """
 from __future__ import annotations
 
 import torch
 from torch import nn
 
+from ._general import cross_attention, relative_attention
 from ._kernel import attention_train, fastflash_attn, fastflash_attn_train, FastFlashAttn, LOG2E  # noqa: F401
 
 __all__ = [
@@ -31,6 +37,9 @@ __all__ = [
     "FastFlashAttention",
     "is_eligible",
     "UnsupportedConfig",
+    "cross_attention",
+    "relative_attention",
+    "RelativeFlashAttention",
     "__version__",
 ]
 
@@ -131,3 +140,33 @@ class FastFlashAttention(nn.Module):
 
     def extra_repr(self) -> str:
         return f"is_causal={self.is_causal}, scale={self.scale}"
+
+
+class RelativeFlashAttention(nn.Module):
+    """``nn.Module`` around :func:`relative_attention` that owns the table of the bias.
+
+    ``bias`` is a bfloat16 parameter ``[num_buckets, num_heads]``, zero at first.
+    ``is_causal`` and ``scale`` are as in :class:`FastFlashAttention`; the other arguments of
+    ``forward`` are those of :func:`relative_attention`.
+    """
+
+    def __init__(self, num_heads: int, num_buckets: int = 32, max_distance: int = 128, bidirectional=None,
+                 is_causal: bool = False, scale=None, device=None):
+        super().__init__()
+        self.max_distance = max_distance
+        self.bidirectional = bidirectional
+        self.is_causal = is_causal
+        self.scale = scale
+        self.bias = nn.Parameter(torch.zeros(num_buckets, num_heads, dtype=torch.bfloat16, device=device))
+
+    def forward(self, query, key, value, query_offset=0, key_lengths=None, is_causal=None, scale=None,
+                enable_gqa=False):
+        causal = self.is_causal if is_causal is None else is_causal
+        sc = self.scale if scale is None else scale
+        return relative_attention(query, key, value, self.bias, max_distance=self.max_distance,
+                                  bidirectional=self.bidirectional, is_causal=causal, query_offset=query_offset,
+                                  key_lengths=key_lengths, scale=sc, enable_gqa=enable_gqa)
+
+    def extra_repr(self) -> str:
+        return (f"num_buckets={self.bias.shape[0]}, num_heads={self.bias.shape[1]}, max_distance={self.max_distance}, "
+                f"bidirectional={self.bidirectional}, is_causal={self.is_causal}, scale={self.scale}")

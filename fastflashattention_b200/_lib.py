@@ -34,10 +34,27 @@ SIGNATURES = {
     "ffa_bwd_dkdv_acc": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _LL, _LL, _D, _I, _VP]),
     "ffa_bwd_dq_acc": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _LL, _LL, _D, _I, _VP]),
     "ffa_lse_merge": (_I, [_VP, _VP, _VP, _VP, _LL, _I, _I, _VP]),
+    "ffa_gen_fwd_workspace": (_LL, [_VP]),
+    "ffa_gen_bwd_workspace": (_LL, [_VP]),
+    "ffa_gen_fwd": (_I, [_VP] * 7 + [_LL, _VP]),
+    "ffa_gen_bwd": (_I, [_VP] * 12 + [_LL, _VP]),
     "ffa_last_error": (_I, [ctypes.c_char_p, _I]),
     "ffa_device_status": (_I, [ctypes.POINTER(ctypes.c_uint)]),
     "ffa_version": (ctypes.c_char_p, []),
 }
+
+
+class GenTensor(ctypes.Structure):
+    """``ffa_gen_tensor``: a bf16 [batch, heads, len, head_dim] tensor, strides in elements."""
+    _fields_ = [("data", _VP), ("stride_b", _LL), ("stride_h", _LL), ("stride_s", _LL)]
+
+
+class GenProblem(ctypes.Structure):
+    """``ffa_gen_problem``: sizes, mask and position bias of general attention."""
+    _fields_ = [("batch", _I), ("q_heads", _I), ("kv_heads", _I), ("q_len", _I), ("k_len", _I), ("head_dim", _I),
+                ("causal", _I), ("scale", _D), ("key_lengths", _VP), ("query_offsets", _VP), ("query_offset", _I),
+                ("bias", _VP), ("buckets", _I), ("both", _I), ("borders", ctypes.POINTER(_I))]
+
 
 _lock = threading.Lock()
 _lib = None

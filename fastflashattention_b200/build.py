@@ -46,14 +46,18 @@ def _stale(target: Path, sources: list[Path]) -> bool:
     return any(p.stat().st_mtime > t for p in sources)
 
 
+def _torch_sources() -> list[Path]:
+    return sorted(CSRC.glob("ffa_torch*.cpp"))
+
+
 def needs_build() -> bool:
-    return _stale(LIB_PATH, _sources()) or _stale(TORCH_LIB_PATH, [CSRC / "ffa_torch.cpp", LIB_PATH,
+    return _stale(LIB_PATH, _sources()) or _stale(TORCH_LIB_PATH, [*_torch_sources(), LIB_PATH,
                                                                    *INCLUDE.glob("*.h")])
 
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     """Compile ``libffa_torch.so`` (g++, against torch's headers and libraries) if stale."""
-    if not force and not _stale(TORCH_LIB_PATH, [CSRC / "ffa_torch.cpp", LIB_PATH, *INCLUDE.glob("*.h")]):
+    if not force and not _stale(TORCH_LIB_PATH, [*_torch_sources(), LIB_PATH, *INCLUDE.glob("*.h")]):
         return TORCH_LIB_PATH
     import torch
     from torch.utils import cpp_extension as ce
@@ -63,7 +67,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     tmp = TORCH_LIB_PATH.with_suffix(".so.tmp")
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", *(f"-I{p}" for p in inc), str(CSRC / "ffa_torch.cpp"),
+           "-DTORCH_API_INCLUDE_EXTENSION_H", *(f"-I{p}" for p in inc), *map(str, _torch_sources()),
            f"-L{torch_lib}", f"-L{PKG_DIR}", "-lffa_sm100", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
            "-lc10_cuda", f"-Wl,-rpath,$ORIGIN:{torch_lib}", "-o", str(tmp)]
     if verbose:

@@ -27,6 +27,15 @@ enum : unsigned int {
   kErrDqProducer = 0x301,
   kErrDqMma = 0x302,
   kErrDqCompute = 0x303,
+  kErrGenFwdProducer = 0x401,  // general attention (ffa_gen_*.cuh)
+  kErrGenFwdMma = 0x402,
+  kErrGenFwdSoftmax = 0x403,
+  kErrGenDkdvProducer = 0x501,
+  kErrGenDkdvMma = 0x502,
+  kErrGenDkdvCompute = 0x503,
+  kErrGenDqProducer = 0x601,
+  kErrGenDqMma = 0x602,
+  kErrGenDqCompute = 0x603,
 };
 
 struct FwdArgs {

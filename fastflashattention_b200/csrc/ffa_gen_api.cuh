@@ -1,0 +1,436 @@
+// ffa_gen_api.cuh — host side of general attention: argument checks, how a problem is split,
+// tensor maps, launches and the ffa_gen_* entry points (include/ffa.h).
+#pragma once
+#include <climits>
+#include <cmath>
+
+#include "ffa_gen_bwd.cuh"
+#include "ffa_gen_fwd.cuh"
+#include "ffa_gen_step.cuh"
+
+namespace ffa {
+
+int make_map4(CUtensorMap* map, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3]);
+
+namespace gen {
+
+constexpr int kSMs = 148;
+
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+int make_map(CUtensorMap* map, const View& t, int B, int H, int S, int D) {
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(H),
+                              static_cast<cuuint64_t>(B)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.ss) * 2, static_cast<cuuint64_t>(t.sh) * 2,
+                                 static_cast<cuuint64_t>(t.sb) * 2};
+  return make_map4(map, t.p, dims, strides);
+}
+
+// ------------------------------------------------------------------------------------
+// arguments
+// ------------------------------------------------------------------------------------
+inline int check_problem(const ffa_gen_problem* p) {
+  if (!p) return set_error(FFA_ERR_INVALID, "null problem");
+  if (p->batch < 0 || p->q_heads < 0 || p->kv_heads < 0 || p->q_len < 0 || p->k_len < 0)
+    return set_error(FFA_ERR_INVALID, "sizes must be non-negative");
+  if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8 != 0)
+    return set_error(FFA_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 in [8, 128]");
+  if (p->kv_heads == 0 ? p->q_heads != 0 : p->q_heads % p->kv_heads != 0)
+    return set_error(FFA_ERR_INVALID, "q_heads must be a multiple of kv_heads");
+  if (p->q_len >= kOffsetLimit || p->k_len >= kOffsetLimit)
+    return set_error(FFA_ERR_UNSUPPORTED, "lengths must be below 2^29");
+  if (p->query_offset > kOffsetLimit || p->query_offset < -kOffsetLimit)
+    return set_error(FFA_ERR_UNSUPPORTED, "query_offset must be within +-2^29");
+  if (!std::isfinite(p->scale)) return set_error(FFA_ERR_INVALID, "scale must be finite");
+  if (p->causal && !p->bias)
+    return set_error(FFA_ERR_UNSUPPORTED, "general attention is causal only with a position bias (see ffa_fwd)");
+  if (p->bias) {
+    if (p->buckets < 1 || p->buckets > kMaxBuckets || (p->both && p->buckets % 2 != 0) || !p->borders)
+      return set_error(FFA_ERR_UNSUPPORTED, "buckets must be in [1, 256], and even for both directions");
+    const int side = p->both ? p->buckets / 2 : p->buckets;
+    if (p->borders[0] != 0) return set_error(FFA_ERR_INVALID, "the first bucket border must be 0");
+    for (int u = 1; u < side; ++u)
+      if (p->borders[u] < p->borders[u - 1] || p->borders[u] > kMaxDistance)
+        return set_error(FFA_ERR_UNSUPPORTED, "bucket borders must ascend, up to 1024");
+  }
+  // one CTA for each 64 keys or queries of a head, at the most
+  const long long heads = static_cast<long long>(p->batch) * p->q_heads;
+  const long long len = p->q_len > p->k_len ? p->q_len : p->k_len;
+  if (heads > INT_MAX || heads * ceil_div(len > 0 ? len : 1, 64) > INT_MAX / 2)
+    return set_error(FFA_ERR_UNSUPPORTED, "the problem exceeds the grid limit of 2^31-1 CTAs");
+  return FFA_OK;
+}
+
+inline int check_tensor(const ffa_gen_tensor* t, bool needed) {
+  if (!t || (needed && !t->data)) return set_error(FFA_ERR_INVALID, "null tensor pointer");
+  if (!needed) return FFA_OK;
+  if (reinterpret_cast<uintptr_t>(t->data) & 15u)
+    return set_error(FFA_ERR_INVALID, "tensor pointers must be 16-byte aligned");
+  for (const long long s : {t->stride_b, t->stride_h, t->stride_s})
+    if (s <= 0 || s % 8 != 0 || s >= (1LL << 39))
+      return set_error(FFA_ERR_INVALID, "strides must be positive multiples of 8 elements below 2^39");
+  return FFA_OK;
+}
+
+inline View view(const ffa_gen_tensor* t) { return {t->data, t->stride_b, t->stride_h, t->stride_s}; }
+
+inline Problem device_problem(const ffa_gen_problem* p) {
+  Problem d;
+  d.B = p->batch;
+  d.Hq = p->q_heads;
+  d.Hkv = p->kv_heads;
+  d.G = p->kv_heads ? p->q_heads / p->kv_heads : 1;
+  d.Sq = p->q_len;
+  d.Sk = p->k_len;
+  d.D = p->head_dim;
+  d.key_lengths = p->key_lengths;
+  d.query_offsets = p->query_offsets;
+  d.query_offset = p->query_offset;
+  d.scale_log2 = static_cast<float>(p->scale * kLog2e);
+  d.scale = static_cast<float>(p->scale);
+  return d;
+}
+
+inline Bias device_bias(const ffa_gen_problem* p) {
+  Bias b{};
+  if (!p->bias) return b;
+  b.table = static_cast<const __nv_bfloat16*>(p->bias);
+  b.buckets = p->buckets;
+  b.both = p->both ? 1 : 0;
+  b.side = b.both ? p->buckets / 2 : p->buckets;
+  for (int u = 0; u < b.side; ++u) b.borders[u] = static_cast<short>(p->borders[u]);
+  const int last = b.borders[b.side - 1];
+  b.left = last;
+  b.right = b.both ? (last > 1 ? last : 1) : 0;
+  return b;
+}
+
+// ------------------------------------------------------------------------------------
+// how a problem is split
+// ------------------------------------------------------------------------------------
+// Parts that the streamed dimension (`units` tiles) is cut into when `ctas` CTAs leave SMs
+// idle: as many as one wave of `slots` CTAs holds, each with at least `least` tiles.
+inline int split_of(long long ctas, long long slots, long long units, long long least) {
+  if (ctas <= 0 || ctas * 2 > slots) return 1;
+  const long long n = slots / ctas, most = units / least;
+  return static_cast<int>(n < most ? n : (most > 1 ? most : 1));
+}
+
+struct FwdPlan {
+  bool step;          // ffa_gen_step_kernel (few query rows for each key head), else ffa_gen_fwd_kernel
+  int mt, row_tiles;  // step: 16-row tiles of a CTA, CTAs along the rows
+  int n_split;
+  long long part_floats, bytes;
+};
+
+inline FwdPlan fwd_plan(const ffa_gen_problem* p) {
+  FwdPlan f{};
+  const long long heads = static_cast<long long>(p->batch) * p->q_heads;
+  const long long rows = p->kv_heads ? static_cast<long long>(p->q_heads / p->kv_heads) * p->q_len : 0;
+  f.step = rows <= 64;
+  f.n_split = 1;
+  if (heads * p->q_len == 0) return f;
+  if (f.step) {
+    f.mt = rows <= 16 ? 1 : 2;
+    f.row_tiles = static_cast<int>(ceil_div(rows, 16 * f.mt));
+    const long long ctas = static_cast<long long>(p->batch) * p->kv_heads * f.row_tiles;
+    f.n_split = split_of(ctas, kSMs * (p->head_dim <= 64 ? 3 : 2), ceil_div(p->k_len, 64), 2);
+  } else {
+    f.n_split = split_of(heads * ceil_div(p->q_len, 256), kSMs, ceil_div(p->k_len, 128), 2);
+  }
+  if (f.n_split > 1) {
+    f.part_floats = f.n_split * heads * p->q_len * p->head_dim;
+    f.bytes = (f.part_floats + f.n_split * heads * p->q_len) * 4;
+  }
+  return f;
+}
+
+struct BwdPlan {
+  int dq_split, dkdv_split;
+  long long stat_floats;              // LSE and delta, each
+  long long dq_off, dk_off, dv_off;   // offsets in floats; all regions start 256-byte aligned
+  long long bias_off, bytes;
+};
+
+inline BwdPlan bwd_plan(const ffa_gen_problem* p) {
+  BwdPlan w{};
+  const long long hq = static_cast<long long>(p->batch) * p->q_heads, hk = static_cast<long long>(p->batch) * p->kv_heads;
+  const long long qb = ceil_div(p->q_len, 128), kb = ceil_div(p->k_len, 128);
+  const long long g = p->kv_heads ? p->q_heads / p->kv_heads : 1;
+  w.dq_split = split_of(hq * qb, kSMs, kb, 4);
+  w.dkdv_split = split_of(hk * kb, kSMs, g * qb, 4);
+  auto round64 = [](long long n) { return (n + 63) / 64 * 64; };
+  w.stat_floats = round64(hq * padded_rows(p->q_len));
+  long long at = 2 * w.stat_floats;
+  w.dq_off = at;
+  if (w.dq_split > 1) at += round64(w.dq_split * hq * p->q_len * p->head_dim);
+  w.dk_off = at;
+  if (w.dkdv_split > 1) at += round64(w.dkdv_split * hk * p->k_len * p->head_dim);
+  w.dv_off = at;
+  if (w.dkdv_split > 1) at += round64(w.dkdv_split * hk * p->k_len * p->head_dim);
+  w.bias_off = at;
+  if (p->bias) at += round64(hq * qb * w.dq_split * p->buckets);
+  w.bytes = at * 4;
+  return w;
+}
+
+// ------------------------------------------------------------------------------------
+// launches
+// ------------------------------------------------------------------------------------
+inline int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? FFA_OK : set_error(FFA_ERR_LAUNCH, cudaGetErrorString(e));
+}
+
+struct Call {
+  Problem pr;
+  Bias bias;
+  View q, k, v, o, dout, dq, dk, dv;
+  float* lse;
+  cudaStream_t stream;
+};
+
+template <int D, bool CAUSAL, bool BIAS>
+static int launch_gen_fwd(const Call& c, const FwdPlan& f, float* ws) {
+  using L = FwdLayout<D, BIAS>;
+  const Problem& pr = c.pr;
+  CUtensorMap tq, tk, tv, to;
+  int rc;
+  if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+  if ((rc = make_map(&to, c.o, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+  tk = tv = tq;  // without keys nothing is loaded through them
+  if (pr.Sk > 0) {
+    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  }
+  auto kern = ffa_gen_fwd_kernel<D, CAUSAL, BIAS>;
+  static unsigned long long configured = 0;
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
+  if ((rc = check_launch_regs(reinterpret_cast<const void*>(kern), fwd::LAUNCH_REGS_NEEDED))) return rc;
+  const long long grid = ceil_div(pr.Sq, 256) * f.n_split * pr.B * pr.Hq;
+  kern<<<static_cast<unsigned>(grid), fwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
+      tq, tk, tv, to, pr, c.bias, c.lse, ws, ws ? ws + f.part_floats : nullptr, f.n_split,
+      work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL));
+  return launched();
+}
+
+template <int D, int MT, bool CAUSAL, bool BIAS>
+static int launch_gen_step_mt(const Call& c, const FwdPlan& f, float* ws) {
+  using L = StepLayout<D, MT>;
+  const Problem& pr = c.pr;
+  int smem = L::LUT_OFF;
+  if (BIAS) smem += L::bias_bytes(c.bias, step_heads(L::ROWS, pr.Sq, pr.G));
+  auto kern = ffa_gen_step_kernel<D, MT, CAUSAL, BIAS>;
+  constexpr int most = L::LUT_OFF + (BIAS ? (2 * kMaxDistance + 2) * 2 + kMaxBuckets * L::ROWS * 4 : 0);
+  static unsigned long long configured = 0;
+  int rc;
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
+  const long long grid = static_cast<long long>(f.n_split) * f.row_tiles * pr.Hkv * pr.B;
+  kern<<<static_cast<unsigned>(grid), 128, smem, c.stream>>>(pr, c.bias, c.q, c.k, c.v, c.o, c.lse, ws,
+                                                             ws ? ws + f.part_floats : nullptr, f.n_split,
+                                                             f.row_tiles);
+  return launched();
+}
+
+template <int D, bool CAUSAL, bool BIAS>
+static int launch_gen_step(const Call& c, const FwdPlan& f, float* ws) {
+  return f.mt == 1 ? launch_gen_step_mt<D, 1, CAUSAL, BIAS>(c, f, ws) : launch_gen_step_mt<D, 2, CAUSAL, BIAS>(c, f, ws);
+}
+
+template <int D, bool CAUSAL, bool BIAS>
+static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
+  using L = DkdvLayout<D, BIAS>;
+  const Problem& pr = c.pr;
+  CUtensorMap tk, tv, tq, tdo, tdk, tdv;
+  int rc;
+  if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  if ((rc = make_map(&tdk, c.dk, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  if ((rc = make_map(&tdv, c.dv, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  tq = tdo = tk;  // without queries nothing is loaded through them
+  if (pr.Sq > 0) {
+    if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+    if ((rc = make_map(&tdo, c.dout, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+  }
+  auto kern = ffa_gen_dkdv_kernel<D, CAUSAL, BIAS>;
+  static unsigned long long configured = 0;
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
+  if ((rc = check_launch_regs(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED))) return rc;
+  const long long grid = ceil_div(pr.Sk, 128) * w.dkdv_split * pr.B * pr.Hkv;
+  kern<<<static_cast<unsigned>(grid), bwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
+      tk, tv, tq, tdo, tdk, tdv, pr, c.bias, ws, ws + w.stat_floats, ws + w.dk_off, ws + w.dv_off, w.dkdv_split,
+      work_group(pr.B * pr.Hkv, pr.Sq * pr.G, pr.D, CAUSAL));
+  return launched();
+}
+
+template <int D, bool CAUSAL, bool BIAS>
+static int launch_gen_dq(const Call& c, const BwdPlan& w, float* ws) {
+  using L = DqLayout<D, BIAS>;
+  const Problem& pr = c.pr;
+  CUtensorMap tk, tv, tdq;
+  int rc;
+  if ((rc = make_map(&tdq, c.dq, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+  tk = tv = tdq;  // without keys nothing is loaded through them
+  if (pr.Sk > 0) {
+    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  }
+  auto kern = ffa_gen_dq_kernel<D, CAUSAL, BIAS>;
+  static unsigned long long configured = 0;
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
+  if ((rc = check_launch_regs(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED))) return rc;
+  const long long grid = ceil_div(pr.Sq, 128) * w.dq_split * pr.B * pr.Hq;
+  kern<<<static_cast<unsigned>(grid), bwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
+      tk, tv, tdq, pr, c.bias, c.q, c.dout, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split,
+      work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL));
+  return launched();
+}
+
+// The instantiation for the problem's head dim, mask and bias (check_problem: causal only
+// with a bias).
+template <template <int, bool, bool> class F, typename... A>
+static int dispatch(const Call& c, bool causal, A&&... a) {
+  const bool bias = c.bias.table != nullptr;
+  if (c.pr.D <= 64) {
+    if (!bias) return F<64, false, false>::run(c, a...);
+    return causal ? F<64, true, true>::run(c, a...) : F<64, false, true>::run(c, a...);
+  }
+  if (!bias) return F<128, false, false>::run(c, a...);
+  return causal ? F<128, true, true>::run(c, a...) : F<128, false, true>::run(c, a...);
+}
+template <int D, bool C, bool B>
+struct RunFwd {
+  static int run(const Call& c, const FwdPlan& f, float* ws) { return launch_gen_fwd<D, C, B>(c, f, ws); }
+};
+template <int D, bool C, bool B>
+struct RunStep {
+  static int run(const Call& c, const FwdPlan& f, float* ws) { return launch_gen_step<D, C, B>(c, f, ws); }
+};
+template <int D, bool C, bool B>
+struct RunDkdv {
+  static int run(const Call& c, const BwdPlan& w, float* ws) { return launch_gen_dkdv<D, C, B>(c, w, ws); }
+};
+template <int D, bool C, bool B>
+struct RunDq {
+  static int run(const Call& c, const BwdPlan& w, float* ws) { return launch_gen_dq<D, C, B>(c, w, ws); }
+};
+
+}  // namespace gen
+}  // namespace ffa
+
+extern "C" {
+
+long long ffa_gen_fwd_workspace(const ffa_gen_problem* p) {
+  if (ffa::gen::check_problem(p)) return -1;
+  return ffa::gen::fwd_plan(p).bytes;
+}
+
+long long ffa_gen_bwd_workspace(const ffa_gen_problem* p) {
+  if (ffa::gen::check_problem(p)) return -1;
+  return ffa::gen::bwd_plan(p).bytes;
+}
+
+int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
+                const ffa_gen_tensor* o, float* lse, void* workspace, long long workspace_bytes, void* stream) {
+  using namespace ffa::gen;
+  int rc = check_problem(p);
+  if (rc) return rc;
+  if (static_cast<long long>(p->batch) * p->q_heads * p->q_len == 0) return FFA_OK;
+  const bool keys = p->k_len > 0;
+  if ((rc = check_tensor(q, true)) || (rc = check_tensor(o, true)) || (rc = check_tensor(k, keys)) ||
+      (rc = check_tensor(v, keys)))
+    return rc;
+  const FwdPlan f = fwd_plan(p);
+  if (f.bytes > 0 && (!workspace || workspace_bytes < f.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+    return ffa::set_error(FFA_ERR_INVALID, "workspace missing, too small or not 16-byte aligned");
+  if ((rc = ffa::ensure_context()) != FFA_OK) return rc;
+  Call c{};
+  c.pr = device_problem(p);
+  c.bias = device_bias(p);
+  c.q = view(q);
+  c.k = view(k);
+  c.v = view(v);
+  c.o = view(o);
+  c.lse = lse;
+  c.stream = static_cast<cudaStream_t>(stream);
+  float* ws = f.n_split > 1 ? static_cast<float*>(workspace) : nullptr;
+  rc = f.step ? dispatch<RunStep>(c, p->causal, f, ws) : dispatch<RunFwd>(c, p->causal, f, ws);
+  if (rc || f.n_split == 1) return rc;
+  const long long rows = static_cast<long long>(p->batch) * p->q_heads * p->q_len;
+  ffa_gen_join_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, c.stream>>>(
+      ws, ws + f.part_floats, c.o, lse, f.n_split, p->batch, p->q_heads, p->q_len, p->head_dim);
+  return launched();
+}
+
+int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
+                const ffa_gen_tensor* o, const ffa_gen_tensor* dout, const float* lse, const ffa_gen_tensor* dq,
+                const ffa_gen_tensor* dk, const ffa_gen_tensor* dv, void* dbias, void* workspace,
+                long long workspace_bytes, void* stream) {
+  using namespace ffa::gen;
+  int rc = check_problem(p);
+  if (rc) return rc;
+  const long long hq = static_cast<long long>(p->batch) * p->q_heads;
+  const bool queries = hq * p->q_len > 0, keys = static_cast<long long>(p->batch) * p->kv_heads * p->k_len > 0;
+  const bool want_dq = dq != nullptr, want_dkdv = dk != nullptr;
+  if (want_dkdv != (dv != nullptr)) return ffa::set_error(FFA_ERR_INVALID, "dk and dv are wanted together");
+  if (dbias && (!p->bias || !want_dq)) return ffa::set_error(FFA_ERR_INVALID, "dbias needs a bias, and comes with dq");
+  if ((rc = check_tensor(q, queries)) || (rc = check_tensor(o, queries)) || (rc = check_tensor(dout, queries)) ||
+      (rc = check_tensor(k, keys)) || (rc = check_tensor(v, keys)))
+    return rc;
+  if (queries && !lse) return ffa::set_error(FFA_ERR_INVALID, "null tensor pointer");
+  if (want_dq && (rc = check_tensor(dq, queries))) return rc;
+  if (want_dkdv && ((rc = check_tensor(dk, keys)) || (rc = check_tensor(dv, keys)))) return rc;
+  const BwdPlan w = bwd_plan(p);
+  if (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+    return ffa::set_error(FFA_ERR_INVALID, "workspace missing, too small or not 16-byte aligned");
+  if ((rc = ffa::ensure_context()) != FFA_OK) return rc;
+  Call c{};
+  c.pr = device_problem(p);
+  c.bias = device_bias(p);
+  c.q = view(q);
+  c.k = view(k);
+  c.v = view(v);
+  c.o = view(o);
+  c.dout = view(dout);
+  c.stream = static_cast<cudaStream_t>(stream);
+  float* ws = static_cast<float*>(workspace);
+  if (queries) {
+    const long long rows = hq * padded_rows(p->q_len);
+    if (p->head_dim <= 64)
+      ffa_gen_prepare_kernel<8><<<static_cast<unsigned>(rows / 32), 256, 0, c.stream>>>(
+          c.o, c.dout, lse, ws, ws + w.stat_floats, p->q_heads, p->q_len, p->head_dim);
+    else
+      ffa_gen_prepare_kernel<16><<<static_cast<unsigned>(rows / 16), 256, 0, c.stream>>>(
+          c.o, c.dout, lse, ws, ws + w.stat_floats, p->q_heads, p->q_len, p->head_dim);
+    if ((rc = launched())) return rc;
+  }
+  auto sum = [&](const float* part, const View& out, int n_split, int H, int S) {
+    const long long chunks = static_cast<long long>(p->batch) * H * S * (p->head_dim / 8);
+    ffa_gen_sum_kernel<<<static_cast<unsigned>(ceil_div(chunks, 256)), 256, 0, c.stream>>>(
+        part, out, n_split, p->batch, H, S, p->head_dim);
+    return launched();
+  };
+  if (want_dkdv && keys) {
+    c.dk = view(dk);
+    c.dv = view(dv);
+    if ((rc = dispatch<RunDkdv>(c, p->causal, w, ws))) return rc;
+    if (w.dkdv_split > 1 && ((rc = sum(ws + w.dk_off, c.dk, w.dkdv_split, p->kv_heads, p->k_len)) ||
+                             (rc = sum(ws + w.dv_off, c.dv, w.dkdv_split, p->kv_heads, p->k_len))))
+      return rc;
+  }
+  if (want_dq && queries) {
+    c.dq = view(dq);
+    if ((rc = dispatch<RunDq>(c, p->causal, w, ws))) return rc;
+    if (w.dq_split > 1 && (rc = sum(ws + w.dq_off, c.dq, w.dq_split, p->q_heads, p->q_len))) return rc;
+  }
+  if (dbias && p->q_heads > 0) {
+    const int blocks = queries ? static_cast<int>(ceil_div(p->q_len, 128)) * w.dq_split : 0;
+    ffa_gen_bias_sum_kernel<<<static_cast<unsigned>(ceil_div(static_cast<long long>(p->q_heads) * p->buckets, 4)), 128,
+                              0, c.stream>>>(ws + w.bias_off, static_cast<__nv_bfloat16*>(dbias), p->batch, p->q_heads,
+                                             blocks, p->buckets);
+    if ((rc = launched())) return rc;
+  }
+  return FFA_OK;
+}
+
+}  // extern "C"

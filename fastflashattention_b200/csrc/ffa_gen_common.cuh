@@ -1,0 +1,143 @@
+// ffa_gen_common.cuh — what the kernels of general attention share.
+//
+// General attention is the family behind ffa_gen_* (include/ffa.h): queries and keys of
+// different lengths, key heads shared by groups of query heads, a key length per sequence,
+// queries that start at an offset, a causal mask and a bias learned by relative position:
+//
+//   S_ij = scale * q_i . k_j + bias[bucket(j - (i + off_b)), h]      P = softmax_j(S)
+//   key j is visible to query i of sequence b iff  j < len_b  and (causal) j <= i + off_b
+//
+// Everything below works in base 2: scores and bias entries are multiplied by log2(e).
+#pragma once
+#include "ffa_common.cuh"
+
+namespace ffa {
+namespace gen {
+
+constexpr int kMaxBuckets = 256;    // buckets of the position bias
+constexpr int kMaxDistance = 1024;  // largest border between two buckets
+constexpr int kOffsetLimit = 1 << 29;  // of lengths and offsets: sums of two stay in 32 bits
+
+// Sizes and masks of a problem, as the kernels get them.
+struct Problem {
+  int B, Hq, Hkv, G, Sq, Sk, D;  // G = Hq / Hkv query heads for each key head; D = true head dim
+  const int* key_lengths;        // [B] or null: all Sk keys
+  const int* query_offsets;      // [B] or null: query_offset for all
+  int query_offset;
+  float scale_log2, scale;
+
+  // Keys that some query of sequence b can see.  Keys behind them are read by nobody, so a
+  // cache may hold anything there, NaN included.
+  __device__ __forceinline__ int keys(int b, int off, bool causal) const {
+    int n = key_lengths ? min(max(key_lengths[b], 0), Sk) : Sk;
+    if (causal) n = min(n, max(off + Sq, 0));
+    return n;
+  }
+  __device__ __forceinline__ int offset(int b) const {
+    return query_offsets ? min(max(query_offsets[b], -kOffsetLimit), kOffsetLimit) : query_offset;
+  }
+};
+
+// The position bias.  Buckets are given by borders: on each side, bucket u holds the
+// distances in [borders[u], borders[u + 1]), the last one all from borders[side - 1] on.
+// A relative position r = key - query with r > 0 is in the second half of the buckets when
+// `both`; else it counts as distance 0.
+// From -left down and from right up the bucket, and so the bias, is constant.
+struct Bias {
+  const __nv_bfloat16* table;  // [buckets, Hq]
+  int side, both, buckets;
+  int left, right;
+  short borders[kMaxBuckets];
+
+  __device__ __forceinline__ int bucket(int r) const {
+    const int d = both ? abs(r) : max(-r, 0);
+    int lo = 0, hi = side;  // borders[lo] <= d < borders[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (borders[mid] <= d)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo + ((both && r > 0) ? side : 0);
+  }
+  // Entry times log2(e).  Entries are clamped to +-2^14 (times log2 e): beyond that one key
+  // outweighs any other by more than fp32 can hold, and the sum of a score and a bias of
+  // the type's lowest value would lose the score.  -inf (the bucket is masked) and NaN stay.
+  __device__ __forceinline__ float entry(int u, int h, int Hq) const {
+    const float v = __bfloat162float(table[static_cast<long long>(u) * Hq + h]);
+    const float lim = 16384.f;
+    const float c = v > lim ? lim : ((v < -lim && v > -INFINITY) ? -lim : v);
+    return c * static_cast<float>(kLog2e);
+  }
+};
+
+// The bias of one head by relative position, in shared memory: entry r + left + kPad for
+// r in [-left - kPad, right + kPad].  A tile of at most 128 x 128 scores that meets a
+// position in (-left, right) lies inside; the others have one bias for all their scores
+// (the first or the last entry).  Neighbouring lanes hold neighbouring positions, so a
+// warp reads 32 consecutive words: no bank conflicts.
+constexpr int kPad = 256;
+constexpr int kTableMax = 2 * kMaxDistance + 2 * kPad + 1;
+__device__ __forceinline__ int table_size(const Bias& bias) { return bias.left + bias.right + 2 * kPad + 1; }
+__device__ __forceinline__ void build_table(const Bias& bias, int h, int Hq, float* tab, int tid, int n) {
+  const int size = table_size(bias);
+  for (int t = tid; t < size; t += n) tab[t] = bias.entry(bias.bucket(t - bias.left - kPad), h, Hq);
+}
+
+// A device tensor [B, H, S, D] with contiguous D, as the C ABI describes it.
+struct View {
+  void* p;
+  long long sb, sh, ss;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2,
+                                            int c3, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+// Untiled copy of `bytes` (a multiple of 16; both addresses 16-byte aligned).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Zero the rows [row, 128) of a 128-row tile in shared memory (64-column slabs of 16 KB,
+// 128 bytes a row; the swizzle moves nothing between rows).  The whole warp calls it,
+// before it issues MMAs that read the tile.  A probability of 0 does not undo a NaN in the
+// value it is multiplied with, so rows behind the last key must not reach an MMA.
+__device__ __forceinline__ void zero_tail(uint32_t tile, int slabs, int row, int lane) {
+  for (int sl = 0; sl < slabs; ++sl)
+    for (int o = row * 128 + lane * 16; o < 16384; o += 512) st_shared_v4(tile + sl * 16384 + o, 0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Write 32 fp32 accumulator columns, times `mul`, to columns [c0, c0 + 32) of an fp32 row of
+// D values (D a multiple of 8).
+__device__ __forceinline__ void write_row32(float* dst, int c0, int D, const uint32_t (&r)[32], float mul) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (c0 + 4 * e < D)
+      *reinterpret_cast<float4*>(dst + c0 + 4 * e) =
+          make_float4(__uint_as_float(r[4 * e]) * mul, __uint_as_float(r[4 * e + 1]) * mul,
+                      __uint_as_float(r[4 * e + 2]) * mul, __uint_as_float(r[4 * e + 3]) * mul);
+}
+
+// 4-D tensor map over a [B, H, S, D] bf16 tensor: boxes of 64 columns x 128 rows, 128-byte
+// swizzle.  Columns from D on and rows from S on read as zero and are not written, so head
+// dims below the kernel's 64 or 128 need no padding in memory.
+int make_map(CUtensorMap* map, const View& t, int B, int H, int S, int D);
+
+}  // namespace gen
+}  // namespace ffa

@@ -120,6 +120,61 @@ int ffa_bwd_dq_acc(const void* q, const void* k, const void* v, const void* dout
 int ffa_lse_merge(float* acc, float* acc_lse, const void* part, const float* part_lse, long long rows, int D,
                   int first, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * General attention: keys of another length than the queries, key heads shared by groups
+ * of query heads, a length per sequence, a query offset and a learned relative position
+ * bias (no reference counterpart: its contract wants equal shapes).
+ *
+ *   S_ij = scale * q_i . k_j + bias[bucket(j - (i + off_b)), h]     O = softmax_j(S) V
+ *   key j is visible to query i of sequence b iff  j < len_b  and  (causal) j <= i + off_b
+ *
+ * A query that sees no key gets O = 0, LSE = -inf and takes no part in the backward.  K and
+ * V rows from len_b on are never multiplied with anything: they may hold NaN.
+ * ------------------------------------------------------------------------------------- */
+
+/* A bf16 tensor [batch, heads, len, head_dim], head_dim contiguous; strides in elements,
+ * positive multiples of 8 (also of dimensions of size 1); data 16-byte aligned. */
+typedef struct ffa_gen_tensor {
+  void* data;
+  long long stride_b, stride_h, stride_s;
+} ffa_gen_tensor;
+
+typedef struct ffa_gen_problem {
+  int batch, q_heads, kv_heads, q_len, k_len; /* query head h reads key head h / (q_heads / kv_heads) */
+  int head_dim;                               /* a multiple of 8, at most 128 */
+  int causal; /* only with a bias; ffa_fwd is the causal form without */
+  double scale;
+  const int* key_lengths;   /* device [batch], clamped to [0, k_len], or NULL: k_len */
+  const int* query_offsets; /* device [batch], clamped to +-2^29, or NULL: query_offset */
+  int query_offset;         /* position of the first query among the keys */
+  /* Position bias, or NULL: device bf16 [buckets, q_heads].  With `both` the positions
+   * j > i + off fall into the second half of the buckets; without it they count as distance
+   * 0.  Bucket u of a side holds the distances [borders[u], borders[u+1]), the last one all
+   * from its border on.  borders: host array, one entry for each bucket of a side, ascending
+   * from 0 to at most 1024.  At most 256 buckets.  Finite entries act as if clamped to
+   * +-2^14; -inf masks its bucket. */
+  const void* bias;
+  int buckets, both;
+  const int* borders;
+} ffa_gen_problem;
+
+/* Bytes of workspace that ffa_gen_fwd / ffa_gen_bwd need on this problem (0: none), or -1
+ * (ffa_last_error says why).  The workspace holds nothing between calls. */
+long long ffa_gen_fwd_workspace(const ffa_gen_problem* p);
+long long ffa_gen_bwd_workspace(const ffa_gen_problem* p);
+
+/* Forward.  lse: [batch, q_heads, q_len] fp32 base-2 log-sum-exp, or NULL. */
+int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
+                const ffa_gen_tensor* o, float* lse, void* workspace, long long workspace_bytes, void* stream);
+
+/* Deterministic backward (no atomics, fixed orders of summation).  dq may be NULL, and dk
+ * with dv.  dbias: bf16 [buckets, q_heads] gradient of the bias, or NULL; it needs dq.
+ * Gradients are written whole: rows without a visible counterpart are 0. */
+int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
+                const ffa_gen_tensor* o, const ffa_gen_tensor* dout, const float* lse, const ffa_gen_tensor* dq,
+                const ffa_gen_tensor* dk, const ffa_gen_tensor* dv, void* dbias, void* workspace,
+                long long workspace_bytes, void* stream);
+
 /* Most recent error message of the calling thread ("" if none). Copies at most n-1
  * bytes into buf (NUL-terminated) and returns the last error code. */
 int ffa_last_error(char* buf, int n);
