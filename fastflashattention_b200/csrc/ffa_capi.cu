@@ -115,11 +115,12 @@ int make_tile_map(CUtensorMap* map, const void* base, int BH, int S, int D, long
   return FFA_OK;
 }
 
-// 4-D bf16 map with 64 x 128 boxes (gen::make_map).  Encoding takes well under a microsecond.
-int make_map4(CUtensorMap* map, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3]) {
+// 4-D bf16 map with boxes of 64 columns x `rows` rows (gen::make_map).  Encoding takes well
+// under a microsecond.
+int make_map4(CUtensorMap* map, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3], int rows) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return set_error(FFA_ERR_LAUNCH, "cuTensorMapEncodeTiled is unavailable");
-  const cuuint32_t box[4] = {64, 128, 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -30,6 +30,8 @@ enum : unsigned int {
   kErrGenFwdProducer = 0x401,  // general attention (ffa_gen_*.cuh)
   kErrGenFwdMma = 0x402,
   kErrGenFwdSoftmax = 0x403,
+  kErrGenStepProducer = 0x404,
+  kErrGenStepCompute = 0x405,
   kErrGenDkdvProducer = 0x501,
   kErrGenDkdvMma = 0x502,
   kErrGenDkdvCompute = 0x503,

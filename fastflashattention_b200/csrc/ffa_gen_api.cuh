@@ -10,7 +10,7 @@
 
 namespace ffa {
 
-int make_map4(CUtensorMap* map, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3]);
+int make_map4(CUtensorMap* map, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3], int rows);
 
 namespace gen {
 
@@ -18,12 +18,12 @@ constexpr int kSMs = 148;
 
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-int make_map(CUtensorMap* map, const View& t, int B, int H, int S, int D) {
+int make_map(CUtensorMap* map, const View& t, int B, int H, int S, int D, int rows) {
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(H),
                               static_cast<cuuint64_t>(B)};
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.ss) * 2, static_cast<cuuint64_t>(t.sh) * 2,
                                  static_cast<cuuint64_t>(t.sb) * 2};
-  return make_map4(map, t.p, dims, strides);
+  return make_map4(map, t.p, dims, strides, rows);
 }
 
 // ------------------------------------------------------------------------------------
@@ -53,10 +53,10 @@ inline int check_problem(const ffa_gen_problem* p) {
       if (p->borders[u] < p->borders[u - 1] || p->borders[u] > kMaxDistance)
         return set_error(FFA_ERR_UNSUPPORTED, "bucket borders must ascend, up to 1024");
   }
-  // one CTA for each 64 keys or queries of a head, at the most
+  // one CTA for each 16 rows of a head, at the most
   const long long heads = static_cast<long long>(p->batch) * p->q_heads;
   const long long len = p->q_len > p->k_len ? p->q_len : p->k_len;
-  if (heads > INT_MAX || heads * ceil_div(len > 0 ? len : 1, 64) > INT_MAX / 2)
+  if (heads > INT_MAX || heads * (len > 0 ? len : 1) > 16LL * INT_MAX)
     return set_error(FFA_ERR_UNSUPPORTED, "the problem exceeds the grid limit of 2^31-1 CTAs");
   return FFA_OK;
 }
@@ -108,40 +108,92 @@ inline Bias device_bias(const ffa_gen_problem* p) {
 // ------------------------------------------------------------------------------------
 // how a problem is split
 // ------------------------------------------------------------------------------------
-// Parts that the streamed dimension (`units` tiles) is cut into when `ctas` CTAs leave SMs
-// idle: as many as one wave of `slots` CTAs holds, each with at least `least` tiles.
+// The backward: parts that the streamed dimension (`units` tiles) is cut into when `ctas`
+// CTAs leave SMs idle: as many as one wave of `slots` CTAs holds, each with at least `least`
+// tiles.
 inline int split_of(long long ctas, long long slots, long long units, long long least) {
   if (ctas <= 0 || ctas * 2 > slots) return 1;
   const long long n = slots / ctas, most = units / least;
   return static_cast<int>(n < most ? n : (most > 1 ? most : 1));
 }
 
+// The forward: steps of a split when `ctas` CTAs, `slots` at a time, each walk `units` steps of
+// `step_us` microseconds.  The estimate of a split's size is its waves times (its steps +
+// `fixed`, a CTA's start and end in steps); where lengths differ, the mean load plus one last
+// split.  Joining costs `join` steps, and for each split the traffic of `rows` fp32 rows of O.
+// The smallest estimate wins.
+inline long long split_steps(long long ctas, long long slots, long long units, bool ragged, long long rows, int D,
+                             double step_us, double fixed, double join) {
+  const double traffic = static_cast<double>(rows) * D * 8 / 6.5e6 / step_us;
+  long long best = units > 0 ? units : 1;
+  double least = 1e300;
+  for (long long n = 1; n <= 64 && n <= (units + 1) / 2; ++n) {
+    const long long per = ceil_div(units, n);
+    if (ceil_div(units, per) != n) continue;
+    const double load = static_cast<double>(ctas) * n / slots;
+    const double cost =
+        (ragged && load > 1 ? 0.6 * load * (per + fixed) + 0.4 * (per + fixed) : std::ceil(load) * (per + fixed)) +
+        (n > 1 ? join + n * traffic : 0.0);
+    if (cost < least) {
+      least = cost;
+      best = per;
+    }
+  }
+  return best;
+}
+
 struct FwdPlan {
-  bool step;          // ffa_gen_step_kernel (few query rows for each key head), else ffa_gen_fwd_kernel
-  int mt, row_tiles;  // step: 16-row tiles of a CTA, CTAs along the rows
-  int n_split;
-  long long part_floats, bytes;
+  bool step;  // ffa_gen_step_kernel (few query rows for each key head), else ffa_gen_fwd_kernel
+  // step: groups of 16 rows of an item, items of a key head, CTAs, one item for each CTA
+  int rg, row_tiles, grid;
+  bool single;
+  // else: splits of the keys and their steps
+  int n_split, per_split, keys_per_split;
+  // workspace, offsets in floats (tables) and of the parts: O, LSE, entries (bytes)
+  long long table_floats, part_off, lse_off, entry_off, bytes;
+  bool join;
 };
 
-inline FwdPlan fwd_plan(const ffa_gen_problem* p) {
+inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias) {
   FwdPlan f{};
   const long long heads = static_cast<long long>(p->batch) * p->q_heads;
-  const long long rows = p->kv_heads ? static_cast<long long>(p->q_heads / p->kv_heads) * p->q_len : 0;
-  f.step = rows <= 64;
-  f.n_split = 1;
+  const long long group_rows = p->kv_heads ? static_cast<long long>(p->q_heads / p->kv_heads) * p->q_len : 0;
+  const bool ragged = p->batch > 1 && (p->key_lengths || (p->causal && p->query_offsets));
+  const bool small_d = p->head_dim <= 64;
+  f.step = group_rows <= 64;
   if (heads * p->q_len == 0) return f;
   if (f.step) {
-    f.mt = rows <= 16 ? 1 : 2;
-    f.row_tiles = static_cast<int>(ceil_div(rows, 16 * f.mt));
-    const long long ctas = static_cast<long long>(p->batch) * p->kv_heads * f.row_tiles;
-    f.n_split = split_of(ctas, kSMs * (p->head_dim <= 64 ? 3 : 2), ceil_div(p->k_len, 64), 2);
-  } else {
-    f.n_split = split_of(heads * ceil_div(p->q_len, 256), kSMs, ceil_div(p->k_len, 128), 2);
+    f.rg = group_rows <= 16 ? 1 : 2;
+    f.row_tiles = static_cast<int>(ceil_div(group_rows, 16 * f.rg));
+    const long long items = static_cast<long long>(p->batch) * p->kv_heads * f.row_tiles;
+    const long long units = std::max<long long>(1, ceil_div(p->k_len, small_d ? 128 : 64));  // tiles of an item, at most
+    const long long slots = kSMs * (f.rg == 1 ? 2 : 1);
+    // Equal shares, unless one item a CTA does: short items in one wave, where the join would
+    // cost more than the last tiles, and sequences too many to look through.
+    f.single = units == 1 || p->batch > 1024 || (items <= slots && items * units <= slots + 3 * items);
+    f.grid = static_cast<int>(f.single ? items : std::min(slots, items * units / 2));
+    f.join = !f.single;
+    if (f.join) {
+      const long long rows = 2LL * f.grid * 16 * f.rg;
+      f.lse_off = rows * p->head_dim;
+      f.entry_off = (f.lse_off + rows) * 4;
+      f.bytes = f.entry_off + static_cast<long long>(f.grid) * sizeof(JoinEntry);
+    }
+    return f;
   }
-  if (f.n_split > 1) {
-    f.part_floats = f.n_split * heads * p->q_len * p->head_dim;
-    f.bytes = (f.part_floats + f.n_split * heads * p->q_len) * 4;
-  }
+  const int rows = small_d ? 128 : 256, keys = small_d ? 64 : 128;
+  const long long units = std::max<long long>(1, ceil_div(p->k_len, keys));
+  // a step of one CTA: four of them share an SM at head dims up to 64
+  f.per_split = static_cast<int>(split_steps(heads * ceil_div(p->q_len, rows), kSMs * (small_d ? 4 : 1), units, ragged,
+                                             heads * p->q_len, p->head_dim, small_d ? 1.0 : 2.2, small_d ? 4.0 : 2.0,
+                                             small_d ? 5.0 : 2.5));
+  f.n_split = static_cast<int>(ceil_div(units, f.per_split));
+  f.keys_per_split = f.per_split * keys;
+  f.join = f.n_split > 1;
+  if (p->bias) f.table_floats = static_cast<long long>(p->q_heads) * table_size(bias);
+  f.part_off = f.table_floats;
+  f.lse_off = f.part_off + (f.join ? f.n_split * heads * p->q_len * p->head_dim : 0);
+  f.bytes = (f.lse_off + (f.join ? f.n_split * heads * p->q_len : 0)) * 4;
   return f;
 }
 
@@ -149,10 +201,10 @@ struct BwdPlan {
   int dq_split, dkdv_split;
   long long stat_floats;              // LSE and delta, each
   long long dq_off, dk_off, dv_off;   // offsets in floats; all regions start 256-byte aligned
-  long long bias_off, bytes;
+  long long table_off, lut_off, bias_off, bytes;
 };
 
-inline BwdPlan bwd_plan(const ffa_gen_problem* p) {
+inline BwdPlan bwd_plan(const ffa_gen_problem* p, const Bias& bias) {
   BwdPlan w{};
   const long long hq = static_cast<long long>(p->batch) * p->q_heads, hk = static_cast<long long>(p->batch) * p->kv_heads;
   const long long qb = ceil_div(p->q_len, 128), kb = ceil_div(p->k_len, 128);
@@ -168,6 +220,10 @@ inline BwdPlan bwd_plan(const ffa_gen_problem* p) {
   if (w.dkdv_split > 1) at += round64(w.dkdv_split * hk * p->k_len * p->head_dim);
   w.dv_off = at;
   if (w.dkdv_split > 1) at += round64(w.dkdv_split * hk * p->k_len * p->head_dim);
+  w.table_off = at;
+  if (p->bias) at += round64(static_cast<long long>(p->q_heads) * table_size(bias));
+  w.lut_off = at;
+  if (p->bias) at += round64(lut_size(bias) / 2);
   w.bias_off = at;
   if (p->bias) at += round64(hq * qb * w.dq_split * p->buckets);
   w.bytes = at * 4;
@@ -182,6 +238,14 @@ inline int launched() {
   return e == cudaSuccess ? FFA_OK : set_error(FFA_ERR_LAUNCH, cudaGetErrorString(e));
 }
 
+// check_launch_regs, asked once for each kernel (the answer is a property of the build).
+inline int check_regs_once(const void* kernel, int needed, bool* done) {
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE)) return FFA_OK;
+  const int rc = check_launch_regs(kernel, needed);
+  if (rc == FFA_OK) __atomic_store_n(done, true, __ATOMIC_RELEASE);
+  return rc;
+}
+
 struct Call {
   Problem pr;
   Bias bias;
@@ -190,9 +254,33 @@ struct Call {
   cudaStream_t stream;
 };
 
+// A launch that may start before the kernel in front of it ends (it waits itself, where it
+// needs that kernel's results), so that its launch costs nothing.
+template <typename... P, typename... A>
+static int launch_early(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, P(args)...);
+  return e == cudaSuccess ? FFA_OK : set_error(FFA_ERR_LAUNCH, cudaGetErrorString(e));
+}
+
+static int launch_tables(const Call& c, float* tables, unsigned short* lut) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(table_size(c.bias), 256)), std::min(c.pr.Hq, 256));
+  ffa_gen_table_kernel<<<grid, 256, 0, c.stream>>>(c.bias, tables, lut, c.pr.Hq);
+  return launched();
+}
+
 template <int D, bool CAUSAL, bool BIAS>
 static int launch_gen_fwd(const Call& c, const FwdPlan& f, float* ws) {
-  using L = FwdLayout<D, BIAS>;
+  using L = FwdLayout<D>;
   const Problem& pr = c.pr;
   CUtensorMap tq, tk, tv, to;
   int rc;
@@ -200,41 +288,65 @@ static int launch_gen_fwd(const Call& c, const FwdPlan& f, float* ws) {
   if ((rc = make_map(&to, c.o, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
   tk = tv = tq;  // without keys nothing is loaded through them
   if (pr.Sk > 0) {
-    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
-    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D, L::KEYS))) return rc;
+    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D, L::KEYS))) return rc;
   }
   auto kern = ffa_gen_fwd_kernel<D, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
-  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
-  if ((rc = check_launch_regs(reinterpret_cast<const void*>(kern), fwd::LAUNCH_REGS_NEEDED))) return rc;
-  const long long grid = ceil_div(pr.Sq, 256) * f.n_split * pr.B * pr.Hq;
-  kern<<<static_cast<unsigned>(grid), fwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
-      tq, tk, tv, to, pr, c.bias, c.lse, ws, ws ? ws + f.part_floats : nullptr, f.n_split,
-      work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL));
+  constexpr int most = L::TAB_OFF + (BIAS ? kTableMax * 4 : 0) + 1024;
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
+  if constexpr (D == 128) {
+    static bool configured_regs = false;
+    if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), fwd::LAUNCH_REGS_NEEDED, &configured_regs)))
+      return rc;
+  }
+  if (BIAS && (rc = launch_tables(c, ws, nullptr))) return rc;
+  const dim3 grid(static_cast<unsigned>(ceil_div(pr.Sq, L::ROWS) * f.n_split * pr.B * pr.Hq));
+  const int group = work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL), smem = L::smem_bytes(c.bias);
+  const float* tables = ws;
+  float *part = ws ? ws + f.part_off : nullptr, *part_lse = ws ? ws + f.lse_off : nullptr;
+  if (BIAS)
+    return launch_early(kern, grid, L::THREADS, smem, c.stream, tq, tk, tv, to, pr, c.bias, tables, c.lse, part,
+                        part_lse, f.n_split, f.per_split, group);
+  kern<<<grid, L::THREADS, smem, c.stream>>>(tq, tk, tv, to, pr, c.bias, tables, c.lse, part, part_lse, f.n_split,
+                                             f.per_split, group);
   return launched();
 }
 
-template <int D, int MT, bool CAUSAL, bool BIAS>
-static int launch_gen_step_mt(const Call& c, const FwdPlan& f, float* ws) {
-  using L = StepLayout<D, MT>;
+template <int D, int RG, bool ROWS8, bool CAUSAL, bool BIAS>
+static int launch_gen_step_rg(const Call& c, const FwdPlan& f, float* ws) {
+  using L = StepLayout<D, RG>;
   const Problem& pr = c.pr;
+  int rc;
+  CUtensorMap tk{}, tv{};
+  if (pr.Sk > 0) {
+    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D, L::KEYS))) return rc;
+    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D, L::KEYS))) return rc;
+  } else {  // the one tile of an item without keys is loaded all the same, and not used
+    if ((rc = make_map(&tk, c.q, pr.B, pr.Hq, pr.Sq, pr.D, L::KEYS))) return rc;
+    tv = tk;
+  }
   int smem = L::LUT_OFF;
   if (BIAS) smem += L::bias_bytes(c.bias, step_heads(L::ROWS, pr.Sq, pr.G));
-  auto kern = ffa_gen_step_kernel<D, MT, CAUSAL, BIAS>;
-  constexpr int most = L::LUT_OFF + (BIAS ? (2 * kMaxDistance + 2) * 2 + kMaxBuckets * L::ROWS * 4 : 0);
+  auto kern = ffa_gen_step_kernel<D, RG, ROWS8, CAUSAL, BIAS>;
+  constexpr int most = L::LUT_OFF + (BIAS ? (2 * kMaxDistance + 8) * 2 + kMaxBuckets * L::ROWS * 4 : 0);
   static unsigned long long configured = 0;
-  int rc;
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
-  const long long grid = static_cast<long long>(f.n_split) * f.row_tiles * pr.Hkv * pr.B;
-  kern<<<static_cast<unsigned>(grid), 128, smem, c.stream>>>(pr, c.bias, c.q, c.k, c.v, c.o, c.lse, ws,
-                                                             ws ? ws + f.part_floats : nullptr, f.n_split,
-                                                             f.row_tiles);
-  return launched();
+  JoinEntry* entries = ws ? reinterpret_cast<JoinEntry*>(reinterpret_cast<uintptr_t>(ws) + f.entry_off) : nullptr;
+  float* part_lse = ws ? ws + f.lse_off : nullptr;
+  kern<<<f.grid, L::THREADS, smem, c.stream>>>(tk, tv, pr, c.bias, c.q, c.o, c.lse, ws, part_lse, entries, f.row_tiles,
+                                               f.single ? 1 : 0);
+  if ((rc = launched()) || !f.join) return rc;
+  const int rows = std::min(L::ROWS, pr.G * pr.Sq);
+  return launch_early(ffa_gen_step_join_kernel, dim3(f.grid, static_cast<unsigned>(ceil_div(rows, 4))), 128, 0,
+                      c.stream, pr, ws, part_lse, entries, c.o, c.lse, f.row_tiles, L::ROWS);
 }
 
 template <int D, bool CAUSAL, bool BIAS>
 static int launch_gen_step(const Call& c, const FwdPlan& f, float* ws) {
-  return f.mt == 1 ? launch_gen_step_mt<D, 1, CAUSAL, BIAS>(c, f, ws) : launch_gen_step_mt<D, 2, CAUSAL, BIAS>(c, f, ws);
+  if (f.rg == 2) return launch_gen_step_rg<D, 2, false, CAUSAL, BIAS>(c, f, ws);
+  return c.pr.G * c.pr.Sq <= 8 ? launch_gen_step_rg<D, 1, true, CAUSAL, BIAS>(c, f, ws)
+                               : launch_gen_step_rg<D, 1, false, CAUSAL, BIAS>(c, f, ws);
 }
 
 template <int D, bool CAUSAL, bool BIAS>
@@ -254,12 +366,13 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   }
   auto kern = ffa_gen_dkdv_kernel<D, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
+  static bool configured_regs = false;
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
-  if ((rc = check_launch_regs(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED))) return rc;
+  if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs))) return rc;
   const long long grid = ceil_div(pr.Sk, 128) * w.dkdv_split * pr.B * pr.Hkv;
   kern<<<static_cast<unsigned>(grid), bwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
-      tk, tv, tq, tdo, tdk, tdv, pr, c.bias, ws, ws + w.stat_floats, ws + w.dk_off, ws + w.dv_off, w.dkdv_split,
-      work_group(pr.B * pr.Hkv, pr.Sq * pr.G, pr.D, CAUSAL));
+      tk, tv, tq, tdo, tdk, tdv, pr, c.bias, ws + w.table_off, ws, ws + w.stat_floats, ws + w.dk_off, ws + w.dv_off, w.dkdv_split,
+      work_group(pr.B * pr.Hkv, static_cast<int>(std::min<long long>(1LL * pr.Sq * pr.G, INT_MAX)), pr.D, CAUSAL));
   return launched();
 }
 
@@ -277,11 +390,13 @@ static int launch_gen_dq(const Call& c, const BwdPlan& w, float* ws) {
   }
   auto kern = ffa_gen_dq_kernel<D, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
+  static bool configured_regs = false;
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
-  if ((rc = check_launch_regs(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED))) return rc;
+  if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs))) return rc;
   const long long grid = ceil_div(pr.Sq, 128) * w.dq_split * pr.B * pr.Hq;
   kern<<<static_cast<unsigned>(grid), bwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
-      tk, tv, tdq, pr, c.bias, c.q, c.dout, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split,
+      tk, tv, tdq, pr, c.bias, ws + w.table_off,
+      reinterpret_cast<const unsigned short*>(ws + w.lut_off), c.q, c.dout, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split,
       work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL));
   return launched();
 }
@@ -322,12 +437,12 @@ extern "C" {
 
 long long ffa_gen_fwd_workspace(const ffa_gen_problem* p) {
   if (ffa::gen::check_problem(p)) return -1;
-  return ffa::gen::fwd_plan(p).bytes;
+  return ffa::gen::fwd_plan(p, ffa::gen::device_bias(p)).bytes;
 }
 
 long long ffa_gen_bwd_workspace(const ffa_gen_problem* p) {
   if (ffa::gen::check_problem(p)) return -1;
-  return ffa::gen::bwd_plan(p).bytes;
+  return ffa::gen::bwd_plan(p, ffa::gen::device_bias(p)).bytes;
 }
 
 int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
@@ -340,26 +455,27 @@ int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   if ((rc = check_tensor(q, true)) || (rc = check_tensor(o, true)) || (rc = check_tensor(k, keys)) ||
       (rc = check_tensor(v, keys)))
     return rc;
-  const FwdPlan f = fwd_plan(p);
+  const Bias bias = device_bias(p);
+  const FwdPlan f = fwd_plan(p, bias);
   if (f.bytes > 0 && (!workspace || workspace_bytes < f.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return ffa::set_error(FFA_ERR_INVALID, "workspace missing, too small or not 16-byte aligned");
   if ((rc = ffa::ensure_context()) != FFA_OK) return rc;
   Call c{};
   c.pr = device_problem(p);
-  c.bias = device_bias(p);
+  c.bias = bias;
   c.q = view(q);
   c.k = view(k);
   c.v = view(v);
   c.o = view(o);
   c.lse = lse;
   c.stream = static_cast<cudaStream_t>(stream);
-  float* ws = f.n_split > 1 ? static_cast<float*>(workspace) : nullptr;
-  rc = f.step ? dispatch<RunStep>(c, p->causal, f, ws) : dispatch<RunFwd>(c, p->causal, f, ws);
-  if (rc || f.n_split == 1) return rc;
+  float* ws = f.bytes > 0 ? static_cast<float*>(workspace) : nullptr;
+  if (f.step) return dispatch<RunStep>(c, p->causal, f, ws);
+  rc = dispatch<RunFwd>(c, p->causal, f, ws);
+  if (rc || !f.join) return rc;
   const long long rows = static_cast<long long>(p->batch) * p->q_heads * p->q_len;
-  ffa_gen_join_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, c.stream>>>(
-      ws, ws + f.part_floats, c.o, lse, f.n_split, p->batch, p->q_heads, p->q_len, p->head_dim);
-  return launched();
+  return launch_early(ffa_gen_join_kernel, dim3(static_cast<unsigned>(ceil_div(rows, 4))), 128, 0, c.stream, c.pr,
+                      ws + f.part_off, ws + f.lse_off, c.o, lse, f.keys_per_split, p->causal ? 1 : 0);
 }
 
 int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
@@ -380,13 +496,14 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   if (queries && !lse) return ffa::set_error(FFA_ERR_INVALID, "null tensor pointer");
   if (want_dq && (rc = check_tensor(dq, queries))) return rc;
   if (want_dkdv && ((rc = check_tensor(dk, keys)) || (rc = check_tensor(dv, keys)))) return rc;
-  const BwdPlan w = bwd_plan(p);
+  const Bias bias = device_bias(p);
+  const BwdPlan w = bwd_plan(p, bias);
   if (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return ffa::set_error(FFA_ERR_INVALID, "workspace missing, too small or not 16-byte aligned");
   if ((rc = ffa::ensure_context()) != FFA_OK) return rc;
   Call c{};
   c.pr = device_problem(p);
-  c.bias = device_bias(p);
+  c.bias = bias;
   c.q = view(q);
   c.k = view(k);
   c.v = view(v);
@@ -394,6 +511,8 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   c.dout = view(dout);
   c.stream = static_cast<cudaStream_t>(stream);
   float* ws = static_cast<float*>(workspace);
+  if (p->bias && queries && (rc = launch_tables(c, ws + w.table_off, reinterpret_cast<unsigned short*>(ws + w.lut_off))))
+    return rc;
   if (queries) {
     const long long rows = hq * padded_rows(p->q_len);
     if (p->head_dim <= 64)

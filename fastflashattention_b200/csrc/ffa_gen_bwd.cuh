@@ -104,6 +104,13 @@ __global__ void __launch_bounds__(128) ffa_gen_bias_sum_kernel(const float* __re
   if (lane == 0) dbias[static_cast<long long>(u) * H + h] = __float2bfloat16_rn(a);
 }
 
+// Head h's table (ffa_gen_table_kernel) into shared memory.
+__device__ __forceinline__ void copy_table(float* tab, const float* tables, int h, const Bias& bias, int tid, int n) {
+  const int units = table_size(bias) / 4;
+  const float4* src = reinterpret_cast<const float4*>(tables) + static_cast<long long>(h) * units;
+  for (int t = tid; t < units; t += n) reinterpret_cast<float4*>(tab)[t] = src[t];
+}
+
 // Write the accumulator columns [g*D/2, (g+1)*D/2) of this lane to fp32 row `dst` (pr.D
 // values); `empty`: nothing was accumulated, write zeros.  The whole warp calls it.
 template <int D>
@@ -185,7 +192,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
                         const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                         const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                         const __grid_constant__ Problem pr, const __grid_constant__ Bias bias,
-                        const float* __restrict__ LSE, const float* __restrict__ DELTA, float* __restrict__ dk_part,
+                        const float* __restrict__ tables, const float* __restrict__ LSE,
+                        const float* __restrict__ DELTA, float* __restrict__ dk_part,
                         float* __restrict__ dv_part, int n_split, int group) {
   using L = DkdvLayout<D, BIAS>;
   constexpr int SLABS = D / 64;
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       constexpr uint32_t IDESC_G = idesc_bf16(128, D, false, true);      // [128 keys x D]
       const uint64_t kdesc = kmajor_desc(sbase + L::K_OFF, 128, 0), vdesc = kmajor_desc(sbase + L::V_OFF, 128, 0);
       auto issue_s = [&](int i) -> bool {  // S^T = K Q_i^T
-        if (!mbar_wait(q_full(i % QS), (i / QS) & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!warp_wait(q_full(i % QS), (i / QS) & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t qd = kmajor_desc(q_addr(i), 128, 0);
         if (elect_one()) {
@@ -339,7 +347,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         return true;
       };
       auto issue_dp = [&](int i) -> bool {  // dP^T = V dO_i^T
-        if (!mbar_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!warp_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t dd = kmajor_desc(do_addr(i), 128, 0);
         if (elect_one()) {
@@ -353,7 +361,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         return true;
       };
       auto issue_dv = [&](int i) -> bool {  // dV += P^T dO_i
-        if (!mbar_wait(p_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!warp_wait(p_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t dd = mnmajor_desc(do_addr(i), 128, 0);
         if (elect_one()) {
@@ -366,7 +374,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         return true;
       };
       auto issue_dk = [&](int i) -> bool {  // dK += dS^T Q_i
-        if (!mbar_wait(ds_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!warp_wait(ds_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t qd = mnmajor_desc(q_addr(i), 128, 0);
         if (elect_one()) {
@@ -382,7 +390,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       };
       bool ok = true;
       if (ns > 0) {
-        ok = mbar_wait(kv_full, 0, abort_flag, kErrGenDkdvMma);
+        ok = warp_wait(kv_full, 0, abort_flag, kErrGenDkdvMma);
         if (ok && n0 + 128 > n_keys && n_keys < pr.Sk) {
           zero_tail(sbase + L::K_OFF, SLABS, n_keys - n0, lane);
           zero_tail(sbase + L::V_OFF, SLABS, n_keys - n0, lane);
@@ -393,7 +401,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       // and dP(i+1): P(i) and dS(i) live in the dP columns.
       for (int i = 0; i < ns && ok; ++i) {
         if (i + 1 < ns) {
-          if (!(ok = mbar_wait(s_free, i & 1, abort_flag, kErrGenDkdvMma))) break;
+          if (!(ok = warp_wait(s_free, i & 1, abort_flag, kErrGenDkdvMma))) break;
           tc_fence_after();
           if (!(ok = issue_s(i + 1))) break;
         }
@@ -430,19 +438,19 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       float bias_l = 0.f, bias_r = 0.f;
       if (BIAS) {
         ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table
-        build_table(bias, hk * pr.G + hg, pr.Hq, tab, threadIdx.x, 256);
+        copy_table(tab, tables, hk * pr.G + hg, bias, threadIdx.x, 256);
         ok = named_barrier_and(2, 256, ok);
         bias_l = tab[0];
-        bias_r = tab[table_size(bias) - 1];
+        bias_r = tab[table_last(bias)];
       }
       const int head_end = min(ns, (hg + 1) * nqb - st0);
       for (; ok && i < head_end; ++i) {
         const int qc = q_begin + (st0 + i - hg * nqb) * 128 + 64 * g;  // first query of this thread's columns
-        if (!(ok = mbar_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvCompute))) break;
+        if (!(ok = warp_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvCompute))) break;
         const float* lse_s = lse_smem(i) + 64 * g;
         const float* dl_s = lse_s + 128;
         float p[64];
-        if (!(ok = mbar_wait(s_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
+        if (!(ok = warp_wait(s_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
         tc_fence_after();
         bwd::tmem_ld64(t_s, p);
         tc_fence_before();
@@ -496,7 +504,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
             pk[e / 2 + 1] = pack_bf16x2(p[e + 2], p[e + 3]);
           }
         }
-        if (!(ok = mbar_wait(dp_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
+        if (!(ok = warp_wait(dp_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
         tc_fence_after();
         // dP(i) comes into registers half by half; its columns then take P(i) and dS(i)
         uint32_t dlo[32], dhi[32];
@@ -532,7 +540,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       }
     }
     const bool empty = ns <= 0;
-    const bool done = ok && (empty || mbar_wait(final_bar, 0, abort_flag, kErrGenDkdvCompute));
+    const bool done = ok && (empty || warp_wait(final_bar, 0, abort_flag, kErrGenDkdvCompute));
     tc_fence_after();
     if (n_split > 1) {
       const long long r = (static_cast<long long>(split) * pr.B * pr.Hkv + cw.bh) * pr.Sk + kg;
@@ -572,7 +580,7 @@ struct DqLayout {
   static constexpr int TAB_OFF = V_OFF + V_STAGES * TILE;
   // bias: table (fp32 by position), buckets by position, per-warp sums, diagonal scratch
   static constexpr int LUT_OFF = TAB_OFF + (kTableMax * 4 + 15) / 16 * 16;
-  static constexpr int SUM_OFF = LUT_OFF + ((2 * kMaxDistance + 2) * 2 + 15) / 16 * 16;
+  static constexpr int SUM_OFF = LUT_OFF + (2 * kMaxDistance + 8) * 2;
   static constexpr int DIAG_OFF = SUM_OFF + 8 * kMaxBuckets * 4;
   static constexpr int BAR_OFF = BIAS ? DIAG_OFF + 8 * 96 * 4 : TAB_OFF;
   // qd_ready, k_full[], k_empty[], v_full[3], v_empty[3], s_full, s_free, dp_full, ds_ready,
@@ -648,7 +656,9 @@ template <int D, bool CAUSAL, bool BIAS>
 __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     ffa_gen_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ Problem pr,
-                      const __grid_constant__ Bias bias, const View q, const View dout, const float* __restrict__ LSE,
+                      const __grid_constant__ Bias bias, const float* __restrict__ tables,
+                      const unsigned short* __restrict__ lut_g, const View q, const View dout,
+                      const float* __restrict__ LSE,
                       const float* __restrict__ DELTA, float* __restrict__ dq_part, float* __restrict__ bias_part,
                       int n_split, int group) {
   using L = DqLayout<D, BIAS>;
@@ -721,9 +731,9 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     tma_prefetch_desc(&tm_v);
   }
   if (BIAS && warp < 8) {
-    build_table(bias, h, pr.Hq, tab, threadIdx.x, 256);
-    for (int t = threadIdx.x; t <= bias.left + bias.right; t += 256)
-      lut[t] = static_cast<unsigned short>(bias.bucket(t - bias.left));
+    copy_table(tab, tables, h, bias, threadIdx.x, 256);
+    for (int t = threadIdx.x; t < lut_size(bias) / 2; t += 256)
+      reinterpret_cast<uint32_t*>(lut)[t] = reinterpret_cast<const uint32_t*>(lut_g)[t];
     for (int t = threadIdx.x; t < 8 * bias.buckets; t += 256) sums_all[t] = 0.f;
   }
   tc_fence_before();
@@ -770,7 +780,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         if (tail < 128 && n_keys < pr.Sk) zero_tail(tile, SLABS, tail, lane);
       };
       auto issue_s = [&](int j) -> bool {  // S_j = Q K_j^T  (Q from TMEM)
-        if (!mbar_wait(k_full(j % KS), (j / KS) & 1, abort_flag, kErrGenDqMma)) return false;
+        if (!warp_wait(k_full(j % KS), (j / KS) & 1, abort_flag, kErrGenDqMma)) return false;
         fix_tail(k_addr(j), j);
         tc_fence_after();
         const uint64_t kd = kmajor_desc(k_addr(j), 128, 0);
@@ -785,7 +795,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         return true;
       };
       auto issue_dp = [&](int j) -> bool {  // dP_j = dO V_j^T  (dO from TMEM)
-        if (!mbar_wait(v_full(j % VS), (j / VS) & 1, abort_flag, kErrGenDqMma)) return false;
+        if (!warp_wait(v_full(j % VS), (j / VS) & 1, abort_flag, kErrGenDqMma)) return false;
         fix_tail(v_addr(j), j);
         tc_fence_after();
         const uint64_t vd = kmajor_desc(v_addr(j), 128, 0);
@@ -801,7 +811,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         return true;
       };
       auto issue_g = [&](int j) -> bool {  // dQ += dS_j K_j  (dS_j packed in the dP columns)
-        if (!mbar_wait(ds_ready, j & 1, abort_flag, kErrGenDqMma)) return false;
+        if (!warp_wait(ds_ready, j & 1, abort_flag, kErrGenDqMma)) return false;
         tc_fence_after();
         const uint64_t kd = mnmajor_desc(k_addr(j), 128, 0);
         if (elect_one()) {
@@ -814,14 +824,14 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         __syncwarp();
         return true;
       };
-      bool ok = mbar_wait(qd_ready, 0, abort_flag, kErrGenDqMma);
+      bool ok = warp_wait(qd_ready, 0, abort_flag, kErrGenDqMma);
       tc_fence_after();
       if (ok && nk > 0) ok = issue_s(0) && issue_dp(0);
       // S(j+1) once the warpgroups hold S(j) in registers; dQ(j) once dS(j) is in the dP
       // columns; then dP(j+1) over them
       for (int j = 0; j < nk && ok; ++j) {
         if (j + 1 < nk) {
-          if (!(ok = mbar_wait(s_free, j & 1, abort_flag, kErrGenDqMma))) break;
+          if (!(ok = warp_wait(s_free, j & 1, abort_flag, kErrGenDqMma))) break;
           tc_fence_after();
           if (!(ok = issue_s(j + 1))) break;
         }
@@ -864,11 +874,11 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     float bias_l = 0.f, bias_r = 0.f, sum_l = 0.f, sum_r = 0.f;
     if (BIAS) {
       bias_l = tab[0];
-      bias_r = tab[table_size(bias) - 1];
+      bias_r = tab[table_last(bias)];
     }
     bool ok = true;
     for (int j = 0; j < nk; ++j) {
-      if (!(ok = mbar_wait(s_full, j & 1, abort_flag, kErrGenDqCompute))) break;
+      if (!(ok = warp_wait(s_full, j & 1, abort_flag, kErrGenDqCompute))) break;
       tc_fence_after();
       float p[64];
       bwd::tmem_ld64(t_s, p);
@@ -911,7 +921,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         p[e] = p0;
         p[e + 1] = p1;
       }
-      if (!(ok = mbar_wait(dp_full, j & 1, abort_flag, kErrGenDqCompute))) break;
+      if (!(ok = warp_wait(dp_full, j & 1, abort_flag, kErrGenDqCompute))) break;
       tc_fence_after();
       uint32_t dlo[32], dhi[32];
       tmem_ld32(t_dp, dlo);
@@ -956,7 +966,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       }
     }
     const bool empty = nk <= 0;
-    const bool done = ok && (empty || mbar_wait(final_bar, 0, abort_flag, kErrGenDqCompute));
+    const bool done = ok && (empty || warp_wait(final_bar, 0, abort_flag, kErrGenDqCompute));
     tc_fence_after();
     if (BIAS) {
 #pragma unroll

@@ -72,17 +72,32 @@ struct Bias {
   }
 };
 
-// The bias of one head by relative position, in shared memory: entry r + left + kPad for
-// r in [-left - kPad, right + kPad].  A tile of at most 128 x 128 scores that meets a
-// position in (-left, right) lies inside; the others have one bias for all their scores
-// (the first or the last entry).  Neighbouring lanes hold neighbouring positions, so a
-// warp reads 32 consecutive words: no bank conflicts.
+// The bias of one head by relative position: entry r + left + kPad for r in [-left - kPad,
+// right + kPad].  A tile of at most 128 x 128 scores that meets a position in (-left, right)
+// lies inside; the others have one bias for all their scores (the first or the last entry).
+// ffa_gen_table_kernel writes the tables of all heads once a call, and a CTA brings its
+// head's into shared memory with one bulk copy.  Neighbouring lanes read neighbouring
+// positions: no bank conflicts.
 constexpr int kPad = 256;
-constexpr int kTableMax = 2 * kMaxDistance + 2 * kPad + 1;
-__device__ __forceinline__ int table_size(const Bias& bias) { return bias.left + bias.right + 2 * kPad + 1; }
-__device__ __forceinline__ void build_table(const Bias& bias, int h, int Hq, float* tab, int tid, int n) {
-  const int size = table_size(bias);
-  for (int t = tid; t < size; t += n) tab[t] = bias.entry(bias.bucket(t - bias.left - kPad), h, Hq);
+constexpr int kTableMax = 2 * kMaxDistance + 2 * kPad + 4;
+// entries of a table, rounded up to whole 16-byte units
+__host__ __device__ __forceinline__ int table_size(const Bias& bias) {
+  return (bias.left + bias.right + 2 * kPad + 1 + 3) / 4 * 4;
+}
+__device__ __forceinline__ int table_last(const Bias& bias) { return bias.left + bias.right + 2 * kPad; }
+// Bucket by position, entry r + left, behind the tables (16-bit, whole 16-byte units).
+__host__ __device__ __forceinline__ int lut_size(const Bias& bias) { return (bias.left + bias.right + 1 + 7) / 8 * 8; }
+
+__global__ void __launch_bounds__(256)
+    ffa_gen_table_kernel(const __grid_constant__ Bias bias, float* __restrict__ tables,
+                         unsigned short* __restrict__ lut, int Hq) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int size = table_size(bias), t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= size) return;
+  const int r = t - bias.left - kPad, u = bias.bucket(r);
+  for (int h = blockIdx.y; h < Hq; h += gridDim.y) tables[static_cast<long long>(h) * size + t] = bias.entry(u, h, Hq);
+  if (lut != nullptr && blockIdx.y == 0 && r >= -bias.left && r + bias.left < lut_size(bias))
+    lut[r + bias.left] = static_cast<unsigned short>(u);
 }
 
 // A device tensor [B, H, S, D] with contiguous D, as the C ABI describes it.
@@ -112,13 +127,30 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// Zero the rows [row, 128) of a 128-row tile in shared memory (64-column slabs of 16 KB,
-// 128 bytes a row; the swizzle moves nothing between rows).  The whole warp calls it,
+// 32 lanes x 16 columns of 32-bit (tmem_ld32 with half the columns).
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// mbar_wait of a whole warp: true in all lanes or in none, so that the warp stays together
+// for the collective instructions that follow.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site));
+}
+
+// Zero the rows from `row` on of a tile of ROWS rows in shared memory (64-column slabs, 128
+// bytes a row; the swizzle moves nothing between rows).  The whole warp calls it,
 // before it issues MMAs that read the tile.  A probability of 0 does not undo a NaN in the
 // value it is multiplied with, so rows behind the last key must not reach an MMA.
+template <int ROWS = 128>
 __device__ __forceinline__ void zero_tail(uint32_t tile, int slabs, int row, int lane) {
   for (int sl = 0; sl < slabs; ++sl)
-    for (int o = row * 128 + lane * 16; o < 16384; o += 512) st_shared_v4(tile + sl * 16384 + o, 0u, 0u, 0u, 0u);
+    for (int o = row * 128 + lane * 16; o < ROWS * 128; o += 512) st_shared_v4(tile + sl * ROWS * 128 + o, 0u, 0u, 0u, 0u);
   fence_proxy_async_smem();
   __syncwarp();
 }
@@ -134,10 +166,10 @@ __device__ __forceinline__ void write_row32(float* dst, int c0, int D, const uin
                       __uint_as_float(r[4 * e + 2]) * mul, __uint_as_float(r[4 * e + 3]) * mul);
 }
 
-// 4-D tensor map over a [B, H, S, D] bf16 tensor: boxes of 64 columns x 128 rows, 128-byte
+// 4-D tensor map over a [B, H, S, D] bf16 tensor: boxes of 64 columns x `rows` rows, 128-byte
 // swizzle.  Columns from D on and rows from S on read as zero and are not written, so head
 // dims below the kernel's 64 or 128 need no padding in memory.
-int make_map(CUtensorMap* map, const View& t, int B, int H, int S, int D);
+int make_map(CUtensorMap* map, const View& t, int B, int H, int S, int D, int rows = 128);
 
 }  // namespace gen
 }  // namespace ffa

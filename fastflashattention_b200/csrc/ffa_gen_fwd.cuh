@@ -2,18 +2,24 @@
 //
 //   O_i = sum_j softmax_j(S_ij) v_j,   LSE_i = base-2 log-sum-exp of S_i (-inf: no key)
 //
-// The plan of the plain forward (ffa_fwd.cuh): a CTA owns 256 queries of one head as two
-// 128-row tiles; two softmax warpgroups (thread = row), a TMA warp and an MMA warp; S and O
-// in tensor memory, P handed back through it in two 64-key halves; the running max is
-// rescaled lazily.  What differs:
+// The plan of the plain forward (ffa_fwd.cuh): a softmax warpgroup for each 128-row query
+// tile (thread = row), a TMA warp and an MMA warp; S and O in tensor memory, P handed back
+// through it over S; the running max is rescaled lazily.  What differs:
 //   * operands are 4-D tensor maps, so any strides of batch, head and row do, and the key
 //     head of a query head is found by division;
-//   * the number of key tiles follows the sequence's own length and offset;
+//   * head dims up to 64: the softmax bounds the kernel, and one warp of a scheduler waits
+//     for its own loads and MMAs most of the time.  So a CTA has one tile and walks 64 keys
+//     a step: 128 columns of tensor memory and 80 registers a thread, four CTAs to an SM;
+//   * head dims up to 128: two tiles and 128 keys a step, one CTA to an SM;
+//   * the loop bodies are 64 scores long and used for every kind of tile.  Tiles that need a
+//     mask, a bias for each score or a negative scale are put right in tensor memory first
+//     (a rolled loop): a short launch spends much of its time fetching instructions that it
+//     runs for the first time;
 //   * a tile whose relative positions all lie in the last bucket of a side has one bias: it
-//     joins the row max and the exponent's constant for free.  Only tiles near the diagonal
-//     look the bias up, one shared-memory word for each score;
-//   * with few CTAs the keys are split: each split writes its normalised O in fp32 and its
-//     LSE, and ffa_gen_join_kernel weighs them (2^(LSE - max LSE)).
+//     joins the row max and the exponent's constant for free;
+//   * with few CTAs the keys are split in units of `per_split` steps (the same for all
+//     sequences, so that units of sequences of different lengths take the same time); each
+//     split writes its normalised O in fp32 and its LSE, and ffa_gen_join_kernel weighs them.
 #pragma once
 #include "ffa_fwd.cuh"
 #include "ffa_gen_common.cuh"
@@ -21,68 +27,92 @@
 namespace ffa {
 namespace gen {
 
-template <int D, bool BIAS>
+template <int D>
 struct FwdLayout {
-  static constexpr int TILE = 128 * D * 2;
-  static constexpr int STAGES = 3;
+  static constexpr int NT = D == 64 ? 1 : 2;        // 128-row tiles (softmax warpgroups) of a CTA
+  static constexpr int CTAS = D == 64 ? 4 : 1;      // CTAs of an SM
+  static constexpr int KEYS = D == 64 ? 64 : 128;   // keys of a step
+  static constexpr int HALVES = KEYS / 64;          // P is handed over 64 keys at a time
+  static constexpr int ROWS = 128 * NT;
+  // D = 128 moves registers between warpgroups (setmaxnreg), so the control warps fill one up
+  static constexpr int THREADS = D == 64 ? 192 : 384;
+  static constexpr int TMEM = D == 64 ? 128 : 512;  // S [0, KEYS) of each tile, then O
+  static constexpr uint32_t O_COL = KEYS * NT;
+  static constexpr int Q_TILE = 128 * D * 2, TILE = KEYS * D * 2;
+  static constexpr int STAGES = D == 64 ? 4 : 4;
   static constexpr int Q_OFF = 0;
-  static constexpr int KV_OFF = 2 * TILE;
-  static constexpr int TAB_OFF = KV_OFF + STAGES * TILE;
-  static constexpr int BAR_OFF = TAB_OFF + (BIAS ? (kTableMax * 4 + 15) / 16 * 16 : 0);
-  // q_full, kv_full[3], kv_empty[3], s_full[2], p_ready[2], o_final[2], drain, p_half[2], exp_done[2]
-  static constexpr int NBARS = 1 + 2 * STAGES + 2 + 2 + 2 + 1 + 2 + 2;
+  static constexpr int KV_OFF = NT * Q_TILE;
+  // q_full, kv_full[], kv_empty[], tab_full; for each tile s_full, o_final, p_ready[2]; drain
+  static constexpr int BAR_OFF = KV_OFF + STAGES * TILE;
+  static constexpr int NBARS = 1 + 2 * STAGES + 1 + 4 * NT + 1;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
-  static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
+  static constexpr int TAB_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
+  static int smem_bytes(const Bias& bias) { return TAB_OFF + (bias.table ? table_size(bias) * 4 : 0) + 1024; }
 };
 
-template <int D, bool CAUSAL, bool BIAS, int EMU = fwd::emu_pairs<D>(), bool SEQ = fwd::seq_turns<D>()>
-__global__ void __launch_bounds__(fwd::NTHREADS, 1)
+// Row max of 64 scores (16 chains of three-input maxima, then a short tree).
+__device__ __forceinline__ float row_max64(const uint32_t (&a)[32], const uint32_t (&b)[32]) {
+  float x[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u)
+    x[u] = fmax3(__uint_as_float(a[u]), __uint_as_float(a[16 + u]), __uint_as_float(b[u]));
+#pragma unroll
+  for (int u = 0; u < 16; u += 2) x[u] = fmax3(x[u], __uint_as_float(b[16 + u]), __uint_as_float(b[17 + u]));
+  const float y0 = fmax3(x[0], x[1], x[2]), y1 = fmax3(x[3], x[4], x[5]), y2 = fmax3(x[6], x[7], x[8]);
+  const float y3 = fmax3(x[9], x[10], x[11]), y4 = fmax3(x[12], x[13], x[14]);
+  return fmax3(fmax3(y0, y1, y2), fmax3(y3, y4, x[15]), y0);
+}
+
+template <int D, bool CAUSAL, bool BIAS, int EMU = fwd::emu_pairs<D>()>
+__global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
     ffa_gen_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
-                       const __grid_constant__ Problem pr, const __grid_constant__ Bias bias, float* __restrict__ LSE,
-                       float* __restrict__ part, float* __restrict__ part_lse, int n_split, int group) {
-  using L = FwdLayout<D, BIAS>;
-  constexpr int SLABS = D / 64, STAGES = L::STAGES;
+                       const __grid_constant__ Problem pr, const __grid_constant__ Bias bias,
+                       const float* __restrict__ tables, float* __restrict__ LSE, float* __restrict__ part,
+                       float* __restrict__ part_lse, int n_split, int per_split, int group) {
+  using L = FwdLayout<D>;
+  constexpr int SLABS = D / 64, STAGES = L::STAGES, NT = L::NT, KEYS = L::KEYS;
+  constexpr int PRODUCER = 4 * NT, MMA = 4 * NT + 1;  // warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const uint32_t bar0 = sbase + L::BAR_OFF;
   const uint32_t q_full = bar0;
-  auto kv_full = [&](int s) { return bar0 + 8 * (1 + s); };
-  auto kv_empty = [&](int s) { return bar0 + 8 * (1 + STAGES + s); };
-  auto s_full = [&](int i) { return bar0 + 8 * (1 + 2 * STAGES + i); };
-  auto p_ready = [&](int i) { return bar0 + 8 * (3 + 2 * STAGES + i); };
-  auto o_final = [&](int i) { return bar0 + 8 * (5 + 2 * STAGES + i); };
-  const uint32_t drain_bar = bar0 + 8 * (7 + 2 * STAGES);
-  auto p_half = [&](int i) { return bar0 + 8 * (8 + 2 * STAGES + i); };
-  auto exp_done = [&](int i) { return bar0 + 8 * (10 + 2 * STAGES + i); };
+  auto kv_full = [&](int n) { return bar0 + 8 * (1 + n % STAGES); };
+  auto kv_empty = [&](int n) { return bar0 + 8 * (1 + STAGES + n % STAGES); };
+  const uint32_t tab_full = bar0 + 8 * (1 + 2 * STAGES);
+  auto s_full = [&](int i) { return tab_full + 8 * (1 + 4 * i); };
+  auto o_final = [&](int i) { return tab_full + 8 * (2 + 4 * i); };
+  auto p_ready = [&](int i, int half) { return tab_full + 8 * (3 + 4 * i + half); };
+  const uint32_t drain_bar = tab_full + 8 * (1 + 4 * NT);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
-  float* tab = reinterpret_cast<float*>(smem + L::TAB_OFF);
+  const float* tab = reinterpret_cast<const float*>(smem + L::TAB_OFF);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // work: (block of 256 queries, split of the keys) of one (sequence, query head); under a
+  // work: (block of ROWS queries, split of the keys) of one (sequence, query head); under a
   // causal mask the last blocks have the most keys and come first
-  const int n_mblk = (pr.Sq + 255) / 256;
+  const int n_mblk = (pr.Sq + L::ROWS - 1) / L::ROWS;
   const CtaWork cw = cta_work(n_mblk * n_split, pr.B * pr.Hq, group);
   const int mblk = CAUSAL ? n_mblk - 1 - cw.rank / n_split : cw.rank / n_split;
   const int split = cw.rank % n_split;
   const int b = cw.bh / pr.Hq, h = cw.bh % pr.Hq, hk = h / pr.G;
-  const int m0 = mblk * 256;
+  const int m0 = mblk * L::ROWS;
   const int off = (CAUSAL || BIAS) ? pr.offset(b) : 0;
   const int n_keys = pr.keys(b, off, CAUSAL);
-  // key tiles [t0, t0 + nt_i) of query tile i in this split
-  auto tiles_of = [&](int mi) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int t0 = split * per_split;
+  // a split behind the sequence's last key leaves at once; the join counts the splits in the same way
+  if (split > 0 && t0 * KEYS >= n_keys) return;
+  // steps [t0, t0 + cnt_i) of query tile i in this split
+  auto steps_of = [&](int mi) {
     if (mi >= pr.Sq) return 0;
     const int end = CAUSAL ? min(n_keys, max(off + mi + 128, 0)) : n_keys;
-    return (end + 127) / 128;
+    return max(0, min((end + KEYS - 1) / KEYS - t0, per_split));
   };
-  const int all0 = tiles_of(m0), all1 = tiles_of(m0 + 128);
-  const int per_split = (max(all0, all1) + n_split - 1) / n_split;
-  const int t0 = split * per_split;
-  const int nt0 = max(0, min(all0 - t0, per_split)), nt1 = max(0, min(all1 - t0, per_split));
-  const int n_kv = max(nt0, nt1);
+  const int cnt0 = steps_of(m0), cnt1 = NT == 1 ? 0 : steps_of(m0 + 128);
+  const int n_kv = max(cnt0, cnt1);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -90,337 +120,295 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1)
       mbar_init(kv_full(s), 1);
       mbar_init(kv_empty(s), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(tab_full, 1);
+    for (int i = 0; i < NT; ++i) {
       mbar_init(s_full(i), 1);
-      mbar_init(p_ready(i), 128);
       mbar_init(o_final(i), 1);
-      mbar_init(p_half(i), 128);
-      mbar_init(exp_done(i), 128);
+      mbar_init(p_ready(i, 0), 128);
+      mbar_init(p_ready(i, 1), 128);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == fwd::MMA_WARP) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == MMA) {
+    tmem_alloc(smem_u32(tmem_slot), L::TMEM);
     tmem_relinquish();
   }
-  if (warp == fwd::PRODUCER_WARP && lane == 0) {
+  if (warp == PRODUCER && lane == 0) {
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (BIAS && warp < 8) build_table(bias, h, pr.Hq, tab, threadIdx.x, 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
-    setmaxnreg_dec<fwd::REGS_CONTROL>();
-    if (warp == fwd::PRODUCER_WARP) {
+  if (warp >= 4 * NT) {
+    if constexpr (D == 128) setmaxnreg_dec<fwd::REGS_CONTROL>();
+    if (warp == PRODUCER) {
       // ---------------------------------------------------------------- producer
       if (lane == 0 && n_kv > 0) {
         const uint64_t keep = policy_evict_last();
-        mbar_arrive_expect_tx(q_full, 2 * L::TILE);
-        for (int i = 0; i < 2; ++i)
+        mbar_arrive_expect_tx(q_full, NT * L::Q_TILE);
+        for (int i = 0; i < NT; ++i)
           for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(sbase + L::Q_OFF + i * L::TILE + sl * 16384, &tm_q, q_full, sl * 64, m0 + i * 128, h, b, keep);
-        int issued = 0;
-        for (; issued < 2 * n_kv; ++issued) {
-          const int s = issued % STAGES;
-          if (!mbar_wait(kv_empty(s), ((issued / STAGES) & 1) ^ 1, abort_flag, kErrGenFwdProducer)) break;
-          mbar_arrive_expect_tx(kv_full(s), L::TILE);
-          const CUtensorMap* tm = (issued & 1) ? &tm_v : &tm_k;
+            tma_load_4d(sbase + L::Q_OFF + i * L::Q_TILE + sl * 16384, &tm_q, q_full, sl * 64, m0 + i * 128, h, b, keep);
+        int n = 0;
+        for (; n < 2 * n_kv; ++n) {
+          if (!mbar_wait(kv_empty(n), ((n / STAGES) & 1) ^ 1, abort_flag, kErrGenFwdProducer)) break;
+          mbar_arrive_expect_tx(kv_full(n), L::TILE);
           for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(sbase + L::KV_OFF + s * L::TILE + sl * 16384, tm, kv_full(s), sl * 64,
-                        (t0 + (issued >> 1)) * 128, hk, b, keep);
+            tma_load_4d(sbase + L::KV_OFF + (n % STAGES) * L::TILE + sl * (KEYS * 128), (n & 1) ? &tm_v : &tm_k,
+                        kv_full(n), sl * 64, (t0 + (n >> 1)) * KEYS, hk, b, keep);
+          if (BIAS && n == 0) {
+            // the table, once its kernel has written it (this one may start before that ends)
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            const int bytes = table_size(bias) * 4;
+            mbar_arrive_expect_tx(tab_full, bytes);
+            bulk_load(smem_u32(tab), tables + static_cast<long long>(h) * table_size(bias), bytes, tab_full);
+          }
         }
         if (*abort_flag) {
           // let in-flight copies land before the CTA's shared memory goes away
-          for (int it = max(0, issued - STAGES); it < issued; ++it)
-            mbar_wait_drain(kv_full(it % STAGES), (it / STAGES) & 1);
+          for (int x = max(0, n - STAGES); x < n; ++x) mbar_wait_drain(kv_full(x), (x / STAGES) & 1);
           mbar_wait_drain(q_full, 0);
+          if (BIAS && n > 0) mbar_wait_drain(tab_full, 0);
         }
       }
-    } else if (warp == fwd::MMA_WARP) {
+    } else if (warp == MMA) {
       // ---------------------------------------------------------------- MMA issuer
-      constexpr uint32_t IDESC_QK = idesc_bf16(128, 128, false, false);
+      constexpr uint32_t IDESC_QK = idesc_bf16(128, KEYS, false, false);
       constexpr uint32_t IDESC_PV = idesc_bf16(128, D, false, true);
-      bool ok = n_kv > 0 && mbar_wait(q_full, 0, abort_flag, kErrGenFwdMma);
-      int it = 0;
+      bool ok = n_kv > 0 && warp_wait(q_full, 0, abort_flag, kErrGenFwdMma);
       auto commit = [&](uint32_t bar) {
         if (elect_one()) mma_commit(bar);
         __syncwarp();
       };
       auto kv_addr = [&](int n) { return sbase + L::KV_OFF + (n % STAGES) * L::TILE; };
       auto kv_wait = [&](int n) {
-        const bool r = mbar_wait(kv_full(n % STAGES), (n / STAGES) & 1, abort_flag, kErrGenFwdMma);
+        const bool r = warp_wait(kv_full(n), (n / STAGES) & 1, abort_flag, kErrGenFwdMma);
         tc_fence_after();
         return r;
       };
-      const uint64_t qdesc0 = kmajor_desc(sbase + L::Q_OFF, 128, 0);
-      const uint64_t qdesc1 = kmajor_desc(sbase + L::Q_OFF + L::TILE, 128, 0);
-      auto issue_qk = [&](int i, uint32_t k_addr) {
-        const uint64_t qd = i ? qdesc1 : qdesc0;
-        const uint64_t kd = kmajor_desc(k_addr, 128, 0);
-        const uint32_t d = tmem + i * 128;
+      auto issue_qk = [&](int i, int n) {  // S_i = Q_i K^T
+        const uint64_t qd = kmajor_desc(sbase + L::Q_OFF + i * L::Q_TILE, 128, 0);
+        const uint64_t kd = kmajor_desc(kv_addr(n), KEYS, 0);
+        const uint32_t d = tmem + i * KEYS;
         if (elect_one()) {
           mma_ss(d, qd, kd, IDESC_QK, 0u);
 #pragma unroll
           for (int ks = 1; ks < D / 16; ++ks)
-            mma_ss_acc(d, qd + kmajor_step(128, ks), kd + kmajor_step(128, ks), IDESC_QK);
+            mma_ss_acc(d, qd + kmajor_step(128, ks), kd + kmajor_step(KEYS, ks), IDESC_QK);
           mma_commit(s_full(i));
         }
         __syncwarp();
       };
-      // K-steps [k0, k1) of O_i += P_i V_j (16 keys = 8 TMEM columns of packed P each)
-      auto issue_pv = [&](int i, uint32_t v_addr, int j, int k0, int k1) {
-        const uint64_t vd = mnmajor_desc(v_addr, 128, 0);
-        const uint32_t d = tmem + 256 + i * 128, a = tmem + i * 128;
-        if (elect_one()) {
-          for (int ks = k0; ks < k1; ++ks) {
-            if (ks == 0)
-              mma_ts(d, a, vd, IDESC_PV, j > 0 ? 1u : 0u);
-            else
-              mma_ts_acc(d, a + ks * 8, vd + mnmajor_step(ks), IDESC_PV);
+      auto issue_pv = [&](int i, int j, int n) -> bool {  // O_i (+)= P_i V_j, as P comes
+        const uint64_t vd = mnmajor_desc(kv_addr(n), KEYS, 0);
+        const uint32_t d = tmem + L::O_COL + i * 128, a = tmem + i * KEYS;
+#pragma unroll 1
+        for (int half = 0; half < L::HALVES; ++half) {
+          if (!warp_wait(p_ready(i, half), j & 1, abort_flag, kErrGenFwdMma)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vh = vd + mnmajor_step(4 * half);
+            mma_ts(d, a + 32 * half, vh, IDESC_PV, (j > 0 || half > 0) ? 1u : 0u);
+#pragma unroll
+            for (int ks = 1; ks < 4; ++ks) mma_ts_acc(d, a + 32 * half + ks * 8, vh + mnmajor_step(ks), IDESC_PV);
           }
+          __syncwarp();
         }
-        __syncwarp();
-      };
-      auto issue_pv_tile = [&](int i, uint32_t v_addr, int j) -> bool {
-        if (!mbar_wait(p_half(i), j & 1, abort_flag, kErrGenFwdMma)) return false;
-        tc_fence_after();
-        issue_pv(i, v_addr, j, 0, 4);
-        if (!mbar_wait(p_ready(i), j & 1, abort_flag, kErrGenFwdMma)) return false;
-        tc_fence_after();
-        issue_pv(i, v_addr, j, 4, 8);
         return true;
       };
-      if (ok && (ok = kv_wait(it))) {
-        const uint32_t k_addr = kv_addr(it);
-        if (nt0 > 0) issue_qk(0, k_addr);
-        if (nt1 > 0) issue_qk(1, k_addr);
-        commit(kv_empty(it % STAGES));
-        ++it;
+      if (ok && (ok = kv_wait(0))) {
+        if (cnt0 > 0) issue_qk(0, 0);
+        if (NT > 1 && cnt1 > 0) issue_qk(1, 0);
+        commit(kv_empty(0));
       }
       for (int j = 0; j < n_kv && ok; ++j) {
-        const int sv = it % STAGES;
-        if (!(ok = kv_wait(it))) break;
-        const uint32_t v_addr = kv_addr(it);
-        ++it;
-        const int tail = n_keys - (t0 + j) * 128;
-        if (tail < 128 && n_keys < pr.Sk) zero_tail(v_addr, SLABS, tail, lane);
-        const bool next = (j + 1 < n_kv);
-        uint32_t k_addr = 0;
-        // tile 0: O0 += P0 V_j, then S0 = Q0 K_{j+1}^T
-        if (j < nt0 && !(ok = issue_pv_tile(0, v_addr, j))) break;
-        if (next) {
-          if (!(ok = kv_wait(it))) break;
-          k_addr = kv_addr(it);
-          if (j + 1 < nt0) issue_qk(0, k_addr);
+        const int nv = 2 * j + 1, nk = 2 * j + 2;  // V_j and K_{j+1}
+        if (!(ok = kv_wait(nv))) break;
+        const int tail = n_keys - (t0 + j) * KEYS;
+        if (tail < KEYS && n_keys < pr.Sk) zero_tail<KEYS>(kv_addr(nv), SLABS, tail, lane);
+        const bool next = j + 1 < n_kv;
+        // tile by tile: O_i += P_i V_j, then S_i = Q_i K_{j+1}^T over P_i
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const int cnt = i ? cnt1 : cnt0;
+          if (j < cnt && !(ok = issue_pv(i, j, nv))) break;
+          if (next) {
+            if (i == 0 && !(ok = kv_wait(nk))) break;
+            if (j + 1 < cnt) issue_qk(i, nk);
+          }
         }
-        // tile 1: O1 += P1 V_j, then S1 = Q1 K_{j+1}^T
-        if (j < nt1 && !(ok = issue_pv_tile(1, v_addr, j))) break;
-        commit(kv_empty(sv));
-        if (next) {
-          if (j + 1 < nt1) issue_qk(1, k_addr);
-          commit(kv_empty(it % STAGES));
-          ++it;
-        }
+        if (!ok) break;
+        commit(kv_empty(nv));
+        if (next) commit(kv_empty(nk));
       }
-      if (ok && nt0 > 0) commit(o_final(0));
-      if (ok && nt1 > 0) commit(o_final(1));
+      if (ok && cnt0 > 0) commit(o_final(0));
+      if (NT > 1 && ok && cnt1 > 0) commit(o_final(1));
       // every issued MMA has finished before TMEM is released
       commit(drain_bar);
       mbar_wait_drain(drain_bar, 0);
     }
   } else {
-    setmaxnreg_inc<fwd::REGS_SOFTMAX>();
+    if constexpr (D == 128) setmaxnreg_inc<fwd::REGS_SOFTMAX>();
     // ------------------------------------------------------------------ softmax
-    const int i = warp >> 2;  // tile
+    const int i = NT == 1 ? 0 : warp >> 2;  // tile
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_off + i * 128;
-    const uint32_t t_o = tmem + lane_off + 256 + i * 128;
+    const uint32_t t_s = tmem + lane_off + i * KEYS;
+    const uint32_t t_o = tmem + lane_off + L::O_COL + i * 128;
     const int mi = m0 + i * 128;
     const int grow = mi + row;
     const int wrow = mi + (warp & 3) * 32;  // the warp's first row
-    const int nt = i ? nt1 : nt0;
-    const int nt_other = i ? nt0 : nt1;
+    const int cnt = i ? cnt1 : cnt0;
     // last key that this row sees
     const int lim = CAUSAL ? min(n_keys - 1, grow + off) : n_keys - 1;
     const float scale_log2 = pr.scale_log2;
-    float bias_l = 0.f, bias_r = 0.f;
-    if (BIAS) {
-      bias_l = tab[0];
-      bias_r = tab[table_size(bias) - 1];
-    }
     bool ok = true;
+    if (BIAS && cnt > 0) ok = warp_wait(tab_full, 0, abort_flag, kErrGenFwdSoftmax);
     float m_used = -INFINITY;
     float l = 0.f;
-    for (int j = 0; j < nt; ++j) {
-      if (!(ok = mbar_wait(s_full(i), j & 1, abort_flag, kErrGenFwdSoftmax))) break;
+    for (int j = 0; ok && j < cnt; ++j) {
+      if (!(ok = warp_wait(s_full(i), j & 1, abort_flag, kErrGenFwdSoftmax))) break;
       tc_fence_after();
-      float s[128];
-      {
-        uint32_t r[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, r[c]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[c * 32 + e] = __uint_as_float(r[c][e]);
-      }
-      const int n0 = (t0 + j) * 128;
-      bool masked = (n0 + 128 > n_keys) || (CAUSAL && n0 + 127 > wrow + off);
+      const int n0 = (t0 + j) * KEYS;
+      const bool masked = (n0 + KEYS > n_keys) || (CAUSAL && n0 + KEYS - 1 > wrow + off);
       // relative positions of the warp's part of the tile: all in a last bucket, or looked up
       bool near = false;
-      float fb = 0.f;
+      float fb = 0.f;  // the tile's bias
       if (BIAS) {
-        const int r_min = n0 - (off + wrow + 31), r_max = n0 + 127 - (off + wrow);
+        const int r_min = n0 - (off + wrow + 31), r_max = n0 + KEYS - 1 - (off + wrow);
         near = r_min < bias.right && r_max > -bias.left;
-        fb = r_min >= bias.right ? bias_r : bias_l;
-        masked |= !near && fb == -INFINITY;  // an infinite constant must not meet the polynomial exp2
+        fb = tab[r_min >= bias.right ? table_last(bias) : 0];
       }
-      const bool adjusted = masked || near;
-      float tmax;
-      if (adjusted) {
-        if (BIAS && near) {
-          const float* tp = tab + (n0 - off - grow + bias.left + kPad);
+      float c = scale_log2;  // what the scores still have to be multiplied with
+      if (masked || near || scale_log2 < 0.f) {
+        const float* tp = tab + (n0 - off - grow + bias.left + kPad);
+#pragma unroll 1
+        for (int x = 0; x < KEYS; x += 32) {
+          uint32_t r[32];
+          tmem_ld32(t_s + x, r);
+          tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = fmaf(s[c], scale_log2, tp[c]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = BIAS ? fmaf(s[c], scale_log2, fb) : s[c] * scale_log2;
+          for (int e = 0; e < 32; ++e) {
+            float y = __uint_as_float(r[e]) * scale_log2;
+            if (BIAS) y += near ? tp[x + e] : fb;
+            r[e] = __float_as_uint(n0 + x + e > lim ? -INFINITY : y);
+          }
+          tmem_st32(t_s + x, r);
         }
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = (n0 + c > lim) ? -INFINITY : s[c];
-        }
-        tmax = row_max128(s);
-      } else if (scale_log2 >= 0.f) {
-        tmax = BIAS ? fmaf(row_max128(s), scale_log2, fb) : row_max128(s) * scale_log2;
-      } else {
-        float a = s[0];
-#pragma unroll
-        for (int c = 1; c < 128; ++c) a = fminf(a, s[c]);
-        tmax = fmaf(a, scale_log2, fb);
+        tmem_st_wait();
+        c = 1.f;
+        fb = 0.f;
       }
+      uint32_t sa[32], sb[32];  // 64 scores
+      float tmax = -INFINITY;
+#pragma unroll 1
+      for (int hf = L::HALVES - 1; hf >= 0; --hf) {
+        tmem_ld32(t_s + 64 * hf, sa);
+        tmem_ld32(t_s + 64 * hf + 32, sb);
+        tmem_ld_wait();
+        tmax = fmaxf(tmax, row_max64(sa, sb));
+      }
+      tmax = BIAS ? fmaf(tmax, c, fb) : tmax * c;
       const float m_new = fmaxf(m_used, tmax);
       const bool need = m_new > m_used + fwd::RESCALE_THRESHOLD;
       if (__any_sync(0xffffffffu, need)) {
         const float m_safe = (m_new == -INFINITY) ? 0.f : m_new;
         const float alpha = fast_exp2(m_used - m_safe);
         if (j > 0) {
-          // O_i(j-1) is complete: S_i(j) was committed after P_i(j-1) V_{j-1}.
+          // O_i(j-1) is complete: S_i(j) was committed after P_i(j-1) V_{j-1}
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld32(t_o + c * 32, r);
+          for (int x = 0; x < D; x += 16) {
+            uint32_t r[16];
+            tmem_ld16(t_o + x, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-            tmem_st32(t_o + c * 32, r);
+            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+            tmem_st16(t_o + x, r);
           }
         }
         l *= alpha;
         m_used = m_new;
       }
       const float m_safe = (m_used == -INFINITY) ? 0.f : m_used;
-      uint32_t p[2][32];
-      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       const float shift = BIAS ? fb - m_safe : -m_safe;
-      const float2 c2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(shift, shift);
-      // Column pairs [hf*32, hf*32+32) -> p[hf] -> TMEM columns [hf*32, hf*32+32) of S_i.
-      auto half = [&](const int hf) {
-        if (adjusted) {
-#pragma unroll
-          for (int u = 0; u < 32; ++u) {
-            const int c = hf * 32 + u;
-            const float p0 = fast_exp2(s[2 * c] - m_safe);
-            const float p1 = fast_exp2(s[2 * c + 1] - m_safe);
-            sum2[u & 1] = add2(sum2[u & 1], make_float2(p0, p1));
-            p[hf][u] = pack_bf16x2(p0, p1);
-          }
-        } else {
-          // EMU of every 8 column pairs take the FMA-pipe exp2, the rest MUFU.EX2
-#pragma unroll
-          for (int u = 0; u < 32; ++u) {
-            const int c = hf * 32 + u;
-            const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), c2, nm2);
-            float p0, p1;
-            if ((c & 7) < EMU) {
-              const float2 e2 = exp2_fma2(x);
-              p0 = e2.x;
-              p1 = e2.y;
-            } else {
-              p0 = fast_exp2(x.x);
-              p1 = fast_exp2(x.y);
-            }
-            sum2[u & 1] = add2(sum2[u & 1], make_float2(p0, p1));
-            p[hf][u] = pack_bf16x2(p0, p1);
-          }
+      const float2 c2 = make_float2(c, c), nm2 = make_float2(shift, shift);
+      // 64 scores -> P -> 32 columns over S (the first half's scores are still in registers)
+#pragma unroll 1
+      for (int hf = 0; hf < L::HALVES; ++hf) {
+        if (hf > 0) {
+          tmem_ld32(t_s + 64 * hf, sa);
+          tmem_ld32(t_s + 64 * hf + 32, sb);
+          tmem_ld_wait();
         }
-        if (SEQ && hf == 1) mbar_arrive(exp_done(i));
-        tmem_st32(t_s + 32 * hf, p[hf]);
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int u = 0; u < 32; ++u) {
+          const uint32_t* src = u < 16 ? sa : sb;
+          const int e = 2 * (u & 15);
+          const float2 x = fma2(make_float2(__uint_as_float(src[e]), __uint_as_float(src[e + 1])), c2, nm2);
+          float p0, p1;
+          if ((u & 7) < EMU) {  // EMU of every 8 column pairs on the FMA pipe
+            const float2 e2 = exp2_fma2(x);
+            p0 = e2.x;
+            p1 = e2.y;
+          } else {
+            p0 = fast_exp2(x.x);
+            p1 = fast_exp2(x.y);
+          }
+          sum2[u & 1] = add2(sum2[u & 1], make_float2(p0, p1));
+          sa[u] = pack_bf16x2(p0, p1);  // pair u replaces a score that is already used
+        }
+        const float2 sv = add2(sum2[0], sum2[1]);
+        l += sv.x + sv.y;
+        tmem_st32(t_s + 32 * hf, sa);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(hf == 0 ? p_half(i) : p_ready(i));
-      };
-      if (SEQ) {
-        // take turns with the other warpgroup: wait for its exponentials of step j (tile 1)
-        // or j-1 (tile 0), when it has such a step
-        const int oj = i ? j : j - 1;
-        if (oj >= 0 && oj < nt_other && !(ok = mbar_wait(exp_done(i ^ 1), oj & 1, abort_flag, kErrGenFwdSoftmax)))
-          break;
+        mbar_arrive(p_ready(i, hf));
       }
-      half(0);
-      half(1);
-      const float2 sv = add2(sum2[0], sum2[1]);
-      l += sv.x + sv.y;
     }
-    // Epilogue.  Every thread of the warpgroup reaches the barrier, finished or not.  A tile
-    // that saw no key writes zeros.
-    // (its Q tile, where the zeros are staged, may still be on its way when the other tile has keys)
-    const bool done = ok && (n_kv == 0 || mbar_wait(nt > 0 ? o_final(i) : q_full, 0, abort_flag, kErrGenFwdSoftmax));
-    const bool valid = done && grow < pr.Sq;
-    const float inv_l = (l == 0.f) ? 0.f : 1.f / l;
-    const float lse = (l == 0.f) ? -INFINITY : m_used + __log2f(l);
+    // Epilogue.  Every thread of the warpgroup reaches the barrier, finished or not.  A row
+    // without keys (no max) is 0: the sum holds what the polynomial makes of 2^-inf, and
+    // tensor memory may hold anything.  Its Q tile, where the output is staged, may still be
+    // on its way when the other tile has keys.
+    const bool done = ok && (n_kv == 0 || warp_wait(cnt > 0 ? o_final(i) : q_full, 0, abort_flag, kErrGenFwdSoftmax));
+    tc_fence_after();
+    const bool valid = done && grow < pr.Sq, none = m_used == -INFINITY;
+    const float inv_l = none ? 0.f : 1.f / l;
+    const float lse = none ? -INFINITY : m_used + __log2f(l);
+    const uint32_t o_tile = sbase + L::Q_OFF + i * L::Q_TILE;
     const long long ridx = static_cast<long long>(b * pr.Hq + h) * pr.Sq + grow;
-    const uint32_t o_tile = sbase + L::Q_OFF + i * L::TILE;
-    if (n_split > 1) {
-      const long long idx = static_cast<long long>(split) * pr.B * pr.Hq * pr.Sq + ridx;
-      if (valid) part_lse[idx] = lse;
-      if (done && nt > 0) {
-        tc_fence_after();
+    const long long prow = static_cast<long long>(split) * pr.B * pr.Hq * pr.Sq + ridx;
+    if (valid) {
+      if (n_split > 1)
+        part_lse[prow] = lse;
+      else if (LSE != nullptr)
+        LSE[ridx] = lse;
+    }
+    if (done) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(t_o + c * 32, r);
+      for (int x = 0; x < D; x += 32) {
+        uint32_t r[32];
+        if (cnt > 0) {
+          tmem_ld32(t_o + x, r);
           tmem_ld_wait();
-          if (valid && l != 0.f) write_row32(part + idx * pr.D, 32 * c, pr.D, r, inv_l);
         }
-      }
-    } else {
-      if (done) {
-        tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t r[32];
-          if (nt > 0) {
-            tmem_ld32(t_o + c * 32, r);
-            tmem_ld_wait();
-          }
-          if (l == 0.f) {  // no key: tensor memory may hold anything
+        if (none) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = 0u;
-          }
-          stage_row32_sw128(o_tile, row, 32 * c, r, inv_l);
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
         }
-        if (LSE != nullptr && valid) LSE[ridx] = lse;
+        if (n_split == 1)
+          stage_row32_sw128(o_tile, row, x, r, inv_l);
+        else if (valid && !none)
+          write_row32(part + prow * pr.D, x, pr.D, r, inv_l);
       }
+    }
+    if (n_split == 1) {
       // the Q tile is free once every MMA has finished; the store leaves out rows from Sq on
       fence_proxy_async_smem();
       const bool store = named_barrier_and(1 + i, 128, done);
@@ -435,10 +423,56 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == fwd::MMA_WARP) {
+  if (warp == MMA) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, L::TMEM);
   }
+}
+
+// Join the splits of a row: O = sum_s w_s O_s / sum_s w_s, w_s = 2^(LSE_s - max LSE).  One
+// warp a row, four columns a lane.  A sequence has as many splits as its keys fill; a split
+// whose keys the row does not see (LSE = -inf) is not read.
+__global__ void __launch_bounds__(128)
+    ffa_gen_join_kernel(const __grid_constant__ Problem pr, const float* __restrict__ part,
+                        const float* __restrict__ part_lse, const View o, float* __restrict__ LSE, int keys_per_split,
+                        int causal) {
+  const int lane = threadIdx.x & 31;
+  const long long rows = static_cast<long long>(pr.B) * pr.Hq * pr.Sq;
+  const long long r = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int bh = static_cast<int>(r / pr.Sq), t = static_cast<int>(r % pr.Sq);
+  const int b = bh / pr.Hq, h = bh % pr.Hq;
+  const int n_keys = pr.keys(b, causal ? pr.offset(b) : 0, causal);
+  const int n = max(1, (n_keys + keys_per_split - 1) / keys_per_split);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits have written
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, part_lse[s * rows + r]);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  float total = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int c = lane * 4;
+  if (m > -INFINITY) {
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float lse = part_lse[s * rows + r];
+      const float w = exp2f(lse - m);
+      total += w;
+      if (c < pr.D && lse > -INFINITY) {
+        const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + r) * pr.D + c);
+        a.x = fmaf(w, x.x, a.x);
+        a.y = fmaf(w, x.y, a.y);
+        a.z = fmaf(w, x.z, a.z);
+        a.w = fmaf(w, x.w, a.w);
+      }
+    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  if (c < pr.D) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + c;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+  }
+  if (lane == 0 && LSE != nullptr) LSE[r] = total == 0.f ? -INFINITY : m + __log2f(total);
 }
 
 }  // namespace gen

@@ -2,29 +2,23 @@
 // one or a few tokens over a cache or an encoder's states.
 //
 // The work is one pass over K and V, so the kernel is bound by HBM.  The G * Sq query rows
-// that share a key head (row r = g * Sq + t) form tiles of 16 MT rows, the M of mma.sync
+// that share a key head (row r = g * Sq + t) form items of 16 MT rows, the M of mma.sync
 // m16n8k16; the tensor cores' rate does not matter here, and a 128-row tcgen05 tile would
-// be empty.  A CTA of four warps takes one row tile and one split of the keys:
-//   * stages of 64 keys (K and V) come through a cp.async ring, 16 bytes a copy, zero-filled
-//     behind the last key (which also keeps what a cache holds there out of the products);
-//   * each warp takes 16 keys of a stage and keeps its own running max, sum and O
-//     (registers); the four are joined in shared memory at the end;
-//   * splits write their normalised O (fp32) and LSE; ffa_gen_join_kernel weighs them.
+// be empty.  Two CTAs to an SM, each a TMA warp and four warps that compute:
+//   * all keys of all items, laid end to end, are cut into equal shares (Work), one for each
+//     CTA, whatever the lengths of the sequences are.  The TMA warp walks through its share
+//     without a stop: HBM sees no gaps between items;
+//   * each warp takes 16 rows and a quarter of a tile's keys, and keeps its own running max,
+//     sum and O (registers); four warps are joined in shared memory at the end of a segment.  ROWS8: at
+//     most 8 rows, and the softmax of the other 8 is left out;
+//   * an item that several CTAs share is joined by ffa_gen_step_join_kernel, launched beside
+//     the last CTAs (programmatic dependent launch), which it waits for.
 #pragma once
 #include "ffa_gen_common.cuh"
 
 namespace ffa {
 namespace gen {
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -45,21 +39,136 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D, int MT>
-struct StepLayout {
-  static constexpr int KEYS = 64;  // keys of a stage, 16 for each warp
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int TILE = KEYS * D * 2;
-  static constexpr int ROWS = 16 * MT;
-  static constexpr int RING = STAGES * 2 * TILE;
-  // the join of the four warps reuses the ring: O [4][ROWS][D] fp32
-  static_assert(4 * ROWS * D * 4 <= RING, "the warps' results fit in the ring");
-  static constexpr int ML_OFF = RING;                       // max and sum [4][ROWS] each
-  static constexpr int LUT_OFF = ML_OFF + 2 * 4 * ROWS * 4; // bias: bucket by position, then entries
-  // bytes of the bias part for `heads` heads
-  static int bias_bytes(const Bias& bias, int heads) {
-    return (bias.left + bias.right + 2) / 2 * 4 + bias.buckets * heads * 4;
+// ------------------------------------------------------------------------------------
+// Work of a CTA
+// ------------------------------------------------------------------------------------
+// Items: `per_seq` for each sequence (key heads times row tiles), all with as many tiles of
+// KEYS keys as the sequence has, at least one (zeros have to be written too).  CTA c of n
+// gets the tiles [U c / n, U (c + 1) / n) of all U.  An item that crosses from one CTA into
+// the next ones is written in parts, in fp32, normalised, with its LSE: by the CTA in which
+// it starts in that CTA's slot 1, by the others in their slot 0.  `single`: one item a CTA.
+struct Segment {
+  int b, item;    // sequence, item of the sequence
+  int keys, off;  // the sequence's visible keys and offset
+  int t0, nt;     // first tile and number of tiles
+  int tiles;      // tiles of the whole item; 0: there is no segment, the CTA is done
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && nt == tiles; }
+};
+// What the join needs of an item that a CTA starts and others finish (parts = 0: none).
+struct JoinEntry {
+  int b, item, parts, pad;
+};
+
+// One thread walks through the CTA's segments (start() is for its whole warp).
+template <bool CAUSAL, bool OFFSETS>
+struct Work {
+  long long left, total, end;  // tiles left to the CTA, all tiles, the tile behind the last segment
+  int b, item, t, keys, off, tiles;
+
+  __device__ __forceinline__ static int tiles_of(int keys, int tile) { return max(1, (keys + tile - 1) / tile); }
+  __device__ __forceinline__ void enter(const Problem& pr, int seq, int tile) {
+    b = seq;
+    off = OFFSETS ? pr.offset(seq) : 0;
+    keys = pr.keys(seq, off, CAUSAL);
+    tiles = tiles_of(keys, tile);
   }
+  __device__ void start(const Problem& pr, int per_seq, int tile, bool single) {
+    if (single) {
+      enter(pr, blockIdx.x / per_seq, tile);
+      item = blockIdx.x % per_seq;
+      t = 0;
+      left = total = tiles;
+      end = 0;
+      return;
+    }
+    // tiles of each sequence: a warp takes 32 sequences at a time
+    const int lane = threadIdx.x & 31;
+    auto seq_tiles = [&](int seq) -> long long {
+      if (seq >= pr.B) return 0;
+      const int o = OFFSETS ? pr.offset(seq) : 0;
+      return static_cast<long long>(per_seq) * tiles_of(pr.keys(seq, o, CAUSAL), tile);
+    };
+    total = 0;
+    for (int s = lane; s < pr.B; s += 32) total += seq_tiles(s);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    end = total * blockIdx.x / gridDim.x;
+    left = total * (blockIdx.x + 1LL) / gridDim.x - end;
+    long long before = 0;  // tiles of the sequences before the chunk
+    for (int s0 = 0; s0 < pr.B; s0 += 32) {
+      const long long own = seq_tiles(s0 + lane);
+      long long sum = own;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, sum, x);
+        if (lane >= x) sum += y;
+      }
+      const uint32_t behind = __ballot_sync(0xffffffffu, before + sum > end);
+      if (behind) {
+        const int l = __ffs(behind) - 1;
+        const long long rest = end - before - __shfl_sync(0xffffffffu, sum - own, l);  // tile within the sequence
+        enter(pr, s0 + l, tile);
+        item = static_cast<int>(rest / tiles);
+        t = static_cast<int>(rest % tiles);
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  // The next segment.  Notes in `entry` the item that this CTA starts and others finish.
+  __device__ void next(const Problem& pr, int per_seq, int tile, Segment& s, JoinEntry& entry) {
+    s.tiles = 0;
+    if (left <= 0) return;
+    s.b = b;
+    s.item = item;
+    s.keys = keys;
+    s.off = off;
+    s.tiles = tiles;
+    s.t0 = t;
+    s.nt = static_cast<int>(min(static_cast<long long>(tiles - t), left));
+    left -= s.nt;
+    end += s.nt;
+    if (left > 0) {  // the item is done, the next one follows
+      t = 0;
+      if (++item == per_seq) {
+        item = 0;
+        enter(pr, b + 1, tile);
+      }
+    } else if (s.t0 == 0 && s.nt < s.tiles) {
+      // the CTAs up to the one that holds the item's last tile
+      const long long last_tile = end + s.tiles - s.nt - 1;
+      int last = static_cast<int>(((last_tile + 1) * gridDim.x - 1) / total);
+      while (last + 1 < static_cast<int>(gridDim.x) && total * (last + 1) / gridDim.x <= last_tile) ++last;
+      while (total * last / gridDim.x > last_tile) --last;
+      entry = {s.b, s.item, last - static_cast<int>(blockIdx.x) + 1, 0};
+    }
+  }
+};
+
+template <int D, int RG>
+struct StepLayout {
+  static constexpr int KEYS = D == 64 ? 128 : 64;  // keys of a tile: 32 KB of K and V
+  static constexpr int WKEYS = KEYS / 4;           // keys of a warp
+  static constexpr int STAGES = RG == 1 ? 3 : 5;
+  static constexpr int CTAS = RG == 1 ? 2 : 1;  // of an SM
+  static constexpr int SLABS = D / 64;
+  static constexpr int TILE = KEYS * D * 2;
+  static constexpr int ROWS = 16 * RG;
+  static constexpr int WARPS = 4 * RG;  // that compute
+  static constexpr int THREADS = 32 * (WARPS + 1);
+  static constexpr int RING = STAGES * 2 * TILE;
+  // the warps' results are joined JOIN columns at a time: [WARPS][16][JOIN] fp32
+  static constexpr int JOIN = 32;
+  static constexpr int JOIN_OFF = RING;
+  static constexpr int ML_OFF = JOIN_OFF + WARPS * 16 * JOIN * 4;  // max and sum [WARPS][16] each
+  static constexpr int SEGS = 4;                                 // segments' ring
+  static constexpr int SEG_OFF = ML_OFF + 2 * WARPS * 16 * 4;
+  static constexpr int BAR_OFF = SEG_OFF + SEGS * 32;  // full[], empty[], seg_full[], seg_empty[]
+  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 2 * SEGS) * 8;
+  // bias: bucket by position, then entries
+  static constexpr int LUT_OFF = MISC_OFF + 16;
+  // bytes of the bias part for `heads` heads
+  static int bias_bytes(const Bias& bias, int heads) { return lut_size(bias) * 2 + bias.buckets * heads * 4; }
 };
 
 // Heads of the group that a tile of `rows` rows can meet.
@@ -68,292 +177,357 @@ __host__ __device__ inline int step_heads(int rows, int Sq, int G) {
   return n < G ? n : G;
 }
 
-template <int D, int MT, bool CAUSAL, bool BIAS>
-__global__ void __launch_bounds__(128)
-    ffa_gen_step_kernel(const __grid_constant__ Problem pr, const __grid_constant__ Bias bias, const View q,
-                        const View k, const View v, const View o, float* __restrict__ LSE, float* __restrict__ part,
-                        float* __restrict__ part_lse, int n_split, int row_tiles) {
-  using L = StepLayout<D, MT>;
-  constexpr int KS = D / 16;       // K-steps of Q K^T
-  constexpr int CHUNKS = D / 8;    // 16-byte chunks of a row
-  constexpr int ROWS = L::ROWS;
+template <int D, int RG, bool ROWS8, bool CAUSAL, bool BIAS>
+__global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>::CTAS)
+    ffa_gen_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const __grid_constant__ Problem pr, const __grid_constant__ Bias bias, const View q,
+                        const View o, float* __restrict__ LSE, float* __restrict__ part, float* __restrict__ part_lse,
+                        JoinEntry* __restrict__ entries, int row_tiles, int single) {
+  using L = StepLayout<D, RG>;
+  constexpr int KS = D / 16;          // K-steps of Q K^T
+  constexpr int NG = L::WKEYS / 16;   // groups of 16 keys of a warp
+  constexpr int NX = ROWS8 ? 1 : 2;   // rows of a thread
+  constexpr int ROWS = L::ROWS, JOIN = L::JOIN, STAGES = L::STAGES, NC = 32 * L::WARPS;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + L::BAR_OFF;
+  auto full = [&](int n) { return bar0 + 8 * (n % STAGES); };
+  auto empty = [&](int n) { return bar0 + 8 * (STAGES + n % STAGES); };
+  auto seg_full = [&](int n) { return bar0 + 8 * (2 * STAGES + n % L::SEGS); };
+  auto seg_empty = [&](int n) { return bar0 + 8 * (2 * STAGES + L::SEGS + n % L::SEGS); };
+  auto seg_slot = [&](int n) { return reinterpret_cast<Segment*>(smem + L::SEG_OFF + 32 * (n % L::SEGS)); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = lane >> 2, qlane = lane & 3;
-
-  const int split = blockIdx.x % n_split;
-  const int row0 = (blockIdx.x / n_split) % row_tiles * ROWS;
-  const int hk = blockIdx.x / (n_split * row_tiles) % pr.Hkv;
-  const int b = blockIdx.x / (n_split * row_tiles) / pr.Hkv;
   const int rows = pr.G * pr.Sq;
-  const int off = (CAUSAL || BIAS) ? pr.offset(b) : 0;
-  const int n_keys = pr.keys(b, off, CAUSAL);
-  const int stages_all = (n_keys + L::KEYS - 1) / L::KEYS;
-  const int per_split = (stages_all + n_split - 1) / n_split;
-  const int s0 = split * per_split;
-  const int ns = max(0, min(stages_all - s0, per_split));
-
-  // ------------------------------------------------------------------ K/V ring
-  const __nv_bfloat16* kb = static_cast<const __nv_bfloat16*>(k.p) + b * k.sb + hk * k.sh;
-  const __nv_bfloat16* vb = static_cast<const __nv_bfloat16*>(v.p) + b * v.sb + hk * v.sh;
-  auto load = [&](int n) {  // stage n of this split; a commit group even when there is none
-    if (n < ns) {
-      const uint32_t dst = sbase + (n % L::STAGES) * 2 * L::TILE;
-      const int key0 = (s0 + n) * L::KEYS;
-#pragma unroll
-      for (int e = 0; e < L::KEYS * CHUNKS / 128; ++e) {
-        const int c = threadIdx.x + e * 128;
-        const int row = c / CHUNKS, ch = c % CHUNKS;
-        const bool ok = key0 + row < n_keys && ch * 8 < pr.D;
-        const uint32_t at = dst + row * (D * 2) + ((ch ^ (row & 7)) << 4);
-        const long long key = ok ? key0 + row : 0, col = ok ? ch * 8 : 0;
-        cp_async16(at, kb + key * k.ss + col, ok);
-        cp_async16(at + L::TILE, vb + key * v.ss + col, ok);
-      }
+  const int per_seq = pr.Hkv * row_tiles;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), L::WARPS);
     }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int n = 0; n < L::STAGES - 1; ++n) load(n);
-
-  // ------------------------------------------------------------------ Q, and each row's limits
-  // the thread's rows: quad and quad + 8 of each 16-row tile
-  uint32_t qf[MT][KS][4];
-  int lim[MT][2], pos[MT][2], head[MT][2];
-  const int g0 = row0 / pr.Sq;  // the tile's first head of the group
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = row0 + mt * 16 + x * 8 + quad;
-      const bool ok = r < rows;
-      const int g = ok ? r / pr.Sq : g0, t = ok ? r % pr.Sq : 0;
-      pos[mt][x] = t + off;
-      lim[mt][x] = ok ? (CAUSAL ? min(n_keys - 1, t + off) : n_keys - 1) : -1;
-      head[mt][x] = g - g0;
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(q.p) + b * q.sb +
-                                 static_cast<long long>(hk * pr.G + g) * q.sh + t * q.ss;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int col = ks * 16 + y * 8 + qlane * 2;
-          qf[mt][ks][x + 2 * y] = (ok && col < pr.D) ? *reinterpret_cast<const uint32_t*>(src + col) : 0u;
-        }
+    for (int s = 0; s < L::SEGS; ++s) {
+      mbar_init(seg_full(s), 1);
+      mbar_init(seg_empty(s), L::WARPS);
     }
-  // bias: bucket of each position in [-left, right], entries [head][bucket]
-  const unsigned short* lut = reinterpret_cast<const unsigned short*>(smem + L::LUT_OFF);
-  const float* entries = nullptr;
-  if (BIAS) {
-    unsigned short* w = reinterpret_cast<unsigned short*>(smem + L::LUT_OFF);
-    float* ew = reinterpret_cast<float*>(smem + L::LUT_OFF + (bias.left + bias.right + 2) / 2 * 4);
-    entries = ew;
-    const int heads = step_heads(ROWS, pr.Sq, pr.G);
-    for (int t = threadIdx.x; t <= bias.left + bias.right; t += 128)
-      w[t] = static_cast<unsigned short>(bias.bucket(t - bias.left));
-    for (int t = threadIdx.x; t < heads * bias.buckets; t += 128) {
-      const int g = g0 + t / bias.buckets;
-      ew[t] = g < pr.G ? bias.entry(t % bias.buckets, hk * pr.G + g, pr.Hq) : 0.f;
-    }
-    __syncthreads();
+    *abort_flag = 0;
+    fence_barrier_init();
   }
+  unsigned short* lut = reinterpret_cast<unsigned short*>(smem + L::LUT_OFF);
+  float* entry = reinterpret_cast<float*>(smem + L::LUT_OFF + (BIAS ? lut_size(bias) * 2 : 0));
+  __syncthreads();
 
-  // ------------------------------------------------------------------ the keys
-  float acc[MT][D / 8][4];
-  float mx[MT][2], sum[MT][2];
+  if (warp == L::WARPS) {
+    // ------------------------------------------------------------------ producer
+    Work<CAUSAL, CAUSAL || BIAS> work;
+    work.start(pr, per_seq, L::KEYS, single != 0);
+    if (lane == 0) {
+      const uint64_t once = policy_evict_first();
+      JoinEntry shared{0, 0, 0, 0};
+      bool ok = true;
+      int it = 0;
+      for (int n = 0; ok; ++n) {
+        Segment s;
+        work.next(pr, per_seq, L::KEYS, s, shared);
+        if (n >= L::SEGS &&
+            !(ok = mbar_wait(seg_empty(n), (n / L::SEGS - 1) & 1, abort_flag, kErrGenStepProducer)))
+          break;
+        *seg_slot(n) = s;
+        mbar_arrive(seg_full(n));
+        if (s.tiles == 0) break;
+        const int hk = s.item / row_tiles;
+        for (int x = 0; x < s.nt; ++x, ++it) {
+          if (!(ok = mbar_wait(empty(it), ((it / STAGES) & 1) ^ 1, abort_flag, kErrGenStepProducer))) break;
+          const uint32_t dst = sbase + (it % STAGES) * 2 * L::TILE;
+          mbar_arrive_expect_tx(full(it), 2 * L::TILE);
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      mx[mt][x] = -INFINITY;
-      sum[mt][x] = 0.f;
-    }
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[mt][n][e] = 0.f;
-  }
-  const int w16 = warp * 16;
-  for (int n = 0; n < ns; ++n) {
-    cp_async_wait<L::STAGES - 2>();
-    __syncthreads();  // stage n has landed; everyone is done with stage n - 1
-    load(n + L::STAGES - 1);
-    const uint32_t kt = sbase + (n % L::STAGES) * 2 * L::TILE, vt = kt + L::TILE;
-    const int key0 = (s0 + n) * L::KEYS + w16;
-    if (key0 >= n_keys) continue;  // the warp's keys are all behind the last one
-    float s[MT][2][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
-    {
-      const int row = w16 + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        uint32_t kf[4];
-        ldmatrix4(kf, kt + row * (D * 2) + (((2 * ks + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma_16816(s[mt][0], qf[mt][ks], kf[0], kf[1]);
-          mma_16816(s[mt][1], qf[mt][ks], kf[2], kf[3]);
+          for (int sl = 0; sl < L::SLABS; ++sl) {
+            tma_load_4d(dst + sl * L::KEYS * 128, &tm_k, full(it), sl * 64, (s.t0 + x) * L::KEYS, hk, s.b, once);
+            tma_load_4d(dst + L::TILE + sl * L::KEYS * 128, &tm_v, full(it), sl * 64, (s.t0 + x) * L::KEYS, hk, s.b,
+                        once);
+          }
         }
       }
+      if (entries != nullptr) entries[blockIdx.x] = shared;
+      if (*abort_flag)
+        for (int x = max(0, it - STAGES); x < it; ++x) mbar_wait_drain(full(x), (x / STAGES) & 1);
     }
-    uint32_t pf[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    return;
+  }
+
+  // -------------------------------------------------------------------- compute
+  const int quad = lane >> 2, qlane = lane & 3;
+  const int rg = warp >> 2;  // the warp's 16 rows of an item
+  if (BIAS)
+    for (int t = threadIdx.x; t <= bias.left + bias.right; t += NC)
+      lut[t] = static_cast<unsigned short>(bias.bucket(t - bias.left));
+  bool ok = true;
+  int it = 0;  // tile of the CTA
+  for (int n = 0;; ++n) {
+    // a wait that ran out ends all warps here, at the next segment
+    Segment sg{};
+    ok = ok && warp_wait(seg_full(n), (n / L::SEGS) & 1, abort_flag, kErrGenStepCompute);
+    if (ok) sg = *seg_slot(n);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(seg_empty(n));
+    ok = named_barrier_and(1, NC, ok);
+    if (!ok || sg.tiles == 0) break;
+    const int b = sg.b, n_keys = sg.keys;
+    const int hk = sg.item / row_tiles, row0 = sg.item % row_tiles * ROWS;
+    // the thread's rows: quad and quad + 8 of the warp's 16; Q as A fragments
+    uint32_t qf[KS][4];
+    int lim[NX], pos[NX], head[NX];
+    const int g0 = row0 / pr.Sq;  // the item's first head of the group
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        // the row's 4 scores of this thread: s[mt][nt][2x], s[mt][nt][2x + 1], keys
-        // key0 + 8 nt + 2 qlane + {0, 1}
-        float m = -INFINITY;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = key0 + 8 * nt + 2 * qlane + e;
-            float& y = s[mt][nt][2 * x + e];
-            y *= pr.scale_log2;
-            if (BIAS) {
-              const int r = min(max(key - pos[mt][x], -bias.left), bias.right);
-              y += entries[head[mt][x] * bias.buckets + lut[r + bias.left]];
-            }
-            if (key > lim[mt][x]) y = -INFINITY;
-            m = fmaxf(m, y);
-          }
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float m_new = fmaxf(mx[mt][x], m);
-        const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = fast_exp2(mx[mt][x] - m_safe);
-        mx[mt][x] = m_new;
-        float t = 0.f;
-        float p[2][2];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            p[nt][e] = fast_exp2(s[mt][nt][2 * x + e] - m_safe);
-            t += p[nt][e];
-          }
-        sum[mt][x] = fmaf(sum[mt][x], alpha, t);
-        // P goes to the product in bf16, as in the other kernels; its sum stays fp32
-        pf[mt][x] = pack_bf16x2(p[0][0], p[0][1]);
-        pf[mt][2 + x] = pack_bf16x2(p[1][0], p[1][1]);
-#pragma unroll
-        for (int d = 0; d < D / 8; ++d) {
-          acc[mt][d][2 * x] *= alpha;
-          acc[mt][d][2 * x + 1] *= alpha;
+        const int r = row0 + rg * 16 + x * 8 + quad;
+        const bool valid = x < NX && r < rows;
+        const int g = valid ? r / pr.Sq : g0, t = valid ? r % pr.Sq : 0;
+        if (x < NX) {
+          pos[x] = t + sg.off;
+          lim[x] = valid ? (CAUSAL ? min(n_keys - 1, t + sg.off) : n_keys - 1) : -1;
+          head[x] = (g - g0) * bias.buckets;
         }
-      }
-    {
-      const int row = w16 + (lane & 15);
+        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(q.p) + b * q.sb +
+                                   static_cast<long long>(hk * pr.G + g) * q.sh + t * q.ss;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        uint32_t vf[4];
-        ldmatrix4_trans(vf, vt + row * (D * 2) + (((2 * d + (lane >> 4)) ^ (row & 7)) << 4));
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma_16816(acc[mt][2 * d], pf[mt], vf[0], vf[1]);
-          mma_16816(acc[mt][2 * d + 1], pf[mt], vf[2], vf[3]);
-        }
+          for (int y = 0; y < 2; ++y) {
+            const int col = ks * 16 + y * 8 + qlane * 2;
+            qf[ks][x + 2 * y] = (valid && col < pr.D) ? *reinterpret_cast<const uint32_t*>(src + col) : 0u;
+          }
       }
+    if (BIAS) {
+      const int heads = step_heads(ROWS, pr.Sq, pr.G);
+      for (int t = threadIdx.x; t < heads * bias.buckets; t += NC) {
+        const int g = g0 + t / bias.buckets;
+        entry[t] = g < pr.G ? bias.entry(t % bias.buckets, hk * pr.G + g, pr.Hq) : 0.f;
+      }
+      named_barrier_and(1, NC, true);
     }
-  }
-  cp_async_wait<0>();
-  __syncthreads();  // the ring is free
 
-  // ------------------------------------------------------------------ join the four warps
-  float* so = reinterpret_cast<float*>(smem);
-  float* sm = reinterpret_cast<float*>(smem + L::ML_OFF);
-  float* sl = sm + 4 * ROWS;
+    float acc[D / 8][4];
+    float mx[NX], sum[NX];
+    {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = mt * 16 + x * 8 + quad;
-      float t = sum[mt][x];
-      t += __shfl_xor_sync(0xffffffffu, t, 1);
-      t += __shfl_xor_sync(0xffffffffu, t, 2);
-      if (qlane == 0) {
-        sm[warp * ROWS + r] = mx[mt][x];
-        sl[warp * ROWS + r] = t;
+      for (int x = 0; x < NX; ++x) {
+        mx[x] = -INFINITY;
+        sum[x] = 0.f;
       }
-      float* dst = so + (warp * ROWS + r) * D + 2 * qlane;
 #pragma unroll
       for (int d = 0; d < D / 8; ++d)
-        *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(acc[mt][d][2 * x], acc[mt][d][2 * x + 1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][e] = 0.f;
     }
-  __syncthreads();
-  for (int c = threadIdx.x; c < ROWS * CHUNKS; c += 128) {
-    const int r = c / CHUNKS, col = c % CHUNKS * 8;
-    if (row0 + r >= rows) break;
-    float m = -INFINITY;
+    const int w0 = (warp & 3) * L::WKEYS;  // the warp's first key of a tile
+    for (int j = 0; j < sg.nt; ++j, ++it) {
+      if (!(ok = warp_wait(full(it), (it / STAGES) & 1, abort_flag, kErrGenStepCompute))) break;
+      const uint32_t kt = sbase + (it % STAGES) * 2 * L::TILE, vt = kt + L::TILE;
+      const int key0 = (sg.t0 + j) * L::KEYS + w0;
+      if (key0 < n_keys) {
+        float s[2 * NG][4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w * ROWS + r]);
-    float total = 0.f, out[8] = {};
+          for (int nt = 0; nt < 2 * NG; ++nt)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = m == -INFINITY ? 0.f : fast_exp2(sm[w * ROWS + r] - m);
-      total = fmaf(f, sl[w * ROWS + r], total);
-      const float* src = so + (w * ROWS + r) * D + col;
+            for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = fmaf(f, src[e], out[e]);
+        for (int gk = 0; gk < NG; ++gk) {
+          const int row = w0 + 16 * gk + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t kf[4];
+            ldmatrix4(kf, kt + (ks >> 2) * (L::KEYS * 128) + row * 128 +
+                              (((2 * (ks & 3) + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+    {
+              mma_16816(s[2 * gk], qf[ks], kf[0], kf[1]);
+              mma_16816(s[2 * gk + 1], qf[ks], kf[2], kf[3]);
+            }
+          }
+        }
+        if (key0 + L::WKEYS > n_keys) {
+          // V rows behind the last key must not reach the product (0 * NaN); this warp is the
+          // only one that reads them, and the fence orders its writes before the next copy
+          for (int r = n_keys - key0; r < L::WKEYS; ++r)
+#pragma unroll
+            for (int sl = 0; sl < L::SLABS; ++sl)
+              if (lane < 8) st_shared_v4(vt + sl * L::KEYS * 128 + (w0 + r) * 128 + lane * 16, 0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        uint32_t pf[NG][4];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (x >= NX) {  // rows 8 to 15: P = 0
+#pragma unroll
+              for (int gk = 0; gk < NG; ++gk) pf[gk][x] = pf[gk][2 + x] = 0u;
+              continue;
+            }
+            constexpr int X = NX - 1;  // (keeps the index below NX for the compiler)
+            const int xx = x < NX ? x : X;
+            // the row's scores of this thread: keys key0 + 8 nt + 2 qlane + {0, 1}
+            float m = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < 2 * NG; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 8 * nt + 2 * qlane + e;
+                float& y = s[nt][2 * x + e];
+                y *= pr.scale_log2;
+                if (BIAS) {
+                  const int r = min(max(key - pos[xx], -bias.left), bias.right);
+                  y += entry[head[xx] + lut[r + bias.left]];
+                }
+                if (key > lim[xx]) y = -INFINITY;
+                m = fmaxf(m, y);
+              }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float old = mx[xx], m_new = fmaxf(old, m);
+            const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+            if (__any_sync(0xffffffffu, m_new > old)) {
+              const float alpha = fast_exp2(old - m_safe);
+              mx[xx] = m_new;
+              sum[xx] *= alpha;
+#pragma unroll
+              for (int d = 0; d < D / 8; ++d) {
+                acc[d][2 * x] *= alpha;
+                acc[d][2 * x + 1] *= alpha;
+              }
+            }
+            // P goes to the product in bf16, as in the other kernels; its sum stays fp32
+#pragma unroll
+            for (int nt = 0; nt < 2 * NG; ++nt) {
+              const float p0 = fast_exp2(s[nt][2 * x] - m_safe), p1 = fast_exp2(s[nt][2 * x + 1] - m_safe);
+              sum[xx] += p0 + p1;
+              pf[nt >> 1][x + 2 * (nt & 1)] = pack_bf16x2(p0, p1);
+            }
+          }
+#pragma unroll
+        for (int gk = 0; gk < NG; ++gk) {
+          const int row = w0 + 16 * gk + (lane & 15);
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            uint32_t vf[4];
+            ldmatrix4_trans(vf, vt + (d >> 2) * (L::KEYS * 128) + row * 128 +
+                                    (((2 * (d & 3) + (lane >> 4)) ^ (row & 7)) << 4));
+    {
+              mma_16816(acc[2 * d], pf[gk], vf[0], vf[1]);
+              mma_16816(acc[2 * d + 1], pf[gk], vf[2], vf[3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty(it));
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int g = (row0 + r) / pr.Sq, t = (row0 + r) % pr.Sq;
-    const long long h = hk * pr.G + g;
-    const long long ridx = (b * static_cast<long long>(pr.Hq) + h) * pr.Sq + t;
-    const float lse = total == 0.f ? -INFINITY : m + __log2f(total);
+
+    // ------------------------------------------------------------------ join the four warps
+    float* so = reinterpret_cast<float*>(smem + L::JOIN_OFF);
+    float* sm = reinterpret_cast<float*>(smem + L::ML_OFF);
+    float* sl = sm + L::WARPS * 16;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] *= inv;
-    if (n_split > 1) {
-      const long long idx = static_cast<long long>(split) * pr.B * pr.Hq * pr.Sq + ridx;
-      if (col == 0) part_lse[idx] = lse;
-      if (col < pr.D) {
-        float4* dst = reinterpret_cast<float4*>(part + idx * pr.D + col);
-        dst[0] = make_float4(out[0], out[1], out[2], out[3]);
-        dst[1] = make_float4(out[4], out[5], out[6], out[7]);
+      for (int x = 0; x < NX; ++x) {
+        float t = sum[x];
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        if (qlane == 0) {
+          sm[warp * 16 + x * 8 + quad] = mx[x];
+          sl[warp * 16 + x * 8 + quad] = t;
+        }
       }
-    } else {
-      if (col == 0 && LSE != nullptr) LSE[ridx] = lse;
-      if (col < pr.D) {
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + col;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3]),
-                                                    pack_bf16x2(out[4], out[5]), pack_bf16x2(out[6], out[7]));
+    // this thread's part of the output: 4 columns of one row in each round; the row's warps
+    // are 4 rg .. 4 rg + 3
+    const int r = threadIdx.x / (JOIN / 4), c4 = threadIdx.x % (JOIN / 4) * 4;
+    const int r16 = (r & 15) + (r >> 4) * 64;
+    const bool valid = row0 + r < rows;
+    const int t = valid ? (row0 + r) % pr.Sq : 0;
+    const long long h = hk * pr.G + (valid ? (row0 + r) / pr.Sq : 0);
+    const long long prow = (2LL * blockIdx.x + (sg.t0 == 0 ? 1 : 0)) * ROWS + r;
+    float f[4] = {}, m = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int round = 0; round < D / JOIN; ++round) {
+      if (round > 0) named_barrier_and(1, NC, true);  // the last round has been read
+#pragma unroll
+        for (int d = 0; d < JOIN / 8; ++d)
+#pragma unroll
+          for (int x = 0; x < NX; ++x)
+            *reinterpret_cast<float2*>(so + (warp * 16 + x * 8 + quad) * JOIN + 8 * d + 2 * qlane) =
+                make_float2(acc[round * (JOIN / 8) + d][2 * x], acc[round * (JOIN / 8) + d][2 * x + 1]);
+      ok = named_barrier_and(1, NC, ok);
+      if (!valid) continue;
+      if (round == 0) {  // the warps' weights, normalised
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[r16 + w * 16]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          f[w] = m == -INFINITY ? 0.f : fast_exp2(sm[r16 + w * 16] - m);
+          total = fmaf(f[w], sl[r16 + w * 16], total);
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) f[w] *= inv;
       }
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(so + (r16 + w * 16) * JOIN + c4);
+        a.x = fmaf(f[w], y.x, a.x);
+        a.y = fmaf(f[w], y.y, a.y);
+        a.z = fmaf(f[w], y.z, a.z);
+        a.w = fmaf(f[w], y.w, a.w);
+      }
+      const int col = round * JOIN + c4;
+      if (ok && col < pr.D) {
+        if (sg.whole())
+          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + col) =
+              make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+        else
+          *reinterpret_cast<float4*>(part + prow * pr.D + col) = a;
+      }
+    }
+    if (ok && valid && c4 == 0) {
+      const float lse = total == 0.f ? -INFINITY : m + __log2f(total);
+      if (!sg.whole())
+        part_lse[prow] = lse;
+      else if (LSE != nullptr)
+        LSE[(b * static_cast<long long>(pr.Hq) + h) * pr.Sq + t] = lse;
     }
   }
 }
 
-// Join the splits of a row: O = sum_s w_s O_s / sum_s w_s, w_s = 2^(LSE_s - max LSE).  One
-// warp a row, four columns a lane; a split without keys (LSE = -inf) is not read.
+// Join the parts of the items that cross CTAs: O = sum_p w_p O_p / sum_p w_p with
+// w_p = 2^(LSE_p - max LSE).  blockIdx.x: the CTA in which an item starts; a warp takes one
+// row, four columns a lane.  A part whose keys the row does not see (LSE = -inf) is not read.
 __global__ void __launch_bounds__(128)
-    ffa_gen_join_kernel(const float* __restrict__ part, const float* __restrict__ part_lse, const View o,
-                        float* __restrict__ LSE, int n_split, int B, int H, int Sq, int D) {
+    ffa_gen_step_join_kernel(const __grid_constant__ Problem pr, const float* __restrict__ part,
+                             const float* __restrict__ part_lse, const JoinEntry* __restrict__ entries, const View o,
+                             float* __restrict__ LSE, int row_tiles, int rows) {
   const int lane = threadIdx.x & 31;
-  const long long rows = static_cast<long long>(B) * H * Sq;
-  const long long r = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (r >= rows) return;
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 5);  // of the item
+  asm volatile("griddepcontrol.wait;" ::: "memory");    // the parts are written
+  const JoinEntry e = entries[blockIdx.x];
+  if (e.parts == 0) return;
+  const int r = e.item % row_tiles * rows + row;
+  if (r >= pr.G * pr.Sq) return;
+  const int h = e.item / row_tiles * pr.G + r / pr.Sq, t = r % pr.Sq;
+  // row of part p: slot 1 of the first CTA, slot 0 of the next ones
+  auto at = [&](int p) { return (2LL * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * rows + row; };
   float m = -INFINITY;
-  for (int s = lane; s < n_split; s += 32) m = fmaxf(m, part_lse[s * rows + r]);
+  for (int p = lane; p < e.parts; p += 32) m = fmaxf(m, part_lse[at(p)]);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
   float total = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   const int c = lane * 4;
   if (m > -INFINITY) {
-#pragma unroll 4
-    for (int s = 0; s < n_split; ++s) {
-      const float lse = part_lse[s * rows + r];
-      if (lse == -INFINITY) continue;
+#pragma unroll 8
+    for (int p = 0; p < e.parts; ++p) {
+      const float lse = part_lse[at(p)];
       const float w = exp2f(lse - m);
       total += w;
-      if (c < D) {
-        const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + r) * D + c);
+      if (c < pr.D && lse > -INFINITY) {
+        const float4 x = *reinterpret_cast<const float4*>(part + at(p) * pr.D + c);
         a.x = fmaf(w, x.x, a.x);
         a.y = fmaf(w, x.y, a.y);
         a.z = fmaf(w, x.z, a.z);
@@ -362,12 +536,12 @@ __global__ void __launch_bounds__(128)
     }
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  if (c < D) {
-    const long long bh = r / Sq, t = r % Sq;
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(o.p) + bh / H * o.sb + bh % H * o.sh + t * o.ss + c;
+  if (c < pr.D) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(o.p) + e.b * o.sb + h * o.sh + t * o.ss + c;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
   }
-  if (lane == 0 && LSE != nullptr) LSE[r] = total == 0.f ? -INFINITY : m + __log2f(total);
+  if (lane == 0 && LSE != nullptr)
+    LSE[(static_cast<long long>(e.b) * pr.Hq + h) * pr.Sq + t] = total == 0.f ? -INFINITY : m + __log2f(total);
 }
 
 }  // namespace gen
