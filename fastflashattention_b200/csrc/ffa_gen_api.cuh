@@ -198,6 +198,7 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias) {
 }
 
 struct BwdPlan {
+  bool narrow;  // 64-wide steps, two CTAs to an SM
   int dq_split, dkdv_split;
   long long stat_floats;              // LSE and delta, each
   long long dq_off, dk_off, dv_off;   // offsets in floats; all regions start 256-byte aligned
@@ -209,8 +210,10 @@ inline BwdPlan bwd_plan(const ffa_gen_problem* p, const Bias& bias) {
   const long long hq = static_cast<long long>(p->batch) * p->q_heads, hk = static_cast<long long>(p->batch) * p->kv_heads;
   const long long qb = ceil_div(p->q_len, 128), kb = ceil_div(p->k_len, 128);
   const long long g = p->kv_heads ? p->q_heads / p->kv_heads : 1;
-  w.dq_split = split_of(hq * qb, kSMs, kb, 4);
-  w.dkdv_split = split_of(hk * kb, kSMs, g * qb, 4);
+  w.narrow = p->head_dim <= 64;
+  const int slots = w.narrow ? 2 * kSMs : kSMs;
+  w.dq_split = split_of(hq * qb, slots, kb, 4);
+  w.dkdv_split = split_of(hk * kb, slots, g * qb, 4);
   auto round64 = [](long long n) { return (n + 63) / 64 * 64; };
   w.stat_floats = round64(hq * padded_rows(p->q_len));
   long long at = 2 * w.stat_floats;
@@ -349,9 +352,10 @@ static int launch_gen_step(const Call& c, const FwdPlan& f, float* ws) {
                                : launch_gen_step_rg<D, 1, false, CAUSAL, BIAS>(c, f, ws);
 }
 
-template <int D, bool CAUSAL, bool BIAS>
+template <int D, int NWG, bool CAUSAL, bool BIAS>
 static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
-  using L = DkdvLayout<D, BIAS>;
+  using L = DkdvLayout<D, NWG, BIAS>;
+  using W = BwdWidth<NWG>;
   const Problem& pr = c.pr;
   CUtensorMap tk, tv, tq, tdo, tdk, tdv;
   int rc;
@@ -361,43 +365,62 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   if ((rc = make_map(&tdv, c.dv, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
   tq = tdo = tk;  // without queries nothing is loaded through them
   if (pr.Sq > 0) {
-    if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
-    if ((rc = make_map(&tdo, c.dout, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+    if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D, L::STEP))) return rc;
+    if ((rc = make_map(&tdo, c.dout, pr.B, pr.Hq, pr.Sq, pr.D, L::STEP))) return rc;
   }
-  auto kern = ffa_gen_dkdv_kernel<D, CAUSAL, BIAS>;
+  auto kern = ffa_gen_dkdv_kernel<D, NWG, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
-  static bool configured_regs = false;
-  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
-  if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs))) return rc;
-  const long long grid = ceil_div(pr.Sk, 128) * w.dkdv_split * pr.B * pr.Hkv;
-  kern<<<static_cast<unsigned>(grid), bwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
-      tk, tv, tq, tdo, tdk, tdv, pr, c.bias, ws + w.table_off, ws, ws + w.stat_floats, ws + w.dk_off, ws + w.dv_off, w.dkdv_split,
-      work_group(pr.B * pr.Hkv, static_cast<int>(std::min<long long>(1LL * pr.Sq * pr.G, INT_MAX)), pr.D, CAUSAL));
+  constexpr int most = L::TAB_OFF + (BIAS ? kTableMax * 4 : 0);
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
+  if constexpr (NWG == 2) {
+    static bool configured_regs = false;
+    if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs)))
+      return rc;
+  }
+  const dim3 grid(static_cast<unsigned>(ceil_div(pr.Sk, 128) * w.dkdv_split * pr.B * pr.Hkv));
+  const int rows = static_cast<int>(std::min<long long>(1LL * pr.Sq * pr.G, INT_MAX));
+  const float* tables = ws + w.table_off;
+  const float *lse = ws, *delta = ws + w.stat_floats;
+  const int smem = L::smem_bytes(c.bias), group = work_group(pr.B * pr.Hkv, rows, pr.D, CAUSAL);
+  if (pr.Sq > 0)  // behind the kernel that writes delta
+    return launch_early(kern, grid, W::THREADS, smem, c.stream, tk, tv, tq, tdo, tdk, tdv, pr, c.bias, tables, lse,
+                        delta, ws + w.dk_off, ws + w.dv_off, w.dkdv_split, group);
+  kern<<<grid, W::THREADS, smem, c.stream>>>(tk, tv, tq, tdo, tdk, tdv, pr, c.bias, tables, lse, delta, ws + w.dk_off,
+                                             ws + w.dv_off, w.dkdv_split, group);
   return launched();
 }
 
-template <int D, bool CAUSAL, bool BIAS>
+template <int D, int NWG, bool CAUSAL, bool BIAS>
 static int launch_gen_dq(const Call& c, const BwdPlan& w, float* ws) {
-  using L = DqLayout<D, BIAS>;
+  using L = DqLayout<D, NWG, BIAS>;
+  using W = BwdWidth<NWG>;
   const Problem& pr = c.pr;
   CUtensorMap tk, tv, tdq;
   int rc;
   if ((rc = make_map(&tdq, c.dq, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
   tk = tv = tdq;  // without keys nothing is loaded through them
   if (pr.Sk > 0) {
-    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
-    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D, L::STEP))) return rc;
+    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D, L::STEP))) return rc;
   }
-  auto kern = ffa_gen_dq_kernel<D, CAUSAL, BIAS>;
+  auto kern = ffa_gen_dq_kernel<D, NWG, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
-  static bool configured_regs = false;
-  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::SMEM_BYTES, &configured))) return rc;
-  if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs))) return rc;
-  const long long grid = ceil_div(pr.Sq, 128) * w.dq_split * pr.B * pr.Hq;
-  kern<<<static_cast<unsigned>(grid), bwd::NTHREADS, L::SMEM_BYTES, c.stream>>>(
-      tk, tv, tdq, pr, c.bias, ws + w.table_off,
-      reinterpret_cast<const unsigned short*>(ws + w.lut_off), c.q, c.dout, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split,
-      work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL));
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::MOST, &configured))) return rc;
+  if constexpr (NWG == 2) {
+    static bool configured_regs = false;
+    if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs)))
+      return rc;
+  }
+  const dim3 grid(static_cast<unsigned>(ceil_div(pr.Sq, 128) * w.dq_split * pr.B * pr.Hq));
+  const int smem = L::smem_bytes(c.bias), group = work_group(pr.B * pr.Hq, pr.Sk, pr.D, CAUSAL);
+  const float* tables = ws + w.table_off;
+  const unsigned short* lut = reinterpret_cast<const unsigned short*>(ws + w.lut_off);
+  const float* lse = c.lse;
+  if (BIAS)
+    return launch_early(kern, grid, W::THREADS, smem, c.stream, tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.dout,
+                        lse, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split, group);
+  kern<<<grid, W::THREADS, smem, c.stream>>>(tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.dout, lse, ws,
+                                             ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split, group);
   return launched();
 }
 
@@ -423,11 +446,19 @@ struct RunStep {
 };
 template <int D, bool C, bool B>
 struct RunDkdv {
-  static int run(const Call& c, const BwdPlan& w, float* ws) { return launch_gen_dkdv<D, C, B>(c, w, ws); }
+  static int run(const Call& c, const BwdPlan& w, float* ws) {
+    if constexpr (D == 64)
+      if (w.narrow) return launch_gen_dkdv<D, 1, C, B>(c, w, ws);
+    return launch_gen_dkdv<D, 2, C, B>(c, w, ws);
+  }
 };
 template <int D, bool C, bool B>
 struct RunDq {
-  static int run(const Call& c, const BwdPlan& w, float* ws) { return launch_gen_dq<D, C, B>(c, w, ws); }
+  static int run(const Call& c, const BwdPlan& w, float* ws) {
+    if constexpr (D == 64)
+      if (w.narrow) return launch_gen_dq<D, 1, C, B>(c, w, ws);
+    return launch_gen_dq<D, 2, C, B>(c, w, ws);
+  }
 };
 
 }  // namespace gen
@@ -509,11 +540,12 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   c.v = view(v);
   c.o = view(o);
   c.dout = view(dout);
+  c.lse = const_cast<float*>(lse);
   c.stream = static_cast<cudaStream_t>(stream);
   float* ws = static_cast<float*>(workspace);
   if (p->bias && queries && (rc = launch_tables(c, ws + w.table_off, reinterpret_cast<unsigned short*>(ws + w.lut_off))))
     return rc;
-  if (queries) {
+  if (queries && !want_dq) {
     const long long rows = hq * padded_rows(p->q_len);
     if (p->head_dim <= 64)
       ffa_gen_prepare_kernel<8><<<static_cast<unsigned>(rows / 32), 256, 0, c.stream>>>(
@@ -529,6 +561,10 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
         part, out, n_split, p->batch, H, S, p->head_dim);
     return launched();
   };
+  if (want_dq && queries) {
+    c.dq = view(dq);
+    if ((rc = dispatch<RunDq>(c, p->causal, w, ws))) return rc;
+  }
   if (want_dkdv && keys) {
     c.dk = view(dk);
     c.dv = view(dv);
@@ -537,11 +573,9 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
                              (rc = sum(ws + w.dv_off, c.dv, w.dkdv_split, p->kv_heads, p->k_len))))
       return rc;
   }
-  if (want_dq && queries) {
-    c.dq = view(dq);
-    if ((rc = dispatch<RunDq>(c, p->causal, w, ws))) return rc;
-    if (w.dq_split > 1 && (rc = sum(ws + w.dq_off, c.dq, w.dq_split, p->q_heads, p->q_len))) return rc;
-  }
+  if (want_dq && queries && w.dq_split > 1 &&
+      (rc = sum(ws + w.dq_off, c.dq, w.dq_split, p->q_heads, p->q_len)))
+    return rc;
   if (dbias && p->q_heads > 0) {
     const int blocks = queries ? static_cast<int>(ceil_div(p->q_len, 128)) * w.dq_split : 0;
     ffa_gen_bias_sum_kernel<<<static_cast<unsigned>(ceil_div(static_cast<long long>(p->q_heads) * p->buckets, 4)), 128,

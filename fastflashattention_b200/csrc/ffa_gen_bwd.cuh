@@ -6,6 +6,12 @@
 //
 // The two kernels of the plain backward (ffa_bwd.cuh), with disjoint output tiles and no
 // atomics.  What differs:
+//   * delta comes from the dQ kernel, which has dO in hand; dK/dV follows it, launched while it
+//     still runs (programmatic dependent launch).  Without a wish for dQ,
+//     ffa_gen_prepare_kernel writes delta;
+//   * two widths of a step at head dims up to 64.  Wide (NWG = 2): 128 columns, two compute
+//     warpgroups, one CTA to an SM.  Narrow (NWG = 1): 64 columns, one warpgroup, 256 columns
+//     of tensor memory, two CTAs to an SM that fill each other's start, end and waits;
 //   * the dK/dV kernel walks the queries of all heads of its key head, one after another, so
 //     a shared key head's gradients are summed in tensor memory;
 //   * P = 0 outside the mask, and K / V rows behind the last key are zeroed in shared memory;
@@ -111,46 +117,38 @@ __device__ __forceinline__ void copy_table(float* tab, const float* tables, int 
   for (int t = tid; t < units; t += n) reinterpret_cast<float4*>(tab)[t] = src[t];
 }
 
-// Write the accumulator columns [g*D/2, (g+1)*D/2) of this lane to fp32 row `dst` (pr.D
-// values); `empty`: nothing was accumulated, write zeros.  The whole warp calls it.
-template <int D>
-__device__ __forceinline__ void write_acc_half(uint32_t t_acc, int g, float* dst, int true_d, bool valid, bool empty,
-                                               float mul) {
+// Give this lane's share of an accumulator (warpgroup g of NWG: D / NWG columns), times
+// `mul`, to the staged bf16 tile (128 rows, for a TMA store) or, with `part`, to an fp32 row
+// of `true_d` values.  `empty`: nothing was accumulated, and tensor memory may hold
+// anything: zeros.  The whole warp calls it.
+template <int D, int NWG>
+__device__ __forceinline__ void give_acc(uint32_t t_acc, int g, uint32_t tile, int row, float* part, int true_d,
+                                         bool done, bool row_ok, bool empty, float mul) {
+  if (!done) return;
 #pragma unroll 1
-  for (int c = g * (D / 64); c < (g + 1) * (D / 64); ++c) {
+  for (int c = g * (D / NWG); c < (g + 1) * (D / NWG); c += 32) {
     uint32_t r[32];
     if (empty) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) r[e] = 0u;
     } else {
-      tmem_ld32(t_acc + 32 * c, r);
+      tmem_ld32(t_acc + c, r);
       tmem_ld_wait();
     }
-    if (valid) write_row32(dst, 32 * c, true_d, r, mul);
+    if (part == nullptr)
+      stage_row32_sw128(tile, row, c, r, mul);
+    else if (row_ok)
+      write_row32(part, c, true_d, r, mul);
   }
 }
 
-// Stage the accumulator half (bwd::stage_acc_half), or zeros.
-template <int D>
-__device__ __forceinline__ void stage_half(uint32_t t_acc, int g, uint32_t tile, int row, bool empty, float mul) {
-  if (!empty) {
-    bwd::stage_acc_half<D>(t_acc, g, tile, row, mul);
-    return;
-  }
-  uint32_t r[32];
-#pragma unroll
-  for (int e = 0; e < 32; ++e) r[e] = 0u;
-#pragma unroll 1
-  for (int c = g * (D / 64); c < (g + 1) * (D / 64); ++c) stage_row32_sw128(tile, row, 32 * c, r, 0.f);
-}
-
-// Barrier of the 256 compute threads, then one TMA store of each staged tile (see
+// Barrier of the compute threads, then one TMA store of each staged tile (see
 // bwd::store_staged).
-template <int D, int NT>
+template <int D, int NWG, int NT>
 __device__ __forceinline__ void store_staged(bool staged, const CUtensorMap* const (&maps)[NT], uint32_t first_tile,
                                              int row0, int h, int b) {
   fence_proxy_async_smem();
-  const bool all = named_barrier_and(1, 256, staged);
+  const bool all = named_barrier_and(1, 128 * NWG, staged);
   if (all && threadIdx.x == 0) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -165,29 +163,48 @@ __device__ __forceinline__ void store_staged(bool staged, const CUtensorMap* con
 // ====================================================================================
 // dK / dV
 // ====================================================================================
-template <int D, bool BIAS>
+// Threads, registers and roles of the two widths.  Narrow CTAs share the registers evenly;
+// the wide one moves them to its compute warpgroups (see ffa_bwd.cuh).
+template <int NWG>
+struct BwdWidth {
+  static constexpr int STEP = 64 * NWG;
+  static constexpr int COMPUTE = 128 * NWG;  // threads
+  // warps; dK/dV: narrow CTAs have one producer for both rings (twelve warps of two CTAs leave
+  // each thread 168 registers, fourteen would leave 128)
+  static constexpr int PRODUCER = 4 * NWG, MMA = 4 * NWG + 1, DO_PRODUCER = NWG == 2 ? 10 : -1;
+  static constexpr int THREADS = NWG == 2 ? bwd::NTHREADS : 192;
+  static constexpr int CTAS = NWG == 2 ? 1 : 2;
+  static constexpr int TMEM = NWG == 2 ? 512 : 256;
+};
+
+template <int D, int NWG, bool BIAS>
 struct DkdvLayout {
-  static constexpr int TILE = 128 * D * 2;
+  static constexpr int STEP = 64 * NWG;
+  static constexpr int KV_TILE = 128 * D * 2;   // K, V (resident)
+  static constexpr int TILE = STEP * D * 2;     // Q, dO (streamed)
   // three Q slots, as in the plain kernel; at D = 128 the bias table takes the third's room
   static constexpr int Q_STAGES = (BIAS && D == 128) ? 2 : 3;
   static constexpr int DO_STAGES = 2;
   static constexpr int K_OFF = 0;
-  static constexpr int V_OFF = TILE;
-  static constexpr int Q_OFF = 2 * TILE;
+  static constexpr int V_OFF = KV_TILE;
+  static constexpr int Q_OFF = 2 * KV_TILE;
   static constexpr int DO_OFF = Q_OFF + Q_STAGES * TILE;
-  static constexpr int DO_STAGE_BYTES = TILE + 2 * 128 * 4;  // dO tile, lse[128], delta[128]
-  static constexpr int TAB_OFF = DO_OFF + DO_STAGES * DO_STAGE_BYTES;
-  static constexpr int BAR_OFF = TAB_OFF + (BIAS ? (kTableMax * 4 + 15) / 16 * 16 : 0);
+  static constexpr int STAT_BYTES = 2 * STEP * 4;  // lse, delta behind a dO tile
+  static constexpr int DO_STAGE_BYTES = TILE + 1024;
+  // tensor memory: S^T, dP^T (P and dS are written over it), dV, dK
+  static constexpr uint32_t DP_COL = STEP, DV_COL = 2 * STEP, DK_COL = 2 * STEP + D;
+  static constexpr int BAR_OFF = DO_OFF + DO_STAGES * DO_STAGE_BYTES;
   // kv_full, q_full[], q_empty[], do_full[2], do_empty[2], s_full, dp_full, p_ready,
   // ds_ready, final, drain, s_free
   static constexpr int NBARS = 1 + 2 * Q_STAGES + 2 * DO_STAGES + 7;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
+  static constexpr int TAB_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
   // no alignment slack (see bwd::DkdvLayout)
-  static constexpr int SMEM_BYTES = MISC_OFF + 16;
+  static int smem_bytes(const Bias& bias) { return TAB_OFF + (BIAS ? table_size(bias) * 4 : 0); }
 };
 
-template <int D, bool CAUSAL, bool BIAS>
-__global__ void __launch_bounds__(bwd::NTHREADS, 1)
+template <int D, int NWG, bool CAUSAL, bool BIAS>
+__global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     ffa_gen_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                         const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
@@ -195,8 +212,9 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
                         const float* __restrict__ tables, const float* __restrict__ LSE,
                         const float* __restrict__ DELTA, float* __restrict__ dk_part,
                         float* __restrict__ dv_part, int n_split, int group) {
-  using L = DkdvLayout<D, BIAS>;
-  constexpr int SLABS = D / 64;
+  using L = DkdvLayout<D, NWG, BIAS>;
+  using W = BwdWidth<NWG>;
+  constexpr int SLABS = D / 64, STEP = L::STEP;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023u) {  // the layout has no room to realign: report and leave
@@ -233,13 +251,13 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
   // mask the first key blocks have the most queries and come first
   const CtaWork cw = cta_work((pr.Sk + 127) / 128 * n_split, pr.B * pr.Hkv, group);
   const int split = cw.rank % n_split;
-  const int b = cw.bh / pr.Hkv, hk = cw.bh % pr.Hkv;
+  const int b = pr.seq_at(cw.bh / pr.Hkv), hk = cw.bh % pr.Hkv;
   const int n0 = cw.rank / n_split * 128;
   const int off = (CAUSAL || BIAS) ? pr.offset(b) : 0;
   const int n_keys = pr.keys(b, off, CAUSAL);
   // first query block that sees a key of this block (query i sees key j iff j <= i + off)
-  const int q_begin = CAUSAL ? max(0, n0 - off) / 128 * 128 : 0;
-  const int nqb = (n0 < n_keys && q_begin < pr.Sq) ? (pr.Sq - q_begin + 127) / 128 : 0;
+  const int q_begin = CAUSAL ? max(0, n0 - off) / STEP * STEP : 0;
+  const int nqb = (n0 < n_keys && q_begin < pr.Sq) ? (pr.Sq - q_begin + STEP - 1) / STEP : 0;
   // steps: the query blocks of each head of the group, one head after another
   const int steps = nqb * pr.G;
   const int per_split = (steps + n_split - 1) / n_split;
@@ -258,20 +276,20 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       mbar_init(do_empty(s), 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, 256);
+    mbar_init(s_free, W::COMPUTE);
     mbar_init(dp_full, 1);
-    mbar_init(p_ready, 256);
-    mbar_init(ds_ready, 256);
+    mbar_init(p_ready, W::COMPUTE);
+    mbar_init(ds_ready, W::COMPUTE);
     mbar_init(final_bar, 1);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == bwd::MMA_WARP) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == W::MMA) {
+    tmem_alloc(smem_u32(tmem_slot), W::TMEM);
     tmem_relinquish();
   }
-  if (warp == bwd::PRODUCER_WARP && lane == 0) {
+  if (warp == W::PRODUCER && lane == 0) {
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
     tma_prefetch_desc(&tm_q);
@@ -282,65 +300,80 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
-    setmaxnreg_dec<bwd::REGS_CONTROL>();
-    if (warp == bwd::PRODUCER_WARP) {
+  if (warp >= 4 * NWG) {
+    if constexpr (NWG == 2) setmaxnreg_dec<bwd::REGS_CONTROL>();
+    const uint64_t keep = policy_evict_last();
+    auto load_q = [&](int it) -> bool {
+      const int s = it % QS;
+      if (!mbar_wait(q_empty(s), ((it / QS) & 1) ^ 1, abort_flag, kErrGenDkdvProducer)) return false;
+      const int hg = (st0 + it) / nqb, q0 = q_begin + (st0 + it) % nqb * STEP;
+      mbar_arrive_expect_tx(q_full(s), L::TILE);
+      for (int sl = 0; sl < SLABS; ++sl)
+        tma_load_4d(q_addr(it) + sl * (STEP * 128), &tm_q, q_full(s), sl * 64, q0, hk * pr.G + hg, b, keep);
+      return true;
+    };
+    auto load_do = [&](int it) -> bool {  // dO with its LSE and delta
+      const int s = it % DS;
+      if (!mbar_wait(do_empty(s), ((it / DS) & 1) ^ 1, abort_flag, kErrGenDkdvProducer)) return false;
+      const int h = hk * pr.G + (st0 + it) / nqb, q0 = q_begin + (st0 + it) % nqb * STEP;
+      mbar_arrive_expect_tx(do_full(s), L::TILE + L::STAT_BYTES);
+      for (int sl = 0; sl < SLABS; ++sl)
+        tma_load_4d(do_addr(it) + sl * (STEP * 128), &tm_do, do_full(s), sl * 64, q0, h, b, keep);
+      const long long r = static_cast<long long>(b * pr.Hq + h) * rows_p + q0;
+      bulk_load(do_addr(it) + L::TILE, LSE + r, STEP * 4, do_full(s));
+      bulk_load(do_addr(it) + L::TILE + STEP * 4, DELTA + r, STEP * 4, do_full(s));
+      return true;
+    };
+    auto wait_stats = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };  // LSE and delta are written
+    if (warp == W::PRODUCER) {
       // -------------------------------------------------------------- producer: K, V, Q ring
-      if (lane == 0 && ns > 0) {
-        const uint64_t keep = policy_evict_last();
-        mbar_arrive_expect_tx(kv_full, 2 * L::TILE);
-        for (int sl = 0; sl < SLABS; ++sl) {
-          tma_load_4d(sbase + L::K_OFF + sl * 16384, &tm_k, kv_full, sl * 64, n0, hk, b, keep);
-          tma_load_4d(sbase + L::V_OFF + sl * 16384, &tm_v, kv_full, sl * 64, n0, hk, b, keep);
+      if (lane == 0) {
+        int n_q = 0, n_do = 0;
+        if (ns > 0) {
+          mbar_arrive_expect_tx(kv_full, 2 * L::KV_TILE);
+          for (int sl = 0; sl < SLABS; ++sl) {
+            tma_load_4d(sbase + L::K_OFF + sl * 16384, &tm_k, kv_full, sl * 64, n0, hk, b, keep);
+            tma_load_4d(sbase + L::V_OFF + sl * 16384, &tm_v, kv_full, sl * 64, n0, hk, b, keep);
+          }
         }
-        int it = 0;
-        for (; it < ns; ++it) {
-          const int s = it % QS;
-          if (!mbar_wait(q_empty(s), ((it / QS) & 1) ^ 1, abort_flag, kErrGenDkdvProducer)) break;
-          const int g = (st0 + it) / nqb, q0 = q_begin + (st0 + it) % nqb * 128;
-          mbar_arrive_expect_tx(q_full(s), L::TILE);
-          for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(q_addr(it) + sl * 16384, &tm_q, q_full(s), sl * 64, q0, hk * pr.G + g, b, keep);
+        bool ok = true;
+        for (int it = 0; it < ns && ok; ++it) {
+          if ((ok = load_q(it))) ++n_q;
+          if (NWG == 1 && ok) {
+            if (it == 0) wait_stats();
+            if ((ok = load_do(it))) ++n_do;
+          }
         }
+        if (NWG == 1 && ns <= 0) wait_stats();
         if (*abort_flag) {
-          mbar_wait_drain(kv_full, 0);
-          for (int x = max(0, it - QS); x < it; ++x) mbar_wait_drain(q_full(x % QS), (x / QS) & 1);
+          if (ns > 0) mbar_wait_drain(kv_full, 0);
+          for (int x = max(0, n_q - QS); x < n_q; ++x) mbar_wait_drain(q_full(x % QS), (x / QS) & 1);
+          for (int x = max(0, n_do - DS); x < n_do; ++x) mbar_wait_drain(do_full(x % DS), (x / DS) & 1);
         }
       }
-    } else if (warp == bwd::DO_PRODUCER_WARP) {
-      // -------------------------------------------------------------- producer: dO ring + lse/delta
+    } else if (warp == W::DO_PRODUCER) {
+      // -------------------------------------------------------------- producer: dO ring
       if (lane == 0) {
-        const uint64_t keep = policy_evict_last();
+        wait_stats();
         int it = 0;
-        for (; it < ns; ++it) {
-          const int s = it % DS;
-          if (!mbar_wait(do_empty(s), ((it / DS) & 1) ^ 1, abort_flag, kErrGenDkdvProducer)) break;
-          const int g = (st0 + it) / nqb, q0 = q_begin + (st0 + it) % nqb * 128;
-          const int h = hk * pr.G + g;
-          mbar_arrive_expect_tx(do_full(s), L::DO_STAGE_BYTES);
-          for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(do_addr(it) + sl * 16384, &tm_do, do_full(s), sl * 64, q0, h, b, keep);
-          const long long r = static_cast<long long>(b * pr.Hq + h) * rows_p + q0;
-          bulk_load(do_addr(it) + L::TILE, LSE + r, 512, do_full(s));
-          bulk_load(do_addr(it) + L::TILE + 512, DELTA + r, 512, do_full(s));
-        }
+        while (it < ns && load_do(it)) ++it;
         if (*abort_flag)
           for (int x = max(0, it - DS); x < it; ++x) mbar_wait_drain(do_full(x % DS), (x / DS) & 1);
       }
-    } else if (warp == bwd::MMA_WARP) {
+    } else if (warp == W::MMA) {
       // -------------------------------------------------------------- MMA issuer
-      constexpr uint32_t IDESC_SD = idesc_bf16(128, 128, false, false);  // [128 keys x 128 queries]
+      constexpr uint32_t IDESC_SD = idesc_bf16(128, STEP, false, false);  // [128 keys x STEP queries]
       constexpr uint32_t IDESC_G = idesc_bf16(128, D, false, true);      // [128 keys x D]
       const uint64_t kdesc = kmajor_desc(sbase + L::K_OFF, 128, 0), vdesc = kmajor_desc(sbase + L::V_OFF, 128, 0);
       auto issue_s = [&](int i) -> bool {  // S^T = K Q_i^T
         if (!warp_wait(q_full(i % QS), (i / QS) & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
-        const uint64_t qd = kmajor_desc(q_addr(i), 128, 0);
+        const uint64_t qd = kmajor_desc(q_addr(i), STEP, 0);
         if (elect_one()) {
           mma_ss(tmem, kdesc, qd, IDESC_SD, 0u);
 #pragma unroll
           for (int ks = 1; ks < D / 16; ++ks)
-            mma_ss_acc(tmem, kdesc + kmajor_step(128, ks), qd + kmajor_step(128, ks), IDESC_SD);
+            mma_ss_acc(tmem, kdesc + kmajor_step(128, ks), qd + kmajor_step(STEP, ks), IDESC_SD);
           mma_commit(s_full);
         }
         __syncwarp();
@@ -349,12 +382,12 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       auto issue_dp = [&](int i) -> bool {  // dP^T = V dO_i^T
         if (!warp_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
-        const uint64_t dd = kmajor_desc(do_addr(i), 128, 0);
+        const uint64_t dd = kmajor_desc(do_addr(i), STEP, 0);
         if (elect_one()) {
-          mma_ss(tmem + 128, vdesc, dd, IDESC_SD, 0u);
+          mma_ss(tmem + L::DP_COL, vdesc, dd, IDESC_SD, 0u);
 #pragma unroll
           for (int ks = 1; ks < D / 16; ++ks)
-            mma_ss_acc(tmem + 128, vdesc + kmajor_step(128, ks), dd + kmajor_step(128, ks), IDESC_SD);
+            mma_ss_acc(tmem + L::DP_COL, vdesc + kmajor_step(128, ks), dd + kmajor_step(STEP, ks), IDESC_SD);
           mma_commit(dp_full);
         }
         __syncwarp();
@@ -363,12 +396,12 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       auto issue_dv = [&](int i) -> bool {  // dV += P^T dO_i
         if (!warp_wait(p_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
-        const uint64_t dd = mnmajor_desc(do_addr(i), 128, 0);
+        const uint64_t dd = mnmajor_desc(do_addr(i), STEP, 0);
         if (elect_one()) {
-          mma_ts(tmem + 256, tmem + 128, dd, IDESC_G, i > 0 ? 1u : 0u);
+          mma_ts(tmem + L::DV_COL, tmem + L::DP_COL, dd, IDESC_G, i > 0 ? 1u : 0u);
 #pragma unroll
-          for (int ks = 1; ks < 8; ++ks)
-            mma_ts_acc(tmem + 256, bwd::packed_kstep_col(tmem + 128, ks), dd + mnmajor_step(ks), IDESC_G);
+          for (int ks = 1; ks < STEP / 16; ++ks)
+            mma_ts_acc(tmem + L::DV_COL, bwd::packed_kstep_col(tmem + L::DP_COL, ks), dd + mnmajor_step(ks), IDESC_G);
         }
         __syncwarp();
         return true;
@@ -376,12 +409,12 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       auto issue_dk = [&](int i) -> bool {  // dK += dS^T Q_i
         if (!warp_wait(ds_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
-        const uint64_t qd = mnmajor_desc(q_addr(i), 128, 0);
+        const uint64_t qd = mnmajor_desc(q_addr(i), STEP, 0);
         if (elect_one()) {
-          mma_ts(tmem + 384, tmem + 128 + 32, qd, IDESC_G, i > 0 ? 1u : 0u);
+          mma_ts(tmem + L::DK_COL, tmem + L::DP_COL + 32, qd, IDESC_G, i > 0 ? 1u : 0u);
 #pragma unroll
-          for (int ks = 1; ks < 8; ++ks)
-            mma_ts_acc(tmem + 384, bwd::packed_kstep_col(tmem + 128 + 32, ks), qd + mnmajor_step(ks), IDESC_G);
+          for (int ks = 1; ks < STEP / 16; ++ks)
+            mma_ts_acc(tmem + L::DK_COL, bwd::packed_kstep_col(tmem + L::DP_COL + 32, ks), qd + mnmajor_step(ks), IDESC_G);
           mma_commit(q_empty(i % QS));
           mma_commit(do_empty(i % DS));
         }
@@ -418,7 +451,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     }
     __syncwarp();
   } else {
-    setmaxnreg_inc<bwd::REGS_COMPUTE>();
+    if constexpr (NWG == 2) setmaxnreg_inc<bwd::REGS_COMPUTE>();
     // ---------------------------------------------------------------- compute
     const int g = warp >> 2;                 // warpgroup: query columns [64g, 64g+64) of a step
     const int row = (warp & 3) * 32 + lane;  // key row within the block
@@ -426,29 +459,30 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     const int kw = n0 + (warp & 3) * 32;  // the warp's first key
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lane_off + 64 * g;
-    const uint32_t t_dp = tmem + lane_off + 128 + 64 * g;
+    const uint32_t t_dp = tmem + lane_off + L::DP_COL + 64 * g;
     // first query that sees this key (none: past every query)
     const int q_first = kg >= n_keys ? INT_MAX : (CAUSAL ? kg - off : INT_MIN);
     const float2 c2 = make_float2(pr.scale_log2, pr.scale_log2);
     bool ok = true;
     int i = 0;
-    // heads of the group; all 256 threads pass the barriers of every head
+    // heads of the group; all compute threads pass the barriers of every head
     for (int hg = ns > 0 ? st0 / nqb : 0; i < ns || !ok; ++hg) {
       if (!ok && hg * nqb >= st0 + ns) break;
       float bias_l = 0.f, bias_r = 0.f;
       if (BIAS) {
-        ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table
-        copy_table(tab, tables, hk * pr.G + hg, bias, threadIdx.x, 256);
-        ok = named_barrier_and(2, 256, ok);
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the tables are written
+        ok = named_barrier_and(2, W::COMPUTE, ok);  // everyone is done with the last head's table
+        copy_table(tab, tables, hk * pr.G + hg, bias, threadIdx.x, W::COMPUTE);
+        ok = named_barrier_and(2, W::COMPUTE, ok);
         bias_l = tab[0];
         bias_r = tab[table_last(bias)];
       }
       const int head_end = min(ns, (hg + 1) * nqb - st0);
       for (; ok && i < head_end; ++i) {
-        const int qc = q_begin + (st0 + i - hg * nqb) * 128 + 64 * g;  // first query of this thread's columns
+        const int qc = q_begin + (st0 + i - hg * nqb) * STEP + 64 * g;  // first query of this thread's columns
         if (!(ok = warp_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvCompute))) break;
         const float* lse_s = lse_smem(i) + 64 * g;
-        const float* dl_s = lse_s + 128;
+        const float* dl_s = lse_s + STEP;
         float p[64];
         if (!(ok = warp_wait(s_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
         tc_fence_after();
@@ -542,52 +576,55 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     const bool empty = ns <= 0;
     const bool done = ok && (empty || warp_wait(final_bar, 0, abort_flag, kErrGenDkdvCompute));
     tc_fence_after();
-    if (n_split > 1) {
-      const long long r = (static_cast<long long>(split) * pr.B * pr.Hkv + cw.bh) * pr.Sk + kg;
-      if (done) {
-        write_acc_half<D>(tmem + lane_off + 256, g, dv_part + r * pr.D, pr.D, kg < pr.Sk, empty, 1.f);
-        write_acc_half<D>(tmem + lane_off + 384, g, dk_part + r * pr.D, pr.D, kg < pr.Sk, empty, pr.scale);
-      }
-    } else {
-      if (done) {
-        // every MMA has finished: the Q ring is free and holds the staged dV, dK tiles
-        stage_half<D>(tmem + lane_off + 256, g, sbase + L::Q_OFF, row, empty, 1.f);
-        stage_half<D>(tmem + lane_off + 384, g, sbase + L::Q_OFF + L::TILE, row, empty, pr.scale);
-      }
+    // every MMA has finished: K's and V's room holds the staged dV and dK tiles
+    const bool row_ok = done && kg < pr.Sk;
+    const long long r = (static_cast<long long>(split) * pr.B * pr.Hkv + b * pr.Hkv + hk) * pr.Sk + kg;
+    give_acc<D, NWG>(tmem + lane_off + L::DV_COL, g, sbase + L::K_OFF, row, n_split > 1 ? dv_part + r * pr.D : nullptr,
+                     pr.D, done, row_ok, empty, 1.f);
+    give_acc<D, NWG>(tmem + lane_off + L::DK_COL, g, sbase + L::V_OFF, row, n_split > 1 ? dk_part + r * pr.D : nullptr,
+                     pr.D, done, row_ok, empty, pr.scale);
+    if (n_split == 1) {
       const CUtensorMap* const maps[2] = {&tm_dv, &tm_dk};
-      store_staged<D, 2>(done, maps, sbase + L::Q_OFF, n0, hk, b);
+      store_staged<D, NWG, 2>(done, maps, sbase + L::K_OFF, n0, hk, b);
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == bwd::MMA_WARP) {
+  if (warp == W::MMA) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, W::TMEM);
   }
 }
 
 // ====================================================================================
 // dQ and dbias
 // ====================================================================================
-template <int D, bool BIAS>
+template <int D, int NWG, bool BIAS>
 struct DqLayout {
-  static constexpr int TILE = 128 * D * 2;
+  static constexpr int STEP = 64 * NWG;
+  static constexpr int TILE = STEP * D * 2;
   static constexpr int K_STAGES = (BIAS && D == 128) ? 3 : 4;  // the bias part takes one slot's room
   static constexpr int V_STAGES = 3;
-  static constexpr int K_OFF = 0;
+  static constexpr int K_OFF = 0;  // also stages the output: 128 rows in two slots at least
   static constexpr int V_OFF = K_OFF + K_STAGES * TILE;
-  static constexpr int TAB_OFF = V_OFF + V_STAGES * TILE;
-  // bias: table (fp32 by position), buckets by position, per-warp sums, diagonal scratch
-  static constexpr int LUT_OFF = TAB_OFF + (kTableMax * 4 + 15) / 16 * 16;
-  static constexpr int SUM_OFF = LUT_OFF + (2 * kMaxDistance + 8) * 2;
-  static constexpr int DIAG_OFF = SUM_OFF + 8 * kMaxBuckets * 4;
-  static constexpr int BAR_OFF = BIAS ? DIAG_OFF + 8 * 96 * 4 : TAB_OFF;
+  // tensor memory: S, dP (dS is written over it), dQ, then Q and dO as packed A operands
+  static constexpr uint32_t DP = STEP, DQ = 2 * STEP, Q = 2 * STEP + D, DO = 2 * STEP + D + D / 2;
+  static constexpr int BAR_OFF = V_OFF + V_STAGES * TILE;
   // qd_ready, k_full[], k_empty[], v_full[3], v_empty[3], s_full, s_free, dp_full, ds_ready,
   // final, drain
   static constexpr int NBARS = 1 + 2 * K_STAGES + 2 * V_STAGES + 6;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
-  static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
+  static constexpr int DELTA_OFF = (MISC_OFF + 16 + 15) / 16 * 16;  // delta of the block's rows
+  // bias: diagonal scratch of each warp, table (fp32 by position), buckets by position,
+  // per-warp sums
+  static constexpr int DIAG_OFF = DELTA_OFF + 512;
+  static constexpr int TAB_OFF = DIAG_OFF + (BIAS ? 4 * NWG * 96 * 4 : 0);
+  static int smem_bytes(const Bias& bias) {
+    return TAB_OFF + (BIAS ? table_size(bias) * 4 + lut_size(bias) * 2 + 4 * NWG * bias.buckets * 4 : 0) + 1024;
+  }
+  // at most, with kMaxDistance and kMaxBuckets
+  static constexpr int MOST = TAB_OFF + (BIAS ? kTableMax * 4 + (2 * kMaxDistance + 8) * 2 + 4 * NWG * kMaxBuckets * 4 : 0) + 1024;
 };
 
 // Copy this thread's row of `true_d` bf16 values into D/2 packed TMEM columns (the rest
@@ -609,6 +646,36 @@ __device__ __forceinline__ void row_to_tmem(const __nv_bfloat16* __restrict__ sr
     }
     tmem_st32(taddr + 32 * c, w);
   }
+}
+
+// The same, and the row's dot product with `other`.
+template <int D>
+__device__ __forceinline__ float row_dot_to_tmem(const __nv_bfloat16* __restrict__ src,
+                                                 const __nv_bfloat16* __restrict__ other, bool valid, int true_d,
+                                                 uint32_t taddr) {
+  float acc = 0.f;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    uint32_t w[32];
+    const uint4 *s4 = reinterpret_cast<const uint4*>(src + 64 * c), *o4 = reinterpret_cast<const uint4*>(other + 64 * c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = valid && 64 * c + 8 * e < true_d;
+      const uint4 x = in ? __ldg(s4 + e) : make_uint4(0u, 0u, 0u, 0u);
+      const uint4 y = in ? __ldg(o4 + e) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        w[4 * e + u] = xs[u];
+        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&xs[u]));
+        const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ys[u]));
+        acc = fmaf(a.x, b.x, acc);
+        acc = fmaf(a.y, b.y, acc);
+      }
+    }
+    tmem_st32(taddr + 32 * c, w);
+  }
+  return acc;
 }
 
 // Add the diagonal sums of a warp's 32 x 64 block of dS (lane = row, ds[e] = column e) to
@@ -652,18 +719,18 @@ __device__ __forceinline__ void add_near_block(const float (&ds)[64], int r0, co
   }
 }
 
-template <int D, bool CAUSAL, bool BIAS>
-__global__ void __launch_bounds__(bwd::NTHREADS, 1)
+template <int D, int NWG, bool CAUSAL, bool BIAS>
+__global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     ffa_gen_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ Problem pr,
                       const __grid_constant__ Bias bias, const float* __restrict__ tables,
-                      const unsigned short* __restrict__ lut_g, const View q, const View dout,
-                      const float* __restrict__ LSE,
-                      const float* __restrict__ DELTA, float* __restrict__ dq_part, float* __restrict__ bias_part,
+                      const unsigned short* __restrict__ lut_g, const View q, const View o, const View dout,
+                      const float* __restrict__ LSE, float* __restrict__ lse_out, float* __restrict__ delta_out,
+                      float* __restrict__ dq_part, float* __restrict__ bias_part,
                       int n_split, int group) {
-  using L = DqLayout<D, BIAS>;
-  using T = DqTmem<D>;
-  constexpr int SLABS = D / 64;
+  using L = DqLayout<D, NWG, BIAS>;
+  using W = BwdWidth<NWG>;
+  constexpr int SLABS = D / 64, STEP = L::STEP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -682,9 +749,10 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
   const uint32_t drain_bar = s_full + 40;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
+  float* delta_s = reinterpret_cast<float*>(smem + L::DELTA_OFF);
   float* tab = reinterpret_cast<float*>(smem + L::TAB_OFF);
-  unsigned short* lut = reinterpret_cast<unsigned short*>(smem + L::LUT_OFF);
-  float* sums_all = reinterpret_cast<float*>(smem + L::SUM_OFF);
+  unsigned short* lut = reinterpret_cast<unsigned short*>(tab + (BIAS ? table_size(bias) : 0));
+  float* sums_all = reinterpret_cast<float*>(lut + (BIAS ? lut_size(bias) : 0));
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -693,18 +761,19 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
   const CtaWork cw = cta_work(nblk * n_split, pr.B * pr.Hq, group);
   const int qblk = CAUSAL ? nblk - 1 - cw.rank / n_split : cw.rank / n_split;
   const int split = cw.rank % n_split;
-  const int b = cw.bh / pr.Hq, h = cw.bh % pr.Hq, hk = h / pr.G;
+  const int b = pr.seq_at(cw.bh / pr.Hq), h = cw.bh % pr.Hq, hk = h / pr.G;
+  const int bh = b * pr.Hq + h;
   const int m0 = qblk * 128;
   const int off = (CAUSAL || BIAS) ? pr.offset(b) : 0;
   const int n_keys = pr.keys(b, off, CAUSAL);
   const int end = CAUSAL ? min(n_keys, max(off + m0 + 128, 0)) : n_keys;
-  const int all = (end + 127) / 128;
+  const int all = (end + STEP - 1) / STEP;
   const int per_split = (all + n_split - 1) / n_split;
   const int t0 = min(split * per_split, all);
   const int nk = min(per_split, all - t0);
 
   if (threadIdx.x == 0) {
-    mbar_init(qd_ready, 256);
+    mbar_init(qd_ready, W::COMPUTE);
     for (int s = 0; s < KS; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(k_empty(s), 1);
@@ -714,36 +783,33 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       mbar_init(v_empty(s), 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, 256);
+    mbar_init(s_free, W::COMPUTE);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 256);
+    mbar_init(ds_ready, W::COMPUTE);
     mbar_init(final_bar, 1);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == bwd::MMA_WARP) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == W::MMA) {
+    tmem_alloc(smem_u32(tmem_slot), W::TMEM);
     tmem_relinquish();
   }
-  if (warp == bwd::PRODUCER_WARP && lane == 0) {
+  if (warp == W::PRODUCER && lane == 0) {
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (BIAS && warp < 8) {
-    copy_table(tab, tables, h, bias, threadIdx.x, 256);
-    for (int t = threadIdx.x; t < lut_size(bias) / 2; t += 256)
-      reinterpret_cast<uint32_t*>(lut)[t] = reinterpret_cast<const uint32_t*>(lut_g)[t];
-    for (int t = threadIdx.x; t < 8 * bias.buckets; t += 256) sums_all[t] = 0.f;
-  }
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (BIAS && warp < 4 * NWG)
+    for (int t = threadIdx.x; t < 4 * NWG * bias.buckets; t += W::COMPUTE) sums_all[t] = 0.f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
-    setmaxnreg_dec<bwd::REGS_CONTROL>();
-    if (warp == bwd::PRODUCER_WARP) {
+  if (warp >= 4 * NWG) {
+    if constexpr (NWG == 2) setmaxnreg_dec<bwd::REGS_CONTROL>();
+    if (warp == W::PRODUCER) {
       // -------------------------------------------------------------- producer: K, V rings
       if (lane == 0) {
         const uint64_t keep = policy_evict_last();
@@ -753,13 +819,13 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
           if (!mbar_wait(k_empty(sk), ((j / KS) & 1) ^ 1, abort_flag, kErrGenDqProducer)) break;
           mbar_arrive_expect_tx(k_full(sk), L::TILE);
           for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(sbase + L::K_OFF + sk * L::TILE + sl * 16384, &tm_k, k_full(sk), sl * 64, (t0 + j) * 128, hk, b,
+            tma_load_4d(sbase + L::K_OFF + sk * L::TILE + sl * (STEP * 128), &tm_k, k_full(sk), sl * 64, (t0 + j) * STEP, hk, b,
                         keep);
           ++k_issued;
           if (!mbar_wait(v_empty(sv), ((j / VS) & 1) ^ 1, abort_flag, kErrGenDqProducer)) break;
           mbar_arrive_expect_tx(v_full(sv), L::TILE);
           for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(sbase + L::V_OFF + sv * L::TILE + sl * 16384, &tm_v, v_full(sv), sl * 64, (t0 + j) * 128, hk, b,
+            tma_load_4d(sbase + L::V_OFF + sv * L::TILE + sl * (STEP * 128), &tm_v, v_full(sv), sl * 64, (t0 + j) * STEP, hk, b,
                         keep);
           ++v_issued;
         }
@@ -768,27 +834,27 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
           for (int it = max(0, v_issued - VS); it < v_issued; ++it) mbar_wait_drain(v_full(it % VS), (it / VS) & 1);
         }
       }
-    } else if (warp == bwd::MMA_WARP) {
+    } else if (warp == W::MMA) {
       // -------------------------------------------------------------- MMA issuer
-      constexpr uint32_t IDESC_SD = idesc_bf16(128, 128, false, false);  // [128 queries x 128 keys]
+      constexpr uint32_t IDESC_SD = idesc_bf16(128, STEP, false, false);  // [128 queries x STEP keys]
       constexpr uint32_t IDESC_G = idesc_bf16(128, D, false, true);      // [128 queries x D]
       auto k_addr = [&](int j) { return sbase + L::K_OFF + (j % KS) * L::TILE; };
       auto v_addr = [&](int j) { return sbase + L::V_OFF + (j % VS) * L::TILE; };
       // rows behind the last key are zeroed before the first MMA that reads the tile
       auto fix_tail = [&](uint32_t tile, int j) {
-        const int tail = n_keys - (t0 + j) * 128;
-        if (tail < 128 && n_keys < pr.Sk) zero_tail(tile, SLABS, tail, lane);
+        const int tail = n_keys - (t0 + j) * STEP;
+        if (tail < STEP && n_keys < pr.Sk) zero_tail<STEP>(tile, SLABS, tail, lane);
       };
       auto issue_s = [&](int j) -> bool {  // S_j = Q K_j^T  (Q from TMEM)
         if (!warp_wait(k_full(j % KS), (j / KS) & 1, abort_flag, kErrGenDqMma)) return false;
         fix_tail(k_addr(j), j);
         tc_fence_after();
-        const uint64_t kd = kmajor_desc(k_addr(j), 128, 0);
+        const uint64_t kd = kmajor_desc(k_addr(j), STEP, 0);
         if (elect_one()) {
-          mma_ts(tmem + T::S, tmem + T::Q, kd, IDESC_SD, 0u);
+          mma_ts(tmem, tmem + L::Q, kd, IDESC_SD, 0u);
 #pragma unroll
           for (int ks = 1; ks < D / 16; ++ks)
-            mma_ts_acc(tmem + T::S, tmem + T::Q + 8 * ks, kd + kmajor_step(128, ks), IDESC_SD);
+            mma_ts_acc(tmem, tmem + L::Q + 8 * ks, kd + kmajor_step(STEP, ks), IDESC_SD);
           mma_commit(s_full);
         }
         __syncwarp();
@@ -798,12 +864,12 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         if (!warp_wait(v_full(j % VS), (j / VS) & 1, abort_flag, kErrGenDqMma)) return false;
         fix_tail(v_addr(j), j);
         tc_fence_after();
-        const uint64_t vd = kmajor_desc(v_addr(j), 128, 0);
+        const uint64_t vd = kmajor_desc(v_addr(j), STEP, 0);
         if (elect_one()) {
-          mma_ts(tmem + T::DP, tmem + T::DO, vd, IDESC_SD, 0u);
+          mma_ts(tmem + L::DP, tmem + L::DO, vd, IDESC_SD, 0u);
 #pragma unroll
           for (int ks = 1; ks < D / 16; ++ks)
-            mma_ts_acc(tmem + T::DP, tmem + T::DO + 8 * ks, vd + kmajor_step(128, ks), IDESC_SD);
+            mma_ts_acc(tmem + L::DP, tmem + L::DO + 8 * ks, vd + kmajor_step(STEP, ks), IDESC_SD);
           mma_commit(dp_full);
           mma_commit(v_empty(j % VS));
         }
@@ -815,10 +881,10 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         tc_fence_after();
         const uint64_t kd = mnmajor_desc(k_addr(j), 128, 0);
         if (elect_one()) {
-          mma_ts(tmem + T::DQ, tmem + T::DP, kd, IDESC_G, j > 0 ? 1u : 0u);
+          mma_ts(tmem + L::DQ, tmem + L::DP, kd, IDESC_G, j > 0 ? 1u : 0u);
 #pragma unroll
-          for (int ks = 1; ks < 8; ++ks)
-            mma_ts_acc(tmem + T::DQ, bwd::packed_kstep_col(tmem + T::DP, ks), kd + mnmajor_step(ks), IDESC_G);
+          for (int ks = 1; ks < STEP / 16; ++ks)
+            mma_ts_acc(tmem + L::DQ, bwd::packed_kstep_col(tmem + L::DP, ks), kd + mnmajor_step(ks), IDESC_G);
           mma_commit(k_empty(j % KS));
         }
         __syncwarp();
@@ -847,28 +913,46 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
     }
     __syncwarp();
   } else {
-    setmaxnreg_inc<bwd::REGS_COMPUTE>();
+    if constexpr (NWG == 2) setmaxnreg_inc<bwd::REGS_COMPUTE>();
     // ---------------------------------------------------------------- compute
     const int g = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // query row within the block
     const int qg = m0 + row;
     const int qw = m0 + (warp & 3) * 32;  // the warp's first query
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    {
-      // warpgroup 0 puts the block's Q rows into tensor memory, warpgroup 1 its dO rows
-      const View& src = g ? dout : q;
-      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(src.p) + b * src.sb + h * src.sh +
-                               static_cast<long long>(qg < pr.Sq ? qg : 0) * src.ss;
-      row_to_tmem<D>(p, qg < pr.Sq, pr.D, tmem + lane_off + (g ? T::DO : T::Q));
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(qd_ready);
+    // Q and dO rows into tensor memory (two warpgroups: one each), and delta = O . dO on the way
+    const bool row_in = qg < pr.Sq;
+    auto row_of = [&](const View& x) {
+      return static_cast<const __nv_bfloat16*>(x.p) + b * x.sb + h * x.sh + static_cast<long long>(row_in ? qg : 0) * x.ss;
+    };
+    float dl = 0.f;
+    if (NWG == 1 || g == 0) row_to_tmem<D>(row_of(q), row_in, pr.D, tmem + lane_off + L::Q);
+    if (NWG == 1 || g == 1) dl = row_dot_to_tmem<D>(row_of(dout), row_of(o), row_in, pr.D, tmem + lane_off + L::DO);
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive(qd_ready);
+    // +inf for a row that saw no key and for rows behind the last one: their P is 0
+    float lse = row_in ? LSE[static_cast<long long>(bh) * pr.Sq + qg] : INFINITY;
+    if (lse == -INFINITY) lse = INFINITY;
+    if (NWG == 1 || g == 1) {
+      if (NWG == 2) delta_s[row] = dl;
+      if (split == 0) {
+        const long long r = static_cast<long long>(bh) * padded_rows(pr.Sq) + qg;
+        lse_out[r] = lse;
+        delta_out[r] = dl;
+      }
     }
-    const long long ridx = static_cast<long long>(cw.bh) * padded_rows(pr.Sq) + qg;
-    const float lse = LSE[ridx], dl = DELTA[ridx];
+    if (BIAS) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the tables are written
+      copy_table(tab, tables, h, bias, threadIdx.x, W::COMPUTE);
+      for (int t = threadIdx.x; t < lut_size(bias) / 2; t += W::COMPUTE)
+        reinterpret_cast<uint32_t*>(lut)[t] = reinterpret_cast<const uint32_t*>(lut_g)[t];
+    }
+    if (BIAS || NWG == 2) named_barrier_and(2, W::COMPUTE, true);
+    if (NWG == 2) dl = delta_s[row];
     const int lim = CAUSAL ? min(n_keys - 1, qg + off) : n_keys - 1;  // last visible key
-    const uint32_t t_s = tmem + lane_off + T::S + 64 * g;
-    const uint32_t t_dp = tmem + lane_off + T::DP + 64 * g;
+    const uint32_t t_s = tmem + lane_off + 64 * g;
+    const uint32_t t_dp = tmem + lane_off + L::DP + 64 * g;
     float* sums = sums_all + warp * bias.buckets;
     float* diag = reinterpret_cast<float*>(smem + L::DIAG_OFF) + warp * 96;
     float bias_l = 0.f, bias_r = 0.f, sum_l = 0.f, sum_r = 0.f;
@@ -884,7 +968,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
       bwd::tmem_ld64(t_s, p);
       tc_fence_before();
       mbar_arrive(s_free);  // S may now be overwritten by S(j+1)
-      const int kc = (t0 + j) * 128 + 64 * g;  // first key of this thread's columns
+      const int kc = (t0 + j) * STEP + 64 * g;  // first key of this thread's columns
       const bool masked = kc + 64 > n_keys || (CAUSAL && kc + 63 > qw + off);
       bool near = false, right = false;
       float fb = 0.f;
@@ -978,33 +1062,31 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1)
         sums[lut[0]] += sum_l;
         sums[lut[bias.left + bias.right]] += sum_r;
       }
-      if (named_barrier_and(2, 256, done)) {
-        float* dst = bias_part + (static_cast<long long>(cw.bh) * nblk * n_split + cw.rank) * bias.buckets;
-        for (int u = threadIdx.x; u < bias.buckets; u += 256) {
+      if (named_barrier_and(2, W::COMPUTE, done)) {
+        float* dst = bias_part + (static_cast<long long>(bh) * nblk * n_split + cw.rank) * bias.buckets;
+        for (int u = threadIdx.x; u < bias.buckets; u += W::COMPUTE) {
           float a = 0.f;
 #pragma unroll
-          for (int w = 0; w < 8; ++w) a += sums_all[w * bias.buckets + u];
+          for (int w = 0; w < 4 * NWG; ++w) a += sums_all[w * bias.buckets + u];
           dst[u] = a;
         }
       }
     }
-    if (n_split > 1) {
-      const long long r = (static_cast<long long>(split) * pr.B * pr.Hq + cw.bh) * pr.Sq + qg;
-      if (done)
-        write_acc_half<D>(tmem + lane_off + T::DQ, g, dq_part + r * pr.D, pr.D, qg < pr.Sq, empty, pr.scale);
-    } else {
-      // every MMA has finished: the K ring is free and holds the staged dQ tile
-      if (done) stage_half<D>(tmem + lane_off + T::DQ, g, sbase + L::K_OFF, row, empty, pr.scale);
+    // every MMA has finished: the K ring is free and holds the staged dQ tile
+    const long long r = (static_cast<long long>(split) * pr.B * pr.Hq + bh) * pr.Sq + qg;
+    give_acc<D, NWG>(tmem + lane_off + L::DQ, g, sbase + L::K_OFF, row, n_split > 1 ? dq_part + r * pr.D : nullptr, pr.D,
+                     done, done && row_in, empty, pr.scale);
+    if (n_split == 1) {
       const CUtensorMap* const maps[1] = {&tm_dq};
-      store_staged<D, 1>(done, maps, sbase + L::K_OFF, m0, h, b);
+      store_staged<D, NWG, 1>(done, maps, sbase + L::K_OFF, m0, h, b);
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == bwd::MMA_WARP) {
+  if (warp == W::MMA) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, W::TMEM);
   }
 }
 

@@ -33,6 +33,21 @@ struct Problem {
     if (causal) n = min(n, max(off + Sq, 0));
     return n;
   }
+  // The sequence whose CTAs come at place `pos`.  Where lengths differ, each 32 sequences
+  // are taken longest first, so that the launch does not end on a long one.  The whole warp
+  // calls it.
+  __device__ __forceinline__ int seq_at(int pos) const {
+    if (key_lengths == nullptr || B == 1) return pos;
+    const int lane = threadIdx.x & 31, first = pos & ~31;
+    const int n = first + lane < B ? min(key_lengths[first + lane], Sk) : -1;
+    int rank = 0;  // sequences of the 32 that come before this lane's
+#pragma unroll 8
+    for (int x = 0; x < 32; ++x) {
+      const int y = __shfl_sync(0xffffffffu, n, x);
+      rank += y > n || (y == n && x < lane);
+    }
+    return first + __ffs(__ballot_sync(0xffffffffu, rank == pos - first)) - 1;
+  }
   __device__ __forceinline__ int offset(int b) const {
     return query_offsets ? min(max(query_offsets[b], -kOffsetLimit), kOffsetLimit) : query_offset;
   }

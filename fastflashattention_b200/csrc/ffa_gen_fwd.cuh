@@ -63,7 +63,7 @@ __device__ __forceinline__ float row_max64(const uint32_t (&a)[32], const uint32
   return fmax3(fmax3(y0, y1, y2), fmax3(y3, y4, x[15]), y0);
 }
 
-template <int D, bool CAUSAL, bool BIAS, int EMU = fwd::emu_pairs<D>()>
+template <int D, bool CAUSAL, bool BIAS, int EMU = D == 64 ? 2 : 0>
 __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
     ffa_gen_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
   const CtaWork cw = cta_work(n_mblk * n_split, pr.B * pr.Hq, group);
   const int mblk = CAUSAL ? n_mblk - 1 - cw.rank / n_split : cw.rank / n_split;
   const int split = cw.rank % n_split;
-  const int b = cw.bh / pr.Hq, h = cw.bh % pr.Hq, hk = h / pr.G;
+  const int b = pr.seq_at(cw.bh / pr.Hq), h = cw.bh % pr.Hq, hk = h / pr.G;
   const int m0 = mblk * L::ROWS;
   const int off = (CAUSAL || BIAS) ? pr.offset(b) : 0;
   const int n_keys = pr.keys(b, off, CAUSAL);
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
     if constexpr (D == 128) setmaxnreg_dec<fwd::REGS_CONTROL>();
     if (warp == PRODUCER) {
       // ---------------------------------------------------------------- producer
+      if (BIAS && n_kv == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // as below: the launch ends after the tables'
       if (lane == 0 && n_kv > 0) {
         const uint64_t keep = policy_evict_last();
         mbar_arrive_expect_tx(q_full, NT * L::Q_TILE);
