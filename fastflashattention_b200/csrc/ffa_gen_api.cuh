@@ -198,7 +198,6 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias) {
 }
 
 struct BwdPlan {
-  bool narrow;  // 64-wide steps, two CTAs to an SM
   int dq_split, dkdv_split;
   long long stat_floats;              // LSE and delta, each
   long long dq_off, dk_off, dv_off;   // offsets in floats; all regions start 256-byte aligned
@@ -210,8 +209,7 @@ inline BwdPlan bwd_plan(const ffa_gen_problem* p, const Bias& bias) {
   const long long hq = static_cast<long long>(p->batch) * p->q_heads, hk = static_cast<long long>(p->batch) * p->kv_heads;
   const long long qb = ceil_div(p->q_len, 128), kb = ceil_div(p->k_len, 128);
   const long long g = p->kv_heads ? p->q_heads / p->kv_heads : 1;
-  w.narrow = p->head_dim <= 64;
-  const int slots = w.narrow ? 2 * kSMs : kSMs;
+  const int slots = p->head_dim <= 64 ? 2 * kSMs : kSMs;
   w.dq_split = split_of(hq * qb, slots, kb, 4);
   w.dkdv_split = split_of(hk * kb, slots, g * qb, 4);
   auto round64 = [](long long n) { return (n + 63) / 64 * 64; };
@@ -352,10 +350,10 @@ static int launch_gen_step(const Call& c, const FwdPlan& f, float* ws) {
                                : launch_gen_step_rg<D, 1, false, CAUSAL, BIAS>(c, f, ws);
 }
 
-template <int D, int NWG, bool CAUSAL, bool BIAS>
+template <int D, bool CAUSAL, bool BIAS>
 static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
-  using L = DkdvLayout<D, NWG, BIAS>;
-  using W = BwdWidth<NWG>;
+  using L = DkdvLayout<D, BIAS>;
+  using W = BwdShape<D>;
   const Problem& pr = c.pr;
   CUtensorMap tk, tv, tq, tdo, tdk, tdv;
   int rc;
@@ -365,14 +363,14 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   if ((rc = make_map(&tdv, c.dv, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
   tq = tdo = tk;  // without queries nothing is loaded through them
   if (pr.Sq > 0) {
-    if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D, L::STEP))) return rc;
-    if ((rc = make_map(&tdo, c.dout, pr.B, pr.Hq, pr.Sq, pr.D, L::STEP))) return rc;
+    if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D, W::STEP))) return rc;
+    if ((rc = make_map(&tdo, c.dout, pr.B, pr.Hq, pr.Sq, pr.D, W::STEP))) return rc;
   }
-  auto kern = ffa_gen_dkdv_kernel<D, NWG, CAUSAL, BIAS>;
+  auto kern = ffa_gen_dkdv_kernel<D, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
   constexpr int most = L::TAB_OFF + (BIAS ? kTableMax * 4 : 0);
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
-  if constexpr (NWG == 2) {
+  if constexpr (D == 128) {
     static bool configured_regs = false;
     if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs)))
       return rc;
@@ -390,23 +388,23 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   return launched();
 }
 
-template <int D, int NWG, bool CAUSAL, bool BIAS>
+template <int D, bool CAUSAL, bool BIAS>
 static int launch_gen_dq(const Call& c, const BwdPlan& w, float* ws) {
-  using L = DqLayout<D, NWG, BIAS>;
-  using W = BwdWidth<NWG>;
+  using L = DqLayout<D, BIAS>;
+  using W = BwdShape<D>;
   const Problem& pr = c.pr;
   CUtensorMap tk, tv, tdq;
   int rc;
   if ((rc = make_map(&tdq, c.dq, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
   tk = tv = tdq;  // without keys nothing is loaded through them
   if (pr.Sk > 0) {
-    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D, L::STEP))) return rc;
-    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D, L::STEP))) return rc;
+    if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D, W::STEP))) return rc;
+    if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D, W::STEP))) return rc;
   }
-  auto kern = ffa_gen_dq_kernel<D, NWG, CAUSAL, BIAS>;
+  auto kern = ffa_gen_dq_kernel<D, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::MOST, &configured))) return rc;
-  if constexpr (NWG == 2) {
+  if constexpr (D == 128) {
     static bool configured_regs = false;
     if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs)))
       return rc;
@@ -446,19 +444,11 @@ struct RunStep {
 };
 template <int D, bool C, bool B>
 struct RunDkdv {
-  static int run(const Call& c, const BwdPlan& w, float* ws) {
-    if constexpr (D == 64)
-      if (w.narrow) return launch_gen_dkdv<D, 1, C, B>(c, w, ws);
-    return launch_gen_dkdv<D, 2, C, B>(c, w, ws);
-  }
+  static int run(const Call& c, const BwdPlan& w, float* ws) { return launch_gen_dkdv<D, C, B>(c, w, ws); }
 };
 template <int D, bool C, bool B>
 struct RunDq {
-  static int run(const Call& c, const BwdPlan& w, float* ws) {
-    if constexpr (D == 64)
-      if (w.narrow) return launch_gen_dq<D, 1, C, B>(c, w, ws);
-    return launch_gen_dq<D, 2, C, B>(c, w, ws);
-  }
+  static int run(const Call& c, const BwdPlan& w, float* ws) { return launch_gen_dq<D, C, B>(c, w, ws); }
 };
 
 }  // namespace gen

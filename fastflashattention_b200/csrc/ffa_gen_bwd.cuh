@@ -9,13 +9,14 @@
 //   * delta comes from the dQ kernel, which has dO in hand; dK/dV follows it, launched while it
 //     still runs (programmatic dependent launch).  Without a wish for dQ,
 //     ffa_gen_prepare_kernel writes delta;
-//   * two widths of a step at head dims up to 64.  Wide (NWG = 2): 128 columns, two compute
-//     warpgroups, one CTA to an SM.  Narrow (NWG = 1): 64 columns, one warpgroup, 256 columns
-//     of tensor memory, two CTAs to an SM that fill each other's start, end and waits;
+//   * head dims up to 64 walk 64 columns a step instead of 128: 256 columns of tensor memory
+//     and two CTAs to an SM, with 32 columns a thread.  The loop of a CTA is a chain of waits
+//     (S, exponentials, dP, dS, MMAs); two CTAs and four warps to a scheduler fill each
+//     other's;
 //   * the dK/dV kernel walks the queries of all heads of its key head, one after another, so
 //     a shared key head's gradients are summed in tensor memory;
 //   * P = 0 outside the mask, and K / V rows behind the last key are zeroed in shared memory;
-//   * dbias rides on the dQ kernel, whose threads hold dS in fp32.  A 32 x 64 block of dS far
+//   * dbias rides on the dQ kernel, whose threads hold dS in fp32.  A warp's block of dS (32 rows) far
 //     from the diagonal lies in one bucket: a plain sum.  A near block is summed along its
 //     diagonals (one shuffle and one add a column: lane l passes its partial sum of a
 //     diagonal to lane l + 1), then by bucket; each warp has its own sums, each CTA its own
@@ -117,16 +118,16 @@ __device__ __forceinline__ void copy_table(float* tab, const float* tables, int 
   for (int t = tid; t < units; t += n) reinterpret_cast<float4*>(tab)[t] = src[t];
 }
 
-// Give this lane's share of an accumulator (warpgroup g of NWG: D / NWG columns), times
+// Give this lane's share of an accumulator (half of the columns for warpgroup g), times
 // `mul`, to the staged bf16 tile (128 rows, for a TMA store) or, with `part`, to an fp32 row
 // of `true_d` values.  `empty`: nothing was accumulated, and tensor memory may hold
 // anything: zeros.  The whole warp calls it.
-template <int D, int NWG>
+template <int D>
 __device__ __forceinline__ void give_acc(uint32_t t_acc, int g, uint32_t tile, int row, float* part, int true_d,
                                          bool done, bool row_ok, bool empty, float mul) {
   if (!done) return;
 #pragma unroll 1
-  for (int c = g * (D / NWG); c < (g + 1) * (D / NWG); c += 32) {
+  for (int c = g * (D / 2); c < (g + 1) * (D / 2); c += 32) {
     uint32_t r[32];
     if (empty) {
 #pragma unroll
@@ -144,11 +145,11 @@ __device__ __forceinline__ void give_acc(uint32_t t_acc, int g, uint32_t tile, i
 
 // Barrier of the compute threads, then one TMA store of each staged tile (see
 // bwd::store_staged).
-template <int D, int NWG, int NT>
+template <int D, int NT>
 __device__ __forceinline__ void store_staged(bool staged, const CUtensorMap* const (&maps)[NT], uint32_t first_tile,
                                              int row0, int h, int b) {
   fence_proxy_async_smem();
-  const bool all = named_barrier_and(1, 128 * NWG, staged);
+  const bool all = named_barrier_and(1, 256, staged);
   if (all && threadIdx.x == 0) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -163,23 +164,46 @@ __device__ __forceinline__ void store_staged(bool staged, const CUtensorMap* con
 // ====================================================================================
 // dK / dV
 // ====================================================================================
-// Threads, registers and roles of the two widths.  Narrow CTAs share the registers evenly;
-// the wide one moves them to its compute warpgroups (see ffa_bwd.cuh).
-template <int NWG>
-struct BwdWidth {
-  static constexpr int STEP = 64 * NWG;
-  static constexpr int COMPUTE = 128 * NWG;  // threads
-  // warps; dK/dV: narrow CTAs have one producer for both rings (twelve warps of two CTAs leave
-  // each thread 168 registers, fourteen would leave 128)
-  static constexpr int PRODUCER = 4 * NWG, MMA = 4 * NWG + 1, DO_PRODUCER = NWG == 2 ? 10 : -1;
-  static constexpr int THREADS = NWG == 2 ? bwd::NTHREADS : 192;
-  static constexpr int CTAS = NWG == 2 ? 1 : 2;
-  static constexpr int TMEM = NWG == 2 ? 512 : 256;
+// Of every 4 groups of 4 exponentials, how many go to the FMA pipe instead of MUFU.EX2.  None
+// is best without a bias (B4 H16 S4096 D128: 1471 us against 1535), one with it (1816 us
+// against 1915, and 208 against 214 at B8 H12 S1024 D64).
+constexpr int bwd_emu(bool bias) { return bias ? 1 : 0; }
+
+// Shape of a CTA: two compute warpgroups, each with CW columns of a step (thread = TMEM lane
+// = row), then the control warps.  At D = 128 setmaxnreg moves registers from those to the
+// compute warpgroups (see ffa_bwd.cuh); at D = 64 all threads have the same.
+template <int D>
+struct BwdShape {
+  static constexpr int CW = D == 64 ? 32 : 64;
+  static constexpr int STEP = 2 * CW;
+  static constexpr int CTAS = D == 64 ? 2 : 1;  // of an SM
+  static constexpr int TMEM = D == 64 ? 256 : 512;
+  static constexpr int THREADS = D == 64 ? 320 : bwd::NTHREADS;
+  static constexpr int PRODUCER = 8, MMA = 9, DO_PRODUCER = D == 64 ? -1 : 10;  // warps
 };
 
-template <int D, int NWG, bool BIAS>
+// TMEM column of the 16-deep K-step `ks` of a packed-bf16 A operand that the two warpgroups
+// wrote, CW values each (CW / 2 columns, CW columns apart).
+template <int CW>
+__device__ __forceinline__ constexpr uint32_t kstep_col(int ks) {
+  return (ks / (CW / 16)) * CW + (ks % (CW / 16)) * 8;
+}
+
+// Load / store N (16, 32 or 64) consecutive columns of this lane.
+__device__ __forceinline__ void ld_cols(uint32_t taddr, float (&v)[64]) { bwd::tmem_ld64(taddr, v); }
+__device__ __forceinline__ void ld_cols(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ld32(taddr, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+}
+__device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
+__device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
+
+template <int D, bool BIAS>
 struct DkdvLayout {
-  static constexpr int STEP = 64 * NWG;
+  static constexpr int STEP = BwdShape<D>::STEP;
   static constexpr int KV_TILE = 128 * D * 2;   // K, V (resident)
   static constexpr int TILE = STEP * D * 2;     // Q, dO (streamed)
   // three Q slots, as in the plain kernel; at D = 128 the bias table takes the third's room
@@ -203,8 +227,8 @@ struct DkdvLayout {
   static int smem_bytes(const Bias& bias) { return TAB_OFF + (BIAS ? table_size(bias) * 4 : 0); }
 };
 
-template <int D, int NWG, bool CAUSAL, bool BIAS>
-__global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
+template <int D, bool CAUSAL, bool BIAS, int EMU = bwd_emu(BIAS)>
+__global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     ffa_gen_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                         const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
@@ -212,9 +236,9 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
                         const float* __restrict__ tables, const float* __restrict__ LSE,
                         const float* __restrict__ DELTA, float* __restrict__ dk_part,
                         float* __restrict__ dv_part, int n_split, int group) {
-  using L = DkdvLayout<D, NWG, BIAS>;
-  using W = BwdWidth<NWG>;
-  constexpr int SLABS = D / 64, STEP = L::STEP;
+  using L = DkdvLayout<D, BIAS>;
+  using W = BwdShape<D>;
+  constexpr int SLABS = D / 64, STEP = W::STEP, CW = W::CW;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023u) {  // the layout has no room to realign: report and leave
@@ -276,10 +300,10 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       mbar_init(do_empty(s), 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, W::COMPUTE);
+    mbar_init(s_free, 256);
     mbar_init(dp_full, 1);
-    mbar_init(p_ready, W::COMPUTE);
-    mbar_init(ds_ready, W::COMPUTE);
+    mbar_init(p_ready, 256);
+    mbar_init(ds_ready, 256);
     mbar_init(final_bar, 1);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -300,8 +324,8 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 4 * NWG) {
-    if constexpr (NWG == 2) setmaxnreg_dec<bwd::REGS_CONTROL>();
+  if (warp >= 8) {
+    if constexpr (D == 128) setmaxnreg_dec<bwd::REGS_CONTROL>();
     const uint64_t keep = policy_evict_last();
     auto load_q = [&](int it) -> bool {
       const int s = it % QS;
@@ -339,12 +363,12 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         bool ok = true;
         for (int it = 0; it < ns && ok; ++it) {
           if ((ok = load_q(it))) ++n_q;
-          if (NWG == 1 && ok) {
+          if (W::DO_PRODUCER < 0 && ok) {
             if (it == 0) wait_stats();
             if ((ok = load_do(it))) ++n_do;
           }
         }
-        if (NWG == 1 && ns <= 0) wait_stats();
+        if (W::DO_PRODUCER < 0 && ns <= 0) wait_stats();
         if (*abort_flag) {
           if (ns > 0) mbar_wait_drain(kv_full, 0);
           for (int x = max(0, n_q - QS); x < n_q; ++x) mbar_wait_drain(q_full(x % QS), (x / QS) & 1);
@@ -366,7 +390,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       constexpr uint32_t IDESC_G = idesc_bf16(128, D, false, true);      // [128 keys x D]
       const uint64_t kdesc = kmajor_desc(sbase + L::K_OFF, 128, 0), vdesc = kmajor_desc(sbase + L::V_OFF, 128, 0);
       auto issue_s = [&](int i) -> bool {  // S^T = K Q_i^T
-        if (!warp_wait(q_full(i % QS), (i / QS) & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!mbar_wait(q_full(i % QS), (i / QS) & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t qd = kmajor_desc(q_addr(i), STEP, 0);
         if (elect_one()) {
@@ -380,7 +404,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         return true;
       };
       auto issue_dp = [&](int i) -> bool {  // dP^T = V dO_i^T
-        if (!warp_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!mbar_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t dd = kmajor_desc(do_addr(i), STEP, 0);
         if (elect_one()) {
@@ -394,27 +418,27 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         return true;
       };
       auto issue_dv = [&](int i) -> bool {  // dV += P^T dO_i
-        if (!warp_wait(p_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!mbar_wait(p_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t dd = mnmajor_desc(do_addr(i), STEP, 0);
         if (elect_one()) {
           mma_ts(tmem + L::DV_COL, tmem + L::DP_COL, dd, IDESC_G, i > 0 ? 1u : 0u);
 #pragma unroll
           for (int ks = 1; ks < STEP / 16; ++ks)
-            mma_ts_acc(tmem + L::DV_COL, bwd::packed_kstep_col(tmem + L::DP_COL, ks), dd + mnmajor_step(ks), IDESC_G);
+            mma_ts_acc(tmem + L::DV_COL, tmem + L::DP_COL + kstep_col<CW>(ks), dd + mnmajor_step(ks), IDESC_G);
         }
         __syncwarp();
         return true;
       };
       auto issue_dk = [&](int i) -> bool {  // dK += dS^T Q_i
-        if (!warp_wait(ds_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
+        if (!mbar_wait(ds_ready, i & 1, abort_flag, kErrGenDkdvMma)) return false;
         tc_fence_after();
         const uint64_t qd = mnmajor_desc(q_addr(i), STEP, 0);
         if (elect_one()) {
-          mma_ts(tmem + L::DK_COL, tmem + L::DP_COL + 32, qd, IDESC_G, i > 0 ? 1u : 0u);
+          mma_ts(tmem + L::DK_COL, tmem + L::DP_COL + CW / 2, qd, IDESC_G, i > 0 ? 1u : 0u);
 #pragma unroll
           for (int ks = 1; ks < STEP / 16; ++ks)
-            mma_ts_acc(tmem + L::DK_COL, bwd::packed_kstep_col(tmem + L::DP_COL + 32, ks), qd + mnmajor_step(ks), IDESC_G);
+            mma_ts_acc(tmem + L::DK_COL, tmem + L::DP_COL + CW / 2 + kstep_col<CW>(ks), qd + mnmajor_step(ks), IDESC_G);
           mma_commit(q_empty(i % QS));
           mma_commit(do_empty(i % DS));
         }
@@ -423,7 +447,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       };
       bool ok = true;
       if (ns > 0) {
-        ok = warp_wait(kv_full, 0, abort_flag, kErrGenDkdvMma);
+        ok = mbar_wait(kv_full, 0, abort_flag, kErrGenDkdvMma);
         if (ok && n0 + 128 > n_keys && n_keys < pr.Sk) {
           zero_tail(sbase + L::K_OFF, SLABS, n_keys - n0, lane);
           zero_tail(sbase + L::V_OFF, SLABS, n_keys - n0, lane);
@@ -434,7 +458,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       // and dP(i+1): P(i) and dS(i) live in the dP columns.
       for (int i = 0; i < ns && ok; ++i) {
         if (i + 1 < ns) {
-          if (!(ok = warp_wait(s_free, i & 1, abort_flag, kErrGenDkdvMma))) break;
+          if (!(ok = mbar_wait(s_free, i & 1, abort_flag, kErrGenDkdvMma))) break;
           tc_fence_after();
           if (!(ok = issue_s(i + 1))) break;
         }
@@ -451,17 +475,17 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     }
     __syncwarp();
   } else {
-    if constexpr (NWG == 2) setmaxnreg_inc<bwd::REGS_COMPUTE>();
+    if constexpr (D == 128) setmaxnreg_inc<bwd::REGS_COMPUTE>();
     // ---------------------------------------------------------------- compute
-    const int g = warp >> 2;                 // warpgroup: query columns [64g, 64g+64) of a step
+    const int g = warp >> 2;                 // warpgroup: query columns [CW g, CW g + CW) of a step
     const int row = (warp & 3) * 32 + lane;  // key row within the block
     const int kg = n0 + row;
     const int kw = n0 + (warp & 3) * 32;  // the warp's first key
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_off + 64 * g;
-    const uint32_t t_dp = tmem + lane_off + L::DP_COL + 64 * g;
+    const uint32_t t_s = tmem + lane_off + CW * g;
+    const uint32_t t_dp = tmem + lane_off + L::DP_COL + CW * g;
     // first query that sees this key (none: past every query)
-    const int q_first = kg >= n_keys ? INT_MAX : (CAUSAL ? kg - off : INT_MIN);
+    const int q_first = kg >= n_keys ? INT_MAX : (CAUSAL ? kg - off : -1);
     const float2 c2 = make_float2(pr.scale_log2, pr.scale_log2);
     bool ok = true;
     int i = 0;
@@ -471,31 +495,31 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       float bias_l = 0.f, bias_r = 0.f;
       if (BIAS) {
         asm volatile("griddepcontrol.wait;" ::: "memory");  // the tables are written
-        ok = named_barrier_and(2, W::COMPUTE, ok);  // everyone is done with the last head's table
-        copy_table(tab, tables, hk * pr.G + hg, bias, threadIdx.x, W::COMPUTE);
-        ok = named_barrier_and(2, W::COMPUTE, ok);
+        ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table
+        copy_table(tab, tables, hk * pr.G + hg, bias, threadIdx.x, 256);
+        ok = named_barrier_and(2, 256, ok);
         bias_l = tab[0];
         bias_r = tab[table_last(bias)];
       }
       const int head_end = min(ns, (hg + 1) * nqb - st0);
       for (; ok && i < head_end; ++i) {
-        const int qc = q_begin + (st0 + i - hg * nqb) * STEP + 64 * g;  // first query of this thread's columns
-        if (!(ok = warp_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvCompute))) break;
-        const float* lse_s = lse_smem(i) + 64 * g;
+        const int qc = q_begin + (st0 + i - hg * nqb) * STEP + CW * g;  // first query of this thread's columns
+        if (!(ok = mbar_wait(do_full(i % DS), (i / DS) & 1, abort_flag, kErrGenDkdvCompute))) break;
+        const float* lse_s = lse_smem(i) + CW * g;
         const float* dl_s = lse_s + STEP;
-        float p[64];
-        if (!(ok = warp_wait(s_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
+        float p[CW];
+        if (!(ok = mbar_wait(s_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
         tc_fence_after();
-        bwd::tmem_ld64(t_s, p);
+        ld_cols(t_s, p);
         tc_fence_before();
         mbar_arrive(s_free);  // S may now be overwritten by S(i+1)
-        uint32_t pk[32];
+        uint32_t pk[CW / 2];
         {
           const bool masked = kw + 32 > n_keys || (CAUSAL && qc + off < kw + 31);
           bool near = false;
           float fb = 0.f;
           if (BIAS) {
-            const int r_min = kw - (off + qc + 63), r_max = kw + 31 - (off + qc);
+            const int r_min = kw - (off + qc + CW - 1), r_max = kw + 31 - (off + qc);
             near = r_min < bias.right && r_max > -bias.left;
             fb = r_min >= bias.right ? bias_r : bias_l;
           }
@@ -503,12 +527,12 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
             // scores that look their bias up: into the score first, the rest as below
             const float* tp = tab + (kg - off - qc + bias.left + kPad);
 #pragma unroll
-            for (int e = 0; e < 64; ++e) p[e] = fmaf(p[e], pr.scale_log2, tp[-e]);
+            for (int e = 0; e < CW; ++e) p[e] = fmaf(p[e], pr.scale_log2, tp[-e]);
           }
           const float2 cc = (BIAS && near) ? make_float2(1.f, 1.f) : c2;
           const float fc = (BIAS && near) ? 0.f : fb;
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
+          for (int e = 0; e < CW; e += 4) {
             const float4 l4 = *reinterpret_cast<const float4*>(lse_s + e);
             float2 la = make_float2(-l4.x, -l4.y), lb = make_float2(-l4.z, -l4.w);
             if (BIAS) {
@@ -517,7 +541,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
             }
             const float2 xa = fma2(make_float2(p[e], p[e + 1]), cc, la);
             const float2 xb = fma2(make_float2(p[e + 2], p[e + 3]), cc, lb);
-            if (bwd::emu_group<D, true>(e >> 2)) {  // this group of 4 on the FMA pipe
+            if ((e >> 2 & 3) < EMU) {  // this group of 4 on the FMA pipe
               const float2 ea = exp2_fma2(xa), eb = exp2_fma2(xb);
               p[e + 0] = ea.x;
               p[e + 1] = ea.y;
@@ -529,33 +553,36 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
               p[e + 2] = fast_exp2(xb.x);
               p[e + 3] = fast_exp2(xb.y);
             }
-            if (masked) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                if (qc + e + u < q_first) p[e + u] = 0.f;
-            }
-            pk[e / 2] = pack_bf16x2(p[e], p[e + 1]);
-            pk[e / 2 + 1] = pack_bf16x2(p[e + 2], p[e + 3]);
           }
+          if (masked) {  // apart from the loop, so that other steps branch around it
+            const int first = q_first - min(qc, 1 << 30);  // column of the first query that sees the key
+#pragma unroll
+            for (int e = 0; e < CW; ++e)
+              if (e < first) p[e] = 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < CW / 2; ++e) pk[e] = pack_bf16x2(p[2 * e], p[2 * e + 1]);
         }
-        if (!(ok = warp_wait(dp_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
+        if (!(ok = mbar_wait(dp_full, i & 1, abort_flag, kErrGenDkdvCompute))) break;
         tc_fence_after();
-        // dP(i) comes into registers half by half; its columns then take P(i) and dS(i)
-        uint32_t dlo[32], dhi[32];
-        tmem_ld32(t_dp, dlo);
+        // dP(i) comes into registers 32 columns at a time; P(i) and dS(i) then take its columns
+        uint32_t dp[CW / 32][32];
+        tmem_ld32(t_dp, dp[0]);
         tmem_ld_wait();
-        tmem_st32(t_dp, pk);
-        tmem_ld32(t_dp + 32, dhi);
-        tmem_ld_wait();
+        st_cols(t_dp, pk);
+        if constexpr (CW == 64) {
+          tmem_ld32(t_dp + 32, dp[1]);
+          tmem_ld_wait();
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(p_ready);
         {
-          uint32_t dk[32];
+          uint32_t dk[CW / 2];
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
+          for (int e = 0; e < CW; e += 4) {
             const float4 d4 = *reinterpret_cast<const float4*>(dl_s + e);
-            const uint32_t* src = (e < 32) ? dlo : dhi;
+            const uint32_t* src = dp[e / 32];
             const int x = e & 31;
             const float2 da = mul2(make_float2(p[e], p[e + 1]),
                                    sub2(make_float2(__uint_as_float(src[x]), __uint_as_float(src[x + 1])),
@@ -566,7 +593,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
             dk[e / 2] = pack_bf16x2(da.x, da.y);
             dk[e / 2 + 1] = pack_bf16x2(db.x, db.y);
           }
-          tmem_st32(t_dp + 32, dk);
+          st_cols(t_dp + CW / 2, dk);
           tmem_st_wait();
         }
         tc_fence_before();
@@ -574,18 +601,18 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       }
     }
     const bool empty = ns <= 0;
-    const bool done = ok && (empty || warp_wait(final_bar, 0, abort_flag, kErrGenDkdvCompute));
+    const bool done = ok && (empty || mbar_wait(final_bar, 0, abort_flag, kErrGenDkdvCompute));
     tc_fence_after();
     // every MMA has finished: K's and V's room holds the staged dV and dK tiles
     const bool row_ok = done && kg < pr.Sk;
     const long long r = (static_cast<long long>(split) * pr.B * pr.Hkv + b * pr.Hkv + hk) * pr.Sk + kg;
-    give_acc<D, NWG>(tmem + lane_off + L::DV_COL, g, sbase + L::K_OFF, row, n_split > 1 ? dv_part + r * pr.D : nullptr,
+    give_acc<D>(tmem + lane_off + L::DV_COL, g, sbase + L::K_OFF, row, n_split > 1 ? dv_part + r * pr.D : nullptr,
                      pr.D, done, row_ok, empty, 1.f);
-    give_acc<D, NWG>(tmem + lane_off + L::DK_COL, g, sbase + L::V_OFF, row, n_split > 1 ? dk_part + r * pr.D : nullptr,
+    give_acc<D>(tmem + lane_off + L::DK_COL, g, sbase + L::V_OFF, row, n_split > 1 ? dk_part + r * pr.D : nullptr,
                      pr.D, done, row_ok, empty, pr.scale);
     if (n_split == 1) {
       const CUtensorMap* const maps[2] = {&tm_dv, &tm_dk};
-      store_staged<D, NWG, 2>(done, maps, sbase + L::K_OFF, n0, hk, b);
+      store_staged<D, 2>(done, maps, sbase + L::K_OFF, n0, hk, b);
     }
   }
 
@@ -600,9 +627,9 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
 // ====================================================================================
 // dQ and dbias
 // ====================================================================================
-template <int D, int NWG, bool BIAS>
+template <int D, bool BIAS>
 struct DqLayout {
-  static constexpr int STEP = 64 * NWG;
+  static constexpr int STEP = BwdShape<D>::STEP;
   static constexpr int TILE = STEP * D * 2;
   static constexpr int K_STAGES = (BIAS && D == 128) ? 3 : 4;  // the bias part takes one slot's room
   static constexpr int V_STAGES = 3;
@@ -619,12 +646,12 @@ struct DqLayout {
   // bias: diagonal scratch of each warp, table (fp32 by position), buckets by position,
   // per-warp sums
   static constexpr int DIAG_OFF = DELTA_OFF + 512;
-  static constexpr int TAB_OFF = DIAG_OFF + (BIAS ? 4 * NWG * 96 * 4 : 0);
+  static constexpr int TAB_OFF = DIAG_OFF + (BIAS ? 8 * 96 * 4 : 0);
   static int smem_bytes(const Bias& bias) {
-    return TAB_OFF + (BIAS ? table_size(bias) * 4 + lut_size(bias) * 2 + 4 * NWG * bias.buckets * 4 : 0) + 1024;
+    return TAB_OFF + (BIAS ? table_size(bias) * 4 + lut_size(bias) * 2 + 8 * bias.buckets * 4 : 0) + 1024;
   }
   // at most, with kMaxDistance and kMaxBuckets
-  static constexpr int MOST = TAB_OFF + (BIAS ? kTableMax * 4 + (2 * kMaxDistance + 8) * 2 + 4 * NWG * kMaxBuckets * 4 : 0) + 1024;
+  static constexpr int MOST = TAB_OFF + (BIAS ? kTableMax * 4 + (2 * kMaxDistance + 8) * 2 + 8 * kMaxBuckets * 4 : 0) + 1024;
 };
 
 // Copy this thread's row of `true_d` bf16 values into D/2 packed TMEM columns (the rest
@@ -678,31 +705,32 @@ __device__ __forceinline__ float row_dot_to_tmem(const __nv_bfloat16* __restrict
   return acc;
 }
 
-// Add the diagonal sums of a warp's 32 x 64 block of dS (lane = row, ds[e] = column e) to
+// Add the diagonal sums of a warp's 32 x CW block of dS (lane = row, ds[e] = column e) to
 // the warp's sums by bucket.  `r0`: relative position of lane 0, column 0; `lut`: bucket of
 // position r at r + left; `diag`: 96 floats of scratch of this warp.
-__device__ __forceinline__ void add_near_block(const float (&ds)[64], int r0, const Bias& bias,
+template <int CW>
+__device__ __forceinline__ void add_near_block(const float (&ds)[CW], int r0, const Bias& bias,
                                                const unsigned short* lut, float* sums, float* diag, int lane) {
   // before column e, lane l holds the sum of diagonal e - l over the lanes below it; after
   // it lane 31's diagonal e - 31 is complete, and comes round to lane 0
   float a = 0.f;
 #pragma unroll
-  for (int e = 0; e < 64; ++e) {
+  for (int e = 0; e < CW; ++e) {
     if (e > 0) {
       a = __shfl_sync(0xffffffffu, a, (lane + 31) & 31);
       if (lane == 0) {
-        diag[e - 1] = a;  // diagonal e - 32, kept at e - 32 + 31
+        diag[e - 1] = a;  // diagonal e - 32, kept 31 places on
         a = 0.f;
       }
     }
     a += ds[e];
   }
-  diag[94 - lane] = a;  // diagonal 63 - l
+  diag[CW + 30 - lane] = a;  // diagonal CW - 1 - l
   __syncwarp();
-#pragma unroll
-  for (int c = 0; c < 3; ++c) {
-    const int x = c * 32 + lane;  // 95 diagonals; the last lane of the last chunk has none
-    float v = x < 95 ? diag[x] : 0.f;
+#pragma unroll 1
+  for (int c = 0; c < CW + 32; c += 32) {
+    const int x = c + lane;  // CW + 31 diagonals; the last lane of the last chunk has none
+    float v = x < CW + 31 ? diag[x] : 0.f;
     const int r = min(max(r0 + x - 31, -bias.left), bias.right);
     const int u = lut[r + bias.left];
     // positions of one bucket are neighbours: sums of runs of equal buckets
@@ -719,8 +747,8 @@ __device__ __forceinline__ void add_near_block(const float (&ds)[64], int r0, co
   }
 }
 
-template <int D, int NWG, bool CAUSAL, bool BIAS>
-__global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
+template <int D, bool CAUSAL, bool BIAS, int EMU = bwd_emu(BIAS)>
+__global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     ffa_gen_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ Problem pr,
                       const __grid_constant__ Bias bias, const float* __restrict__ tables,
@@ -728,9 +756,9 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
                       const float* __restrict__ LSE, float* __restrict__ lse_out, float* __restrict__ delta_out,
                       float* __restrict__ dq_part, float* __restrict__ bias_part,
                       int n_split, int group) {
-  using L = DqLayout<D, NWG, BIAS>;
-  using W = BwdWidth<NWG>;
-  constexpr int SLABS = D / 64, STEP = L::STEP;
+  using L = DqLayout<D, BIAS>;
+  using W = BwdShape<D>;
+  constexpr int SLABS = D / 64, STEP = W::STEP, CW = W::CW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -773,7 +801,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
   const int nk = min(per_split, all - t0);
 
   if (threadIdx.x == 0) {
-    mbar_init(qd_ready, W::COMPUTE);
+    mbar_init(qd_ready, 256);
     for (int s = 0; s < KS; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(k_empty(s), 1);
@@ -783,9 +811,9 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       mbar_init(v_empty(s), 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, W::COMPUTE);
+    mbar_init(s_free, 256);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, W::COMPUTE);
+    mbar_init(ds_ready, 256);
     mbar_init(final_bar, 1);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -800,15 +828,15 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     tma_prefetch_desc(&tm_v);
   }
   asm volatile("griddepcontrol.launch_dependents;");
-  if (BIAS && warp < 4 * NWG)
-    for (int t = threadIdx.x; t < 4 * NWG * bias.buckets; t += W::COMPUTE) sums_all[t] = 0.f;
+  if (BIAS && warp < 8)
+    for (int t = threadIdx.x; t < 8 * bias.buckets; t += 256) sums_all[t] = 0.f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 4 * NWG) {
-    if constexpr (NWG == 2) setmaxnreg_dec<bwd::REGS_CONTROL>();
+  if (warp >= 8) {
+    if constexpr (D == 128) setmaxnreg_dec<bwd::REGS_CONTROL>();
     if (warp == W::PRODUCER) {
       // -------------------------------------------------------------- producer: K, V rings
       if (lane == 0) {
@@ -846,7 +874,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         if (tail < STEP && n_keys < pr.Sk) zero_tail<STEP>(tile, SLABS, tail, lane);
       };
       auto issue_s = [&](int j) -> bool {  // S_j = Q K_j^T  (Q from TMEM)
-        if (!warp_wait(k_full(j % KS), (j / KS) & 1, abort_flag, kErrGenDqMma)) return false;
+        if (!mbar_wait(k_full(j % KS), (j / KS) & 1, abort_flag, kErrGenDqMma)) return false;
         fix_tail(k_addr(j), j);
         tc_fence_after();
         const uint64_t kd = kmajor_desc(k_addr(j), STEP, 0);
@@ -861,7 +889,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         return true;
       };
       auto issue_dp = [&](int j) -> bool {  // dP_j = dO V_j^T  (dO from TMEM)
-        if (!warp_wait(v_full(j % VS), (j / VS) & 1, abort_flag, kErrGenDqMma)) return false;
+        if (!mbar_wait(v_full(j % VS), (j / VS) & 1, abort_flag, kErrGenDqMma)) return false;
         fix_tail(v_addr(j), j);
         tc_fence_after();
         const uint64_t vd = kmajor_desc(v_addr(j), STEP, 0);
@@ -877,27 +905,27 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         return true;
       };
       auto issue_g = [&](int j) -> bool {  // dQ += dS_j K_j  (dS_j packed in the dP columns)
-        if (!warp_wait(ds_ready, j & 1, abort_flag, kErrGenDqMma)) return false;
+        if (!mbar_wait(ds_ready, j & 1, abort_flag, kErrGenDqMma)) return false;
         tc_fence_after();
         const uint64_t kd = mnmajor_desc(k_addr(j), 128, 0);
         if (elect_one()) {
           mma_ts(tmem + L::DQ, tmem + L::DP, kd, IDESC_G, j > 0 ? 1u : 0u);
 #pragma unroll
           for (int ks = 1; ks < STEP / 16; ++ks)
-            mma_ts_acc(tmem + L::DQ, bwd::packed_kstep_col(tmem + L::DP, ks), kd + mnmajor_step(ks), IDESC_G);
+            mma_ts_acc(tmem + L::DQ, tmem + L::DP + kstep_col<CW>(ks), kd + mnmajor_step(ks), IDESC_G);
           mma_commit(k_empty(j % KS));
         }
         __syncwarp();
         return true;
       };
-      bool ok = warp_wait(qd_ready, 0, abort_flag, kErrGenDqMma);
+      bool ok = mbar_wait(qd_ready, 0, abort_flag, kErrGenDqMma);
       tc_fence_after();
       if (ok && nk > 0) ok = issue_s(0) && issue_dp(0);
       // S(j+1) once the warpgroups hold S(j) in registers; dQ(j) once dS(j) is in the dP
       // columns; then dP(j+1) over them
       for (int j = 0; j < nk && ok; ++j) {
         if (j + 1 < nk) {
-          if (!(ok = warp_wait(s_free, j & 1, abort_flag, kErrGenDqMma))) break;
+          if (!(ok = mbar_wait(s_free, j & 1, abort_flag, kErrGenDqMma))) break;
           tc_fence_after();
           if (!(ok = issue_s(j + 1))) break;
         }
@@ -913,29 +941,32 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     }
     __syncwarp();
   } else {
-    if constexpr (NWG == 2) setmaxnreg_inc<bwd::REGS_COMPUTE>();
+    if constexpr (D == 128) setmaxnreg_inc<bwd::REGS_COMPUTE>();
     // ---------------------------------------------------------------- compute
     const int g = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // query row within the block
     const int qg = m0 + row;
     const int qw = m0 + (warp & 3) * 32;  // the warp's first query
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    // Q and dO rows into tensor memory (two warpgroups: one each), and delta = O . dO on the way
+    // warpgroup 0 puts the Q rows into tensor memory, warpgroup 1 the dO rows, and takes
+    // delta = O . dO on the way
     const bool row_in = qg < pr.Sq;
     auto row_of = [&](const View& x) {
       return static_cast<const __nv_bfloat16*>(x.p) + b * x.sb + h * x.sh + static_cast<long long>(row_in ? qg : 0) * x.ss;
     };
     float dl = 0.f;
-    if (NWG == 1 || g == 0) row_to_tmem<D>(row_of(q), row_in, pr.D, tmem + lane_off + L::Q);
-    if (NWG == 1 || g == 1) dl = row_dot_to_tmem<D>(row_of(dout), row_of(o), row_in, pr.D, tmem + lane_off + L::DO);
+    if (g == 0)
+      row_to_tmem<D>(row_of(q), row_in, pr.D, tmem + lane_off + L::Q);
+    else
+      dl = row_dot_to_tmem<D>(row_of(dout), row_of(o), row_in, pr.D, tmem + lane_off + L::DO);
     tmem_st_wait();
     tc_fence_before();
     mbar_arrive(qd_ready);
     // +inf for a row that saw no key and for rows behind the last one: their P is 0
     float lse = row_in ? LSE[static_cast<long long>(bh) * pr.Sq + qg] : INFINITY;
     if (lse == -INFINITY) lse = INFINITY;
-    if (NWG == 1 || g == 1) {
-      if (NWG == 2) delta_s[row] = dl;
+    if (g == 1) {
+      delta_s[row] = dl;
       if (split == 0) {
         const long long r = static_cast<long long>(bh) * padded_rows(pr.Sq) + qg;
         lse_out[r] = lse;
@@ -944,15 +975,15 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     }
     if (BIAS) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the tables are written
-      copy_table(tab, tables, h, bias, threadIdx.x, W::COMPUTE);
-      for (int t = threadIdx.x; t < lut_size(bias) / 2; t += W::COMPUTE)
+      copy_table(tab, tables, h, bias, threadIdx.x, 256);
+      for (int t = threadIdx.x; t < lut_size(bias) / 2; t += 256)
         reinterpret_cast<uint32_t*>(lut)[t] = reinterpret_cast<const uint32_t*>(lut_g)[t];
     }
-    if (BIAS || NWG == 2) named_barrier_and(2, W::COMPUTE, true);
-    if (NWG == 2) dl = delta_s[row];
+    named_barrier_and(2, 256, true);
+    dl = delta_s[row];
     const int lim = CAUSAL ? min(n_keys - 1, qg + off) : n_keys - 1;  // last visible key
-    const uint32_t t_s = tmem + lane_off + 64 * g;
-    const uint32_t t_dp = tmem + lane_off + L::DP + 64 * g;
+    const uint32_t t_s = tmem + lane_off + CW * g;
+    const uint32_t t_dp = tmem + lane_off + L::DP + CW * g;
     float* sums = sums_all + warp * bias.buckets;
     float* diag = reinterpret_cast<float*>(smem + L::DIAG_OFF) + warp * 96;
     float bias_l = 0.f, bias_r = 0.f, sum_l = 0.f, sum_r = 0.f;
@@ -962,35 +993,35 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
     }
     bool ok = true;
     for (int j = 0; j < nk; ++j) {
-      if (!(ok = warp_wait(s_full, j & 1, abort_flag, kErrGenDqCompute))) break;
+      if (!(ok = mbar_wait(s_full, j & 1, abort_flag, kErrGenDqCompute))) break;
       tc_fence_after();
-      float p[64];
-      bwd::tmem_ld64(t_s, p);
+      float p[CW];
+      ld_cols(t_s, p);
       tc_fence_before();
       mbar_arrive(s_free);  // S may now be overwritten by S(j+1)
-      const int kc = (t0 + j) * STEP + 64 * g;  // first key of this thread's columns
-      const bool masked = kc + 64 > n_keys || (CAUSAL && kc + 63 > qw + off);
+      const int kc = (t0 + j) * STEP + CW * g;  // first key of this thread's columns
+      const bool masked = kc + CW > n_keys || (CAUSAL && kc + CW - 1 > qw + off);
       bool near = false, right = false;
       float fb = 0.f;
       if (BIAS) {
-        const int r_min = kc - (off + qw + 31), r_max = kc + 63 - (off + qw);
+        const int r_min = kc - (off + qw + 31), r_max = kc + CW - 1 - (off + qw);
         near = r_min < bias.right && r_max > -bias.left;
         right = r_min >= bias.right;
         fb = right ? bias_r : bias_l;
         if (near) {
           const float* tp = tab + (kc - off - qg + bias.left + kPad);
 #pragma unroll
-          for (int e = 0; e < 64; ++e) p[e] = fmaf(p[e], pr.scale_log2, tp[e]);
+          for (int e = 0; e < CW; ++e) p[e] = fmaf(p[e], pr.scale_log2, tp[e]);
         }
       }
       const bool looked = BIAS && near;
       const float c1 = looked ? 1.f : pr.scale_log2, l1 = looked ? -lse : fb - lse;
       const float2 c2 = make_float2(c1, c1), l2 = make_float2(l1, l1);
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
+      for (int e = 0; e < CW; e += 2) {
         const float2 x = fma2(make_float2(p[e], p[e + 1]), c2, l2);
         float p0, p1;
-        if (bwd::emu_group<D, false>(e >> 2)) {  // this pair on the FMA pipe
+        if ((e >> 2 & 3) < EMU) {  // this pair on the FMA pipe
           const float2 ex = exp2_fma2(x);
           p0 = ex.x;
           p1 = ex.y;
@@ -998,27 +1029,24 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
           p0 = fast_exp2(x.x);
           p1 = fast_exp2(x.y);
         }
-        if (masked) {
-          if (kc + e > lim) p0 = 0.f;
-          if (kc + e + 1 > lim) p1 = 0.f;
-        }
         p[e] = p0;
         p[e + 1] = p1;
       }
-      if (!(ok = warp_wait(dp_full, j & 1, abort_flag, kErrGenDqCompute))) break;
+      if (masked) {  // apart from the loop, so that other steps branch around it
+        const int last = lim - kc;
+#pragma unroll
+        for (int e = 0; e < CW; ++e)
+          if (e > last) p[e] = 0.f;
+      }
+      if (!(ok = mbar_wait(dp_full, j & 1, abort_flag, kErrGenDqCompute))) break;
       tc_fence_after();
-      uint32_t dlo[32], dhi[32];
-      tmem_ld32(t_dp, dlo);
-      tmem_ld32(t_dp + 32, dhi);
-      tmem_ld_wait();
-      uint32_t dsp[32];
+      float dp[CW];
+      ld_cols(t_dp, dp);
+      uint32_t dsp[CW / 2];
       const float2 d2 = make_float2(dl, dl);
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        const uint32_t* src = (e < 32) ? dlo : dhi;
-        const int x = e & 31;
-        const float2 ds = mul2(make_float2(p[e], p[e + 1]),
-                               sub2(make_float2(__uint_as_float(src[x]), __uint_as_float(src[x + 1])), d2));
+      for (int e = 0; e < CW; e += 2) {
+        const float2 ds = mul2(make_float2(p[e], p[e + 1]), sub2(make_float2(dp[e], dp[e + 1]), d2));
         dsp[e >> 1] = pack_bf16x2(ds.x, ds.y);
         if (BIAS) {
           p[e] = ds.x;
@@ -1026,18 +1054,18 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         }
       }
       // dS(j) over the first half of this warpgroup's dP columns: the A operand of dQ(j)
-      tmem_st32(t_dp, dsp);
+      st_cols(t_dp, dsp);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(ds_ready);
       if (BIAS) {
         // this step's share of dbias, while the tensor core is at dQ(j)
         if (near) {
-          add_near_block(p, kc - (off + qw), bias, lut, sums, diag, lane);
+          add_near_block<CW>(p, kc - (off + qw), bias, lut, sums, diag, lane);
         } else {
           float2 a = make_float2(0.f, 0.f), c = a;
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
+          for (int e = 0; e < CW; e += 4) {
             a = add2(a, make_float2(p[e], p[e + 1]));
             c = add2(c, make_float2(p[e + 2], p[e + 3]));
           }
@@ -1050,7 +1078,7 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
       }
     }
     const bool empty = nk <= 0;
-    const bool done = ok && (empty || warp_wait(final_bar, 0, abort_flag, kErrGenDqCompute));
+    const bool done = ok && (empty || mbar_wait(final_bar, 0, abort_flag, kErrGenDqCompute));
     tc_fence_after();
     if (BIAS) {
 #pragma unroll
@@ -1062,23 +1090,23 @@ __global__ void __launch_bounds__(BwdWidth<NWG>::THREADS, BwdWidth<NWG>::CTAS)
         sums[lut[0]] += sum_l;
         sums[lut[bias.left + bias.right]] += sum_r;
       }
-      if (named_barrier_and(2, W::COMPUTE, done)) {
+      if (named_barrier_and(2, 256, done)) {
         float* dst = bias_part + (static_cast<long long>(bh) * nblk * n_split + cw.rank) * bias.buckets;
-        for (int u = threadIdx.x; u < bias.buckets; u += W::COMPUTE) {
+        for (int u = threadIdx.x; u < bias.buckets; u += 256) {
           float a = 0.f;
 #pragma unroll
-          for (int w = 0; w < 4 * NWG; ++w) a += sums_all[w * bias.buckets + u];
+          for (int w = 0; w < 8; ++w) a += sums_all[w * bias.buckets + u];
           dst[u] = a;
         }
       }
     }
     // every MMA has finished: the K ring is free and holds the staged dQ tile
     const long long r = (static_cast<long long>(split) * pr.B * pr.Hq + bh) * pr.Sq + qg;
-    give_acc<D, NWG>(tmem + lane_off + L::DQ, g, sbase + L::K_OFF, row, n_split > 1 ? dq_part + r * pr.D : nullptr, pr.D,
+    give_acc<D>(tmem + lane_off + L::DQ, g, sbase + L::K_OFF, row, n_split > 1 ? dq_part + r * pr.D : nullptr, pr.D,
                      done, done && row_in, empty, pr.scale);
     if (n_split == 1) {
       const CUtensorMap* const maps[1] = {&tm_dq};
-      store_staged<D, NWG, 1>(done, maps, sbase + L::K_OFF, m0, h, b);
+      store_staged<D, 1>(done, maps, sbase + L::K_OFF, m0, h, b);
     }
   }
 

@@ -152,12 +152,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-// mbar_wait of a whole warp: true in all lanes or in none, so that the warp stays together
-// for the collective instructions that follow.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int site) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site));
-}
-
 // Zero the rows from `row` on of a tile of ROWS rows in shared memory (64-column slabs, 128
 // bytes a row; the swizzle moves nothing between rows).  The whole warp calls it,
 // before it issues MMAs that read the tile.  A probability of 0 does not undo a NaN in the

@@ -11,10 +11,10 @@
 //     for its own loads and MMAs most of the time.  So a CTA has one tile and walks 64 keys
 //     a step: 128 columns of tensor memory and 80 registers a thread, four CTAs to an SM;
 //   * head dims up to 128: two tiles and 128 keys a step, one CTA to an SM;
-//   * the loop bodies are 64 scores long and used for every kind of tile.  Tiles that need a
-//     mask, a bias for each score or a negative scale are put right in tensor memory first
-//     (a rolled loop): a short launch spends much of its time fetching instructions that it
-//     runs for the first time;
+//   * the loop bodies are 64 scores long and the same for every kind of tile; a mask, a bias
+//     for each score or a negative scale is applied in tensor memory first (a rolled loop).
+//     A short launch spends much of its time fetching instructions that it runs for the first
+//     time (B8 H12 S1024 D64: 91 us with bodies of 128 scores for each kind, 58 so);
 //   * a tile whose relative positions all lie in the last bucket of a side has one bias: it
 //     joins the row max and the exponent's constant for free;
 //   * with few CTAs the keys are split in units of `per_split` steps (the same for all
@@ -182,14 +182,14 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
       // ---------------------------------------------------------------- MMA issuer
       constexpr uint32_t IDESC_QK = idesc_bf16(128, KEYS, false, false);
       constexpr uint32_t IDESC_PV = idesc_bf16(128, D, false, true);
-      bool ok = n_kv > 0 && warp_wait(q_full, 0, abort_flag, kErrGenFwdMma);
+      bool ok = n_kv > 0 && mbar_wait(q_full, 0, abort_flag, kErrGenFwdMma);
       auto commit = [&](uint32_t bar) {
         if (elect_one()) mma_commit(bar);
         __syncwarp();
       };
       auto kv_addr = [&](int n) { return sbase + L::KV_OFF + (n % STAGES) * L::TILE; };
       auto kv_wait = [&](int n) {
-        const bool r = warp_wait(kv_full(n), (n / STAGES) & 1, abort_flag, kErrGenFwdMma);
+        const bool r = mbar_wait(kv_full(n), (n / STAGES) & 1, abort_flag, kErrGenFwdMma);
         tc_fence_after();
         return r;
       };
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
         const uint32_t d = tmem + L::O_COL + i * 128, a = tmem + i * KEYS;
 #pragma unroll 1
         for (int half = 0; half < L::HALVES; ++half) {
-          if (!warp_wait(p_ready(i, half), j & 1, abort_flag, kErrGenFwdMma)) return false;
+          if (!mbar_wait(p_ready(i, half), j & 1, abort_flag, kErrGenFwdMma)) return false;
           tc_fence_after();
           if (elect_one()) {
             const uint64_t vh = vd + mnmajor_step(4 * half);
@@ -270,11 +270,11 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
     const int lim = CAUSAL ? min(n_keys - 1, grow + off) : n_keys - 1;
     const float scale_log2 = pr.scale_log2;
     bool ok = true;
-    if (BIAS && cnt > 0) ok = warp_wait(tab_full, 0, abort_flag, kErrGenFwdSoftmax);
+    if (BIAS && cnt > 0) ok = mbar_wait(tab_full, 0, abort_flag, kErrGenFwdSoftmax);
     float m_used = -INFINITY;
     float l = 0.f;
     for (int j = 0; ok && j < cnt; ++j) {
-      if (!(ok = warp_wait(s_full(i), j & 1, abort_flag, kErrGenFwdSoftmax))) break;
+      if (!(ok = mbar_wait(s_full(i), j & 1, abort_flag, kErrGenFwdSoftmax))) break;
       tc_fence_after();
       const int n0 = (t0 + j) * KEYS;
       const bool masked = (n0 + KEYS > n_keys) || (CAUSAL && n0 + KEYS - 1 > wrow + off);
@@ -286,26 +286,33 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
         near = r_min < bias.right && r_max > -bias.left;
         fb = tab[r_min >= bias.right ? table_last(bias) : 0];
       }
-      float c = scale_log2;  // what the scores still have to be multiplied with
-      if (masked || near || scale_log2 < 0.f) {
-        const float* tp = tab + (n0 - off - grow + bias.left + kPad);
+      // With a bias for each score or a scale that does not keep the order, the scores in
+      // tensor memory become scaled scores; masked ones become -inf.
+      const bool scaled = near || scale_log2 <= 0.f;
+      const float c = scaled ? 1.f : scale_log2;  // what the scores still have to be multiplied with
+      if (scaled || masked) {
 #pragma unroll 1
         for (int x = 0; x < KEYS; x += 32) {
           uint32_t r[32];
           tmem_ld32(t_s + x, r);
           tmem_ld_wait();
+          if (scaled) {
+            const float* tp = tab + (n0 + x - off - grow + bias.left + kPad);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float y = __uint_as_float(r[e]) * scale_log2;
-            if (BIAS) y += near ? tp[x + e] : fb;
-            r[e] = __float_as_uint(n0 + x + e > lim ? -INFINITY : y);
+            for (int e = 0; e < 32; ++e)
+              r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), scale_log2, BIAS && near ? tp[e] : fb));
+          }
+          if (masked) {
+            const int last = lim - n0 - x;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e > last) r[e] = 0xff800000u;
           }
           tmem_st32(t_s + x, r);
         }
         tmem_st_wait();
-        c = 1.f;
-        fb = 0.f;
       }
+      if (scaled) fb = 0.f;
       uint32_t sa[32], sb[32];  // 64 scores
       float tmax = -INFINITY;
 #pragma unroll 1
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
     // without keys (no max) is 0: the sum holds what the polynomial makes of 2^-inf, and
     // tensor memory may hold anything.  Its Q tile, where the output is staged, may still be
     // on its way when the other tile has keys.
-    const bool done = ok && (n_kv == 0 || warp_wait(cnt > 0 ? o_final(i) : q_full, 0, abort_flag, kErrGenFwdSoftmax));
+    const bool done = ok && (n_kv == 0 || mbar_wait(cnt > 0 ? o_final(i) : q_full, 0, abort_flag, kErrGenFwdSoftmax));
     tc_fence_after();
     const bool valid = done && grow < pr.Sq, none = m_used == -INFINITY;
     const float inv_l = none ? 0.f : 1.f / l;

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
   for (int n = 0;; ++n) {
     // a wait that ran out ends all warps here, at the next segment
     Segment sg{};
-    ok = ok && warp_wait(seg_full(n), (n / L::SEGS) & 1, abort_flag, kErrGenStepCompute);
+    ok = ok && mbar_wait(seg_full(n), (n / L::SEGS) & 1, abort_flag, kErrGenStepCompute);
     if (ok) sg = *seg_slot(n);
     __syncwarp();
     if (lane == 0) mbar_arrive(seg_empty(n));
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     }
     const int w0 = (warp & 3) * L::WKEYS;  // the warp's first key of a tile
     for (int j = 0; j < sg.nt; ++j, ++it) {
-      if (!(ok = warp_wait(full(it), (it / STAGES) & 1, abort_flag, kErrGenStepCompute))) break;
+      if (!(ok = mbar_wait(full(it), (it / STAGES) & 1, abort_flag, kErrGenStepCompute))) break;
       const uint32_t kt = sbase + (it % STAGES) * 2 * L::TILE, vt = kt + L::TILE;
       const int key0 = (sg.t0 + j) * L::KEYS + w0;
       if (key0 < n_keys) {
