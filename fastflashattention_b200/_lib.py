@@ -34,10 +34,10 @@ SIGNATURES = {
     "ffa_bwd_dkdv_acc": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _LL, _LL, _D, _I, _VP]),
     "ffa_bwd_dq_acc": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _LL, _LL, _D, _I, _VP]),
     "ffa_lse_merge": (_I, [_VP, _VP, _VP, _VP, _LL, _I, _I, _VP]),
-    "ffa_gen_fwd_workspace": (_LL, [_VP]),
+    "ffa_gen_fwd_workspace": (_LL, [_VP, _I]),
     "ffa_gen_bwd_workspace": (_LL, [_VP]),
-    "ffa_gen_fwd": (_I, [_VP] * 7 + [_LL, _VP]),
-    "ffa_gen_bwd": (_I, [_VP] * 12 + [_LL, _VP]),
+    "ffa_gen_fwd": (_I, [_VP] * 8 + [_LL, _VP]),
+    "ffa_gen_bwd": (_I, [_VP] * 13 + [_LL, _VP]),
     "ffa_last_error": (_I, [ctypes.c_char_p, _I]),
     "ffa_device_status": (_I, [ctypes.POINTER(ctypes.c_uint)]),
     "ffa_version": (ctypes.c_char_p, []),

@@ -117,12 +117,15 @@ inline int split_of(long long ctas, long long slots, long long units, long long 
   return static_cast<int>(n < most ? n : (most > 1 ? most : 1));
 }
 
-// The forward: steps of a split when `ctas` CTAs, `slots` at a time, each walk `units` steps of
-// `step_us` microseconds.  The estimate of a split's size is its waves times (its steps +
-// `fixed`, a CTA's start and end in steps); where lengths differ, the mean load plus one last
-// split.  Joining costs `join` steps, and for each split the traffic of `rows` fp32 rows of O.
-// The smallest estimate wins.
-inline long long split_steps(long long ctas, long long slots, long long units, bool ragged, long long rows, int D,
+// The forward: steps of a split when `ctas` CTAs, `slots` at a time, each walk up to `units`
+// steps, `mean` on average, of `step_us` microseconds.  The estimate of a split's size, in
+// steps: where all CTAs are alike, waves times (a split's steps + `fixed`, a CTA's start and
+// end); else (a causal mask, lengths that differ; the longest come first) one longest split
+// where a single wave holds them all, or the mean load and a part of a split at the end.
+// Joining costs `join`, and for each split the traffic of `rows` fp32 rows of O.  The
+// smallest estimate wins.  (B200, B2 H32 over 8 heads, 500 tokens on 8192 keys, D128: 142 us
+// in one split, 132 in two, 124 in three, 146 in four.)
+inline long long split_steps(long long ctas, long long slots, long long units, double mean, long long rows, int D,
                              double step_us, double fixed, double join) {
   const double traffic = static_cast<double>(rows) * D * 8 / 6.5e6 / step_us;
   long long best = units > 0 ? units : 1;
@@ -130,10 +133,17 @@ inline long long split_steps(long long ctas, long long slots, long long units, b
   for (long long n = 1; n <= 64 && n <= (units + 1) / 2; ++n) {
     const long long per = ceil_div(units, n);
     if (ceil_div(units, per) != n) continue;
-    const double load = static_cast<double>(ctas) * n / slots;
-    const double cost =
-        (ragged && load > 1 ? 0.6 * load * (per + fixed) + 0.4 * (per + fixed) : std::ceil(load) * (per + fixed)) +
-        (n > 1 ? join + n * traffic : 0.0);
+    const double load = static_cast<double>(ctas) / slots;
+    double cost;
+    if (mean > 0.99 * units) {
+      cost = std::ceil(load * n) * (per + fixed);
+    } else {
+      const double splits = std::max(1.0, mean / per + (n > 1 ? 0.5 : 0.0));  // of a CTA's steps, on average
+      cost = load * splits <= 1.0 ? per + fixed
+                                  : std::max(per + fixed, load * (mean + splits * fixed)) +
+                                        (n > 1 ? 0.5 : 0.15) * (per + fixed);
+    }
+    if (n > 1) cost += join + n * traffic;
     if (cost < least) {
       least = cost;
       best = per;
@@ -154,13 +164,12 @@ struct FwdPlan {
   bool join;
 };
 
-inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias) {
+inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias, bool exact) {
   FwdPlan f{};
   const long long heads = static_cast<long long>(p->batch) * p->q_heads;
   const long long group_rows = p->kv_heads ? static_cast<long long>(p->q_heads / p->kv_heads) * p->q_len : 0;
-  const bool ragged = p->batch > 1 && (p->key_lengths || (p->causal && p->query_offsets));
   const bool small_d = p->head_dim <= 64;
-  f.step = group_rows <= 64;
+  f.step = group_rows <= 64 && !exact;  // the step kernel has no form with remainders
   if (heads * p->q_len == 0) return f;
   if (f.step) {
     f.rg = group_rows <= 16 ? 1 : 2;
@@ -183,10 +192,19 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias) {
   }
   const int rows = small_d ? 128 : 256, keys = small_d ? 64 : 128;
   const long long units = std::max<long long>(1, ceil_div(p->k_len, keys));
+  // steps of a block of queries on average: lengths that differ are taken as two thirds of
+  // the longest; under a causal mask the blocks see more and more keys
+  double mean = static_cast<double>(units);
+  if (p->batch > 1 && p->key_lengths) mean *= 0.67;
+  if (p->causal) {
+    const double off = p->query_offsets ? std::max(0, p->k_len - p->q_len) : p->query_offset;
+    const double seen = std::min<double>(p->k_len, std::max(0.0, off + 0.5 * p->q_len)) / std::max(1, p->k_len);
+    mean = std::max(1.0, mean * seen);
+  }
   // a step of one CTA: four of them share an SM at head dims up to 64
-  f.per_split = static_cast<int>(split_steps(heads * ceil_div(p->q_len, rows), kSMs * (small_d ? 4 : 1), units, ragged,
-                                             heads * p->q_len, p->head_dim, small_d ? 1.0 : 2.2, small_d ? 4.0 : 2.0,
-                                             small_d ? 5.0 : 2.5));
+  f.per_split = static_cast<int>(split_steps(heads * ceil_div(p->q_len, rows), kSMs * (small_d ? 4 : 1), units, mean,
+                                             heads * p->q_len, p->head_dim, small_d ? 1.0 : 2.2, small_d ? 5.0 : 2.7,
+                                             small_d ? 11.0 : 4.5));
   f.n_split = static_cast<int>(ceil_div(units, f.per_split));
   f.keys_per_split = f.per_split * keys;
   f.join = f.n_split > 1;
@@ -250,7 +268,7 @@ inline int check_regs_once(const void* kernel, int needed, bool* done) {
 struct Call {
   Problem pr;
   Bias bias;
-  View q, k, v, o, dout, dq, dk, dv;
+  View q, k, v, o, o_lo, dout, dq, dk, dv;
   float* lse;
   cudaStream_t stream;
 };
@@ -279,20 +297,22 @@ static int launch_tables(const Call& c, float* tables, unsigned short* lut) {
   return launched();
 }
 
-template <int D, bool CAUSAL, bool BIAS>
+template <int D, bool CAUSAL, bool BIAS, bool EXACT>
 static int launch_gen_fwd(const Call& c, const FwdPlan& f, float* ws) {
   using L = FwdLayout<D>;
   const Problem& pr = c.pr;
-  CUtensorMap tq, tk, tv, to;
+  CUtensorMap tq, tk, tv, to, tlo;
   int rc;
   if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
   if ((rc = make_map(&to, c.o, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
+  tlo = to;
+  if (EXACT && (rc = make_map(&tlo, c.o_lo, pr.B, pr.Hq, pr.Sq, pr.D))) return rc;
   tk = tv = tq;  // without keys nothing is loaded through them
   if (pr.Sk > 0) {
     if ((rc = make_map(&tk, c.k, pr.B, pr.Hkv, pr.Sk, pr.D, L::KEYS))) return rc;
     if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D, L::KEYS))) return rc;
   }
-  auto kern = ffa_gen_fwd_kernel<D, CAUSAL, BIAS>;
+  auto kern = ffa_gen_fwd_kernel<D, CAUSAL, BIAS, EXACT>;
   static unsigned long long configured = 0;
   constexpr int most = L::TAB_OFF + (BIAS ? kTableMax * 4 : 0) + 1024;
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
@@ -307,9 +327,9 @@ static int launch_gen_fwd(const Call& c, const FwdPlan& f, float* ws) {
   const float* tables = ws;
   float *part = ws ? ws + f.part_off : nullptr, *part_lse = ws ? ws + f.lse_off : nullptr;
   if (BIAS)
-    return launch_early(kern, grid, L::THREADS, smem, c.stream, tq, tk, tv, to, pr, c.bias, tables, c.lse, part,
+    return launch_early(kern, grid, L::THREADS, smem, c.stream, tq, tk, tv, to, tlo, pr, c.bias, tables, c.lse, part,
                         part_lse, f.n_split, f.per_split, group);
-  kern<<<grid, L::THREADS, smem, c.stream>>>(tq, tk, tv, to, pr, c.bias, tables, c.lse, part, part_lse, f.n_split,
+  kern<<<grid, L::THREADS, smem, c.stream>>>(tq, tk, tv, to, tlo, pr, c.bias, tables, c.lse, part, part_lse, f.n_split,
                                              f.per_split, group);
   return launched();
 }
@@ -415,9 +435,9 @@ static int launch_gen_dq(const Call& c, const BwdPlan& w, float* ws) {
   const unsigned short* lut = reinterpret_cast<const unsigned short*>(ws + w.lut_off);
   const float* lse = c.lse;
   if (BIAS)
-    return launch_early(kern, grid, W::THREADS, smem, c.stream, tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.dout,
+    return launch_early(kern, grid, W::THREADS, smem, c.stream, tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.o_lo, c.dout,
                         lse, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split, group);
-  kern<<<grid, W::THREADS, smem, c.stream>>>(tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.dout, lse, ws,
+  kern<<<grid, W::THREADS, smem, c.stream>>>(tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.o_lo, c.dout, lse, ws,
                                              ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split, group);
   return launched();
 }
@@ -436,7 +456,11 @@ static int dispatch(const Call& c, bool causal, A&&... a) {
 }
 template <int D, bool C, bool B>
 struct RunFwd {
-  static int run(const Call& c, const FwdPlan& f, float* ws) { return launch_gen_fwd<D, C, B>(c, f, ws); }
+  static int run(const Call& c, const FwdPlan& f, float* ws) {
+    if constexpr (B)
+      if (c.o_lo.p) return launch_gen_fwd<D, C, B, true>(c, f, ws);
+    return launch_gen_fwd<D, C, B, false>(c, f, ws);
+  }
 };
 template <int D, bool C, bool B>
 struct RunStep {
@@ -456,9 +480,9 @@ struct RunDq {
 
 extern "C" {
 
-long long ffa_gen_fwd_workspace(const ffa_gen_problem* p) {
+long long ffa_gen_fwd_workspace(const ffa_gen_problem* p, int with_o_lo) {
   if (ffa::gen::check_problem(p)) return -1;
-  return ffa::gen::fwd_plan(p, ffa::gen::device_bias(p)).bytes;
+  return ffa::gen::fwd_plan(p, ffa::gen::device_bias(p), with_o_lo != 0).bytes;
 }
 
 long long ffa_gen_bwd_workspace(const ffa_gen_problem* p) {
@@ -467,7 +491,8 @@ long long ffa_gen_bwd_workspace(const ffa_gen_problem* p) {
 }
 
 int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
-                const ffa_gen_tensor* o, float* lse, void* workspace, long long workspace_bytes, void* stream) {
+                const ffa_gen_tensor* o, const ffa_gen_tensor* o_lo, float* lse, void* workspace,
+                long long workspace_bytes, void* stream) {
   using namespace ffa::gen;
   int rc = check_problem(p);
   if (rc) return rc;
@@ -477,7 +502,9 @@ int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
       (rc = check_tensor(v, keys)))
     return rc;
   const Bias bias = device_bias(p);
-  const FwdPlan f = fwd_plan(p, bias);
+  if (o_lo && !p->bias) return ffa::set_error(FFA_ERR_INVALID, "o_lo comes with a bias");
+  if (o_lo && (rc = check_tensor(o_lo, true))) return rc;
+  const FwdPlan f = fwd_plan(p, bias, o_lo != nullptr);
   if (f.bytes > 0 && (!workspace || workspace_bytes < f.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return ffa::set_error(FFA_ERR_INVALID, "workspace missing, too small or not 16-byte aligned");
   if ((rc = ffa::ensure_context()) != FFA_OK) return rc;
@@ -488,6 +515,7 @@ int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   c.k = view(k);
   c.v = view(v);
   c.o = view(o);
+  if (o_lo) c.o_lo = view(o_lo);
   c.lse = lse;
   c.stream = static_cast<cudaStream_t>(stream);
   float* ws = f.bytes > 0 ? static_cast<float*>(workspace) : nullptr;
@@ -495,13 +523,16 @@ int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   rc = dispatch<RunFwd>(c, p->causal, f, ws);
   if (rc || !f.join) return rc;
   const long long rows = static_cast<long long>(p->batch) * p->q_heads * p->q_len;
-  return launch_early(ffa_gen_join_kernel, dim3(static_cast<unsigned>(ceil_div(rows, 4))), 128, 0, c.stream, c.pr,
-                      ws + f.part_off, ws + f.lse_off, c.o, lse, f.keys_per_split, p->causal ? 1 : 0);
+  auto join = [&](auto kern, int lanes) {
+    return launch_early(kern, dim3(static_cast<unsigned>(ceil_div(rows * lanes, 256))), 256, 0, c.stream, c.pr,
+                        ws + f.part_off, ws + f.lse_off, c.o, c.o_lo, lse, f.keys_per_split, p->causal ? 1 : 0);
+  };
+  return p->head_dim <= 64 ? join(ffa_gen_join_kernel<16>, 16) : join(ffa_gen_join_kernel<32>, 32);
 }
 
 int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
-                const ffa_gen_tensor* o, const ffa_gen_tensor* dout, const float* lse, const ffa_gen_tensor* dq,
-                const ffa_gen_tensor* dk, const ffa_gen_tensor* dv, void* dbias, void* workspace,
+                const ffa_gen_tensor* o, const ffa_gen_tensor* o_lo, const ffa_gen_tensor* dout, const float* lse,
+                const ffa_gen_tensor* dq, const ffa_gen_tensor* dk, const ffa_gen_tensor* dv, void* dbias, void* workspace,
                 long long workspace_bytes, void* stream) {
   using namespace ffa::gen;
   int rc = check_problem(p);
@@ -514,6 +545,7 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   if ((rc = check_tensor(q, queries)) || (rc = check_tensor(o, queries)) || (rc = check_tensor(dout, queries)) ||
       (rc = check_tensor(k, keys)) || (rc = check_tensor(v, keys)))
     return rc;
+  if (o_lo && (rc = check_tensor(o_lo, queries))) return rc;
   if (queries && !lse) return ffa::set_error(FFA_ERR_INVALID, "null tensor pointer");
   if (want_dq && (rc = check_tensor(dq, queries))) return rc;
   if (want_dkdv && ((rc = check_tensor(dk, keys)) || (rc = check_tensor(dv, keys)))) return rc;
@@ -529,6 +561,7 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   c.k = view(k);
   c.v = view(v);
   c.o = view(o);
+  if (o_lo) c.o_lo = view(o_lo);
   c.dout = view(dout);
   c.lse = const_cast<float*>(lse);
   c.stream = static_cast<cudaStream_t>(stream);

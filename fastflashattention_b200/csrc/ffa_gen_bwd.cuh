@@ -119,12 +119,12 @@ __device__ __forceinline__ void copy_table(float* tab, const float* tables, int 
 }
 
 // Give this lane's share of an accumulator (half of the columns for warpgroup g), times
-// `mul`, to the staged bf16 tile (128 rows, for a TMA store) or, with `part`, to an fp32 row
-// of `true_d` values.  `empty`: nothing was accumulated, and tensor memory may hold
+// `mul`, to the staged bf16 tile (128 rows, for a TMA store) or, with `part`, to the warp's
+// fp32 rows of `true_d` values, of which `rows` exist.  `empty`: nothing was accumulated, and tensor memory may hold
 // anything: zeros.  The whole warp calls it.
 template <int D>
 __device__ __forceinline__ void give_acc(uint32_t t_acc, int g, uint32_t tile, int row, float* part, int true_d,
-                                         bool done, bool row_ok, bool empty, float mul) {
+                                         bool done, int rows, bool empty, float mul) {
   if (!done) return;
 #pragma unroll 1
   for (int c = g * (D / 2); c < (g + 1) * (D / 2); c += 32) {
@@ -138,8 +138,8 @@ __device__ __forceinline__ void give_acc(uint32_t t_acc, int g, uint32_t tile, i
     }
     if (part == nullptr)
       stage_row32_sw128(tile, row, c, r, mul);
-    else if (row_ok)
-      write_row32(part, c, true_d, r, mul);
+    else  // the tile's room is this function's scratch: 4 KB for each of eight warps
+      write_rows32(tile + (threadIdx.x >> 5) * 4096, part, c, true_d, rows, r, mul, threadIdx.x & 31);
   }
 }
 
@@ -604,12 +604,11 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     const bool done = ok && (empty || mbar_wait(final_bar, 0, abort_flag, kErrGenDkdvCompute));
     tc_fence_after();
     // every MMA has finished: K's and V's room holds the staged dV and dK tiles
-    const bool row_ok = done && kg < pr.Sk;
-    const long long r = (static_cast<long long>(split) * pr.B * pr.Hkv + b * pr.Hkv + hk) * pr.Sk + kg;
+    const long long r = (static_cast<long long>(split) * pr.B * pr.Hkv + b * pr.Hkv + hk) * pr.Sk + kw;
     give_acc<D>(tmem + lane_off + L::DV_COL, g, sbase + L::K_OFF, row, n_split > 1 ? dv_part + r * pr.D : nullptr,
-                     pr.D, done, row_ok, empty, 1.f);
-    give_acc<D>(tmem + lane_off + L::DK_COL, g, sbase + L::V_OFF, row, n_split > 1 ? dk_part + r * pr.D : nullptr,
-                     pr.D, done, row_ok, empty, pr.scale);
+                     pr.D, done, pr.Sk - kw, empty, 1.f);
+    give_acc<D>(tmem + lane_off + L::DK_COL, g, n_split > 1 ? sbase + L::K_OFF : sbase + L::V_OFF, row, n_split > 1 ? dk_part + r * pr.D : nullptr,
+                     pr.D, done, pr.Sk - kw, empty, pr.scale);
     if (n_split == 1) {
       const CUtensorMap* const maps[2] = {&tm_dv, &tm_dk};
       store_staged<D, 2>(done, maps, sbase + L::K_OFF, n0, hk, b);
@@ -675,12 +674,19 @@ __device__ __forceinline__ void row_to_tmem(const __nv_bfloat16* __restrict__ sr
   }
 }
 
-// The same, and the row's dot product with `other`.
+// The same, and the row's dot product with `other` and, where given, its remainder `rem`.
 template <int D>
 __device__ __forceinline__ float row_dot_to_tmem(const __nv_bfloat16* __restrict__ src,
-                                                 const __nv_bfloat16* __restrict__ other, bool valid, int true_d,
+                                                 const __nv_bfloat16* __restrict__ other,
+                                                 const __nv_bfloat16* __restrict__ rem, bool valid, int true_d,
                                                  uint32_t taddr) {
   float acc = 0.f;
+  auto add = [&](uint32_t x, uint32_t y) {
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y));
+    acc = fmaf(a.x, b.x, acc);
+    acc = fmaf(a.y, b.y, acc);
+  };
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
     uint32_t w[32];
@@ -690,14 +696,24 @@ __device__ __forceinline__ float row_dot_to_tmem(const __nv_bfloat16* __restrict
       const bool in = valid && 64 * c + 8 * e < true_d;
       const uint4 x = in ? __ldg(s4 + e) : make_uint4(0u, 0u, 0u, 0u);
       const uint4 y = in ? __ldg(o4 + e) : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      w[4 * e + 0] = x.x;
+      w[4 * e + 1] = x.y;
+      w[4 * e + 2] = x.z;
+      w[4 * e + 3] = x.w;
+      add(x.x, y.x);
+      add(x.y, y.y);
+      add(x.z, y.z);
+      add(x.w, y.w);
+    }
+    if (rem != nullptr) {  // apart, so that its loads go out together as well
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        w[4 * e + u] = xs[u];
-        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&xs[u]));
-        const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ys[u]));
-        acc = fmaf(a.x, b.x, acc);
-        acc = fmaf(a.y, b.y, acc);
+      for (int e = 0; e < 8; ++e) {
+        const bool in = valid && 64 * c + 8 * e < true_d;
+        const uint4 z = in ? __ldg(reinterpret_cast<const uint4*>(rem + 64 * c) + e) : make_uint4(0u, 0u, 0u, 0u);
+        add(w[4 * e + 0], z.x);
+        add(w[4 * e + 1], z.y);
+        add(w[4 * e + 2], z.z);
+        add(w[4 * e + 3], z.w);
       }
     }
     tmem_st32(taddr + 32 * c, w);
@@ -752,7 +768,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     ffa_gen_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ Problem pr,
                       const __grid_constant__ Bias bias, const float* __restrict__ tables,
-                      const unsigned short* __restrict__ lut_g, const View q, const View o, const View dout,
+                      const unsigned short* __restrict__ lut_g, const View q, const View o, const View o_lo, const View dout,
                       const float* __restrict__ LSE, float* __restrict__ lse_out, float* __restrict__ delta_out,
                       float* __restrict__ dq_part, float* __restrict__ bias_part,
                       int n_split, int group) {
@@ -958,7 +974,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     if (g == 0)
       row_to_tmem<D>(row_of(q), row_in, pr.D, tmem + lane_off + L::Q);
     else
-      dl = row_dot_to_tmem<D>(row_of(dout), row_of(o), row_in, pr.D, tmem + lane_off + L::DO);
+      dl = row_dot_to_tmem<D>(row_of(dout), row_of(o), o_lo.p ? row_of(o_lo) : nullptr, row_in, pr.D, tmem + lane_off + L::DO);
     tmem_st_wait();
     tc_fence_before();
     mbar_arrive(qd_ready);
@@ -1101,9 +1117,9 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
       }
     }
     // every MMA has finished: the K ring is free and holds the staged dQ tile
-    const long long r = (static_cast<long long>(split) * pr.B * pr.Hq + bh) * pr.Sq + qg;
+    const long long r = (static_cast<long long>(split) * pr.B * pr.Hq + bh) * pr.Sq + qw;
     give_acc<D>(tmem + lane_off + L::DQ, g, sbase + L::K_OFF, row, n_split > 1 ? dq_part + r * pr.D : nullptr, pr.D,
-                     done, done && row_in, empty, pr.scale);
+                     done, pr.Sq - qw, empty, pr.scale);
     if (n_split == 1) {
       const CUtensorMap* const maps[1] = {&tm_dq};
       store_staged<D, 1>(done, maps, sbase + L::K_OFF, m0, h, b);

@@ -39,7 +39,7 @@ struct Problem {
   __device__ __forceinline__ int seq_at(int pos) const {
     if (key_lengths == nullptr || B == 1) return pos;
     const int lane = threadIdx.x & 31, first = pos & ~31;
-    const int n = first + lane < B ? min(key_lengths[first + lane], Sk) : -1;
+    const int n = first + lane < B ? min(max(key_lengths[first + lane], 0), Sk) : -1;  // -1: behind them all
     int rank = 0;  // sequences of the 32 that come before this lane's
 #pragma unroll 8
     for (int x = 0; x < 32; ++x) {
@@ -164,15 +164,32 @@ __device__ __forceinline__ void zero_tail(uint32_t tile, int slabs, int row, int
   __syncwarp();
 }
 
-// Write 32 fp32 accumulator columns, times `mul`, to columns [c0, c0 + 32) of an fp32 row of
-// D values (D a multiple of 8).
-__device__ __forceinline__ void write_row32(float* dst, int c0, int D, const uint32_t (&r)[32], float mul) {
+// Write a warp's 32 rows x 32 fp32 accumulator columns (lane = row), times `mul`, to columns
+// [c0, c0 + 32) of the fp32 rows dst, dst + D, ... of which `rows` exist.  D is a multiple
+// of 8.  The values change places in `scratch` (4 KB of shared memory of this warp), so that
+// eight lanes write 128 bytes of a row: lanes that wrote a row each would leave 32 pieces of
+// 16 bytes for every store.
+__device__ __forceinline__ void write_rows32(uint32_t scratch, float* dst, int c0, int D, int rows,
+                                             const uint32_t (&r)[32], float mul, int lane) {
+  __syncwarp();  // the last call's values have been read
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    if (c0 + 4 * e < D)
-      *reinterpret_cast<float4*>(dst + c0 + 4 * e) =
-          make_float4(__uint_as_float(r[4 * e]) * mul, __uint_as_float(r[4 * e + 1]) * mul,
-                      __uint_as_float(r[4 * e + 2]) * mul, __uint_as_float(r[4 * e + 3]) * mul);
+    st_shared_v4(scratch + lane * 128 + ((e ^ (lane & 7)) << 4), __float_as_uint(__uint_as_float(r[4 * e]) * mul),
+                 __float_as_uint(__uint_as_float(r[4 * e + 1]) * mul),
+                 __float_as_uint(__uint_as_float(r[4 * e + 2]) * mul),
+                 __float_as_uint(__uint_as_float(r[4 * e + 3]) * mul));
+  __syncwarp();
+  const int col = c0 + 4 * (lane & 7);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int row = 4 * e + (lane >> 3);
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(scratch + row * 128 + (((lane & 7) ^ (row & 7)) << 4))
+                 : "memory");
+    if (row < rows && col < D) *reinterpret_cast<float4*>(dst + static_cast<long long>(row) * D + col) = v;
+  }
 }
 
 // 4-D tensor map over a [B, H, S, D] bf16 tensor: boxes of 64 columns x `rows` rows, 128-byte

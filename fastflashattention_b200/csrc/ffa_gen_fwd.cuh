@@ -17,6 +17,12 @@
 //     time (B8 H12 S1024 D64: 91 us with bodies of 128 scores for each kind, 58 so);
 //   * a tile whose relative positions all lie in the last bucket of a side has one bias: it
 //     joins the row max and the exponent's constant for free;
+//   * EXACT, for a training step that wants the bias's gradient: P goes to the product as two
+//     bf16 values (rounded and remainder, twice the MMAs), and O is written with its own
+//     remainder (o_lo), which gives the backward delta = O . dO to 16 bits.  The bias's
+//     gradient adds dS over whole rows, whose sum is 0: an error of delta, common to a row,
+//     adds up where dS cancels (with O in 8 bits: up to 0.7 % of the gradient's norm at 16
+//     buckets, S = 1485; with the remainder 0.2 %, its rounding to bf16);
 //   * with few CTAs the keys are split in units of `per_split` steps (the same for all
 //     sequences, so that units of sequences of different lengths take the same time); each
 //     split writes its normalised O in fp32 and its LSE, and ffa_gen_join_kernel weighs them.
@@ -63,11 +69,11 @@ __device__ __forceinline__ float row_max64(const uint32_t (&a)[32], const uint32
   return fmax3(fmax3(y0, y1, y2), fmax3(y3, y4, x[15]), y0);
 }
 
-template <int D, bool CAUSAL, bool BIAS, int EMU = D == 64 ? 2 : 0>
+template <int D, bool CAUSAL, bool BIAS, bool EXACT, int EMU = D == 64 ? 2 : 0>
 __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
     ffa_gen_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
-                       const __grid_constant__ Problem pr, const __grid_constant__ Bias bias,
+                       const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ Problem pr, const __grid_constant__ Bias bias,
                        const float* __restrict__ tables, float* __restrict__ LSE, float* __restrict__ part,
                        float* __restrict__ part_lse, int n_split, int per_split, int group) {
   using L = FwdLayout<D>;
@@ -215,9 +221,10 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
           tc_fence_after();
           if (elect_one()) {
             const uint64_t vh = vd + mnmajor_step(4 * half);
-            mma_ts(d, a + 32 * half, vh, IDESC_PV, (j > 0 || half > 0) ? 1u : 0u);
+            mma_ts(d, a + 64 * half, vh, IDESC_PV, (j > 0 || half > 0) ? 1u : 0u);
 #pragma unroll
-            for (int ks = 1; ks < 4; ++ks) mma_ts_acc(d, a + 32 * half + ks * 8, vh + mnmajor_step(ks), IDESC_PV);
+            for (int ks = 1; ks < (EXACT ? 8 : 4); ++ks)  // 4 to 7: the remainders of P, behind it
+              mma_ts_acc(d, a + 64 * half + ks * 8, vh + mnmajor_step(ks & 3), IDESC_PV);
           }
           __syncwarp();
         }
@@ -346,7 +353,8 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
       const float m_safe = (m_used == -INFINITY) ? 0.f : m_used;
       const float shift = BIAS ? fb - m_safe : -m_safe;
       const float2 c2 = make_float2(c, c), nm2 = make_float2(shift, shift);
-      // 64 scores -> P -> 32 columns over S (the first half's scores are still in registers)
+      // 64 scores -> P -> 32 columns over these scores, and 32 of remainders behind them (the
+      // first half's scores are still in registers)
 #pragma unroll 1
       for (int hf = 0; hf < L::HALVES; ++hf) {
         if (hf > 0) {
@@ -355,6 +363,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
           tmem_ld_wait();
         }
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t hi[32], lo[EXACT ? 32 : 1];
 #pragma unroll
         for (int u = 0; u < 32; ++u) {
           const uint32_t* src = u < 16 ? sa : sb;
@@ -370,11 +379,14 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
             p1 = fast_exp2(x.y);
           }
           sum2[u & 1] = add2(sum2[u & 1], make_float2(p0, p1));
-          sa[u] = pack_bf16x2(p0, p1);  // pair u replaces a score that is already used
+          hi[u] = pack_bf16x2(p0, p1);
+          if (EXACT)
+            lo[u] = pack_bf16x2(p0 - __uint_as_float(hi[u] << 16), p1 - __uint_as_float(hi[u] & 0xffff0000u));
         }
         const float2 sv = add2(sum2[0], sum2[1]);
         l += sv.x + sv.y;
-        tmem_st32(t_s + 32 * hf, sa);
+        tmem_st32(t_s + 64 * hf, hi);
+        if constexpr (EXACT) tmem_st32(t_s + 64 * hf + 32, lo);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(p_ready(i, hf));
@@ -398,33 +410,46 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
       else if (LSE != nullptr)
         LSE[ridx] = lse;
     }
-    if (done) {
+    // O, then (EXACT) its remainder, over the Q tile, which is free once every MMA has finished
 #pragma unroll 1
-      for (int x = 0; x < D; x += 32) {
-        uint32_t r[32];
-        if (cnt > 0) {
-          tmem_ld32(t_o + x, r);
-          tmem_ld_wait();
-        }
-        if (none) {
+    for (int rem = 0; rem < (EXACT && n_split == 1 ? 2 : 1); ++rem) {
+      if (done) {
+#pragma unroll 1
+        for (int x = 0; x < D; x += 32) {
+          uint32_t r[32];
+          if (cnt > 0) {
+            tmem_ld32(t_o + x, r);
+            tmem_ld_wait();
+          }
+          if (none) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = 0u;
+            for (int e = 0; e < 32; ++e) r[e] = 0u;
+          }
+          if (EXACT && rem) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float y = __uint_as_float(r[e]) * inv_l;
+              r[e] = __float_as_uint(y - __bfloat162float(__float2bfloat16_rn(y)));
+            }
+          }
+          if (n_split == 1)
+            stage_row32_sw128(o_tile, row, x, r, rem ? 1.f : inv_l);
+          else
+            write_rows32(o_tile + (warp & 3) * 4096, part + (prow - lane) * pr.D, x, pr.D, pr.Sq - wrow, r, inv_l,
+                         lane);
         }
-        if (n_split == 1)
-          stage_row32_sw128(o_tile, row, x, r, inv_l);
-        else if (valid && !none)
-          write_row32(part + prow * pr.D, x, pr.D, r, inv_l);
       }
-    }
-    if (n_split == 1) {
-      // the Q tile is free once every MMA has finished; the store leaves out rows from Sq on
-      fence_proxy_async_smem();
-      const bool store = named_barrier_and(1 + i, 128, done);
-      if (row == 0 && store && mi < pr.Sq) {
+      if (n_split == 1) {  // the store leaves out rows from Sq on
+        fence_proxy_async_smem();
+        const bool store = named_barrier_and(1 + i, 128, done);
+        if (row == 0 && store && mi < pr.Sq) {
 #pragma unroll
-        for (int sl = 0; sl < SLABS; ++sl) tma_store_4d(&tm_o, o_tile + sl * 16384, sl * 64, mi, h, b);
-        bulk_commit_group();
-        bulk_wait_read();
+          for (int sl = 0; sl < SLABS; ++sl)
+            tma_store_4d(rem ? &tm_lo : &tm_o, o_tile + sl * 16384, sl * 64, mi, h, b);
+          bulk_commit_group();
+          bulk_wait_read();
+        }
+        if (EXACT) named_barrier_and(1 + i, 128, true);  // the tile has been read
       }
     }
   }
@@ -437,50 +462,47 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::CTAS)
   }
 }
 
-// Join the splits of a row: O = sum_s w_s O_s / sum_s w_s, w_s = 2^(LSE_s - max LSE).  One
-// warp a row, four columns a lane.  A sequence has as many splits as its keys fill; a split
-// whose keys the row does not see (LSE = -inf) is not read.
-__global__ void __launch_bounds__(128)
+// Join the splits of a row: O = sum_s w_s O_s / sum_s w_s, w_s = 2^(LSE_s - max LSE).  LANES
+// threads a row (D <= 4 LANES), four columns each.  A sequence has as many splits as its
+// keys fill; a split whose keys the row does not see (LSE = -inf) weighs nothing.
+template <int LANES>
+__global__ void __launch_bounds__(256)
     ffa_gen_join_kernel(const __grid_constant__ Problem pr, const float* __restrict__ part,
-                        const float* __restrict__ part_lse, const View o, float* __restrict__ LSE, int keys_per_split,
-                        int causal) {
-  const int lane = threadIdx.x & 31;
+                        const float* __restrict__ part_lse, const View o, const View o_lo, float* __restrict__ LSE,
+                        int keys_per_split, int causal) {
   const long long rows = static_cast<long long>(pr.B) * pr.Hq * pr.Sq;
-  const long long r = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (r >= rows) return;
+  const long long r = static_cast<long long>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  const int c = threadIdx.x % LANES * 4;
+  if (r >= rows || c >= pr.D) return;
   const int bh = static_cast<int>(r / pr.Sq), t = static_cast<int>(r % pr.Sq);
   const int b = bh / pr.Hq, h = bh % pr.Hq;
   const int n_keys = pr.keys(b, causal ? pr.offset(b) : 0, causal);
   const int n = max(1, (n_keys + keys_per_split - 1) / keys_per_split);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits have written
-  float m = -INFINITY;
-  for (int s = lane; s < n; s += 32) m = fmaxf(m, part_lse[s * rows + r]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  float total = 0.f;
+  // one pass with a running max: the loads of four splits do not wait for one another
+  float m = -INFINITY, total = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int c = lane * 4;
-  if (m > -INFINITY) {
 #pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float lse = part_lse[s * rows + r];
-      const float w = exp2f(lse - m);
-      total += w;
-      if (c < pr.D && lse > -INFINITY) {
-        const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + r) * pr.D + c);
-        a.x = fmaf(w, x.x, a.x);
-        a.y = fmaf(w, x.y, a.y);
-        a.z = fmaf(w, x.z, a.z);
-        a.w = fmaf(w, x.w, a.w);
-      }
-    }
+  for (int s = 0; s < n; ++s) {
+    const float lse = part_lse[s * rows + r];
+    const float4 x = *reinterpret_cast<const float4*>(part + (s * rows + r) * pr.D + c);
+    const float m_new = fmaxf(m, lse), m_safe = m_new == -INFINITY ? 0.f : m_new;
+    const float f = exp2f(m - m_safe), w = exp2f(lse - m_safe);
+    m = m_new;
+    total = fmaf(total, f, w);
+    a.x = fmaf(a.x, f, w * x.x);
+    a.y = fmaf(a.y, f, w * x.y);
+    a.z = fmaf(a.z, f, w * x.z);
+    a.w = fmaf(a.w, f, w * x.w);
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  if (c < pr.D) {
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + c;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
-  }
-  if (lane == 0 && LSE != nullptr) LSE[r] = total == 0.f ? -INFINITY : m + __log2f(total);
+  const uint2 hi = make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + c) = hi;
+  if (o_lo.p != nullptr)
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(o_lo.p) + b * o_lo.sb + h * o_lo.sh + t * o_lo.ss + c) =
+        make_uint2(pack_bf16x2(a.x * inv - __uint_as_float(hi.x << 16), a.y * inv - __uint_as_float(hi.x & 0xffff0000u)),
+                   pack_bf16x2(a.z * inv - __uint_as_float(hi.y << 16), a.w * inv - __uint_as_float(hi.y & 0xffff0000u)));
+  if (c == 0 && LSE != nullptr) LSE[r] = total == 0.f ? -INFINITY : m + __log2f(total);
 }
 
 }  // namespace gen

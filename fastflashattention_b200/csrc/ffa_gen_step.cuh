@@ -54,9 +54,10 @@ struct Segment {
   int tiles;      // tiles of the whole item; 0: there is no segment, the CTA is done
   __device__ __forceinline__ bool whole() const { return t0 == 0 && nt == tiles; }
 };
-// What the join needs of an item that a CTA starts and others finish (parts = 0: none).
+// What the join needs of a CTA: the item that it starts and others finish (parts = 0: none),
+// and whether it has a part in slot 0 (with fewer tiles than CTAs some have none).
 struct JoinEntry {
-  int b, item, parts, pad;
+  int b, item, parts, slot0;
 };
 
 // One thread walks through the CTA's segments (start() is for its whole warp).
@@ -140,7 +141,9 @@ struct Work {
       int last = static_cast<int>(((last_tile + 1) * gridDim.x - 1) / total);
       while (last + 1 < static_cast<int>(gridDim.x) && total * (last + 1) / gridDim.x <= last_tile) ++last;
       while (total * last / gridDim.x > last_tile) --last;
-      entry = {s.b, s.item, last - static_cast<int>(blockIdx.x) + 1, 0};
+      entry.b = s.b;
+      entry.item = s.item;
+      entry.parts = last - static_cast<int>(blockIdx.x) + 1;
     }
   }
 };
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     work.start(pr, per_seq, L::KEYS, single != 0);
     if (lane == 0) {
       const uint64_t once = policy_evict_first();
-      JoinEntry shared{0, 0, 0, 0};
+      JoinEntry shared{0, 0, 0, work.left > 0 && work.t > 0};
       bool ok = true;
       int it = 0;
       for (int n = 0; ok; ++n) {
@@ -498,7 +501,8 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
 
 // Join the parts of the items that cross CTAs: O = sum_p w_p O_p / sum_p w_p with
 // w_p = 2^(LSE_p - max LSE).  blockIdx.x: the CTA in which an item starts; a warp takes one
-// row, four columns a lane.  A part whose keys the row does not see (LSE = -inf) is not read.
+// row, four columns a lane.  A part whose keys the row does not see (LSE = -inf) is not read,
+// nor is the slot of a CTA that has none.
 __global__ void __launch_bounds__(128)
     ffa_gen_step_join_kernel(const __grid_constant__ Problem pr, const float* __restrict__ part,
                              const float* __restrict__ part_lse, const JoinEntry* __restrict__ entries, const View o,
@@ -513,8 +517,9 @@ __global__ void __launch_bounds__(128)
   const int h = e.item / row_tiles * pr.G + r / pr.Sq, t = r % pr.Sq;
   // row of part p: slot 1 of the first CTA, slot 0 of the next ones
   auto at = [&](int p) { return (2LL * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * rows + row; };
+  auto lse_of = [&](int p) { return p == 0 || entries[blockIdx.x + p].slot0 ? part_lse[at(p)] : -INFINITY; };
   float m = -INFINITY;
-  for (int p = lane; p < e.parts; p += 32) m = fmaxf(m, part_lse[at(p)]);
+  for (int p = lane; p < e.parts; p += 32) m = fmaxf(m, lse_of(p));
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
   float total = 0.f;
@@ -523,7 +528,7 @@ __global__ void __launch_bounds__(128)
   if (m > -INFINITY) {
 #pragma unroll 8
     for (int p = 0; p < e.parts; ++p) {
-      const float lse = part_lse[at(p)];
+      const float lse = lse_of(p);
       const float w = exp2f(lse - m);
       total += w;
       if (c < pr.D && lse > -INFINITY) {

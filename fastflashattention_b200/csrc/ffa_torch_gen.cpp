@@ -2,9 +2,9 @@
 // include/ffa.h), beside ffa_torch.cpp and in its manner:
 //
 //   ffa_b200::general(q, k, v, <mask>)            -> o          (no LSE, no grad)
-//   ffa_b200::general_lse(q, k, v, <mask>)        -> (o, lse)
-//   ffa_b200::general_backward(q, k, v, o, do, lse, <mask>, want_dq, want_dkdv, want_dbias)
-//                                                 -> (dq, dk, dv, dbias)
+//   ffa_b200::general_lse(q, k, v, <mask>, with_lo) -> (o, o_lo, lse)
+//   ffa_b200::general_backward(q, k, v, o, o_lo, do, lse, <mask>, want_dq, want_dkdv,
+//                              want_dbias)        -> (dq, dk, dv, dbias)
 //   ffa_b200::general_attention(q, k, v, <mask>)  -> o, differentiable (C++ autograd node)
 //
 // <mask> is (bias, key_lengths, query_offsets, query_offset, borders, both, causal, scale).
@@ -129,38 +129,45 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
-std::tuple<Tensor, Tensor> forward_impl(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Mask& m,
-                                        bool with_lse) {
+// -> o, its remainder (for the bias's gradient, see ffa_gen_fwd), lse
+std::tuple<Tensor, Tensor, Tensor> forward_impl(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Mask& m,
+                                                bool with_lse, bool with_lo) {
   Args a;
   fill(a, q0, k0, v0, m);
   const c10::cuda::CUDAGuard guard(q0.device());
   const Tensor q = prep(q0), k = prep(k0), v = prep(v0);
-  Tensor o = output_like(q), lse;
+  Tensor o = output_like(q), o_lo, lse;
+  if (with_lo) o_lo = at::empty_like(o);
   if (with_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-  const long long bytes = ffa_gen_fwd_workspace(&a.p);
+  const long long bytes = ffa_gen_fwd_workspace(&a.p, with_lo ? 1 : 0);
   const Tensor ws = workspace(bytes, "ffa_gen_fwd_workspace", q);
   const ffa_gen_tensor tq = tensor(q), tk = tensor(k), tv = tensor(v), to = tensor(o);
-  check(ffa_gen_fwd(&a.p, &tq, &tk, &tv, &to, with_lse ? lse.data_ptr<float>() : nullptr, data(ws), bytes,
+  const ffa_gen_tensor tlo = with_lo ? tensor(o_lo) : ffa_gen_tensor{};
+  check(ffa_gen_fwd(&a.p, &tq, &tk, &tv, &to, with_lo ? &tlo : nullptr, with_lse ? lse.data_ptr<float>() : nullptr, data(ws), bytes,
                     stream_of(q)),
         "ffa_gen_fwd");
-  return {o, lse};
+  return {o, o_lo, lse};
 }
 
 // want: dq, dk and dv, dbias
 std::tuple<Tensor, Tensor, Tensor, Tensor> backward_impl(const Tensor& q0, const Tensor& k0, const Tensor& v0,
-                                                         const Tensor& o0, const Tensor& do0, const Tensor& lse0,
-                                                         const Mask& m, bool want_dq, bool want_dkdv,
+                                                         const Tensor& o0, const Tensor& lo0, const Tensor& do0,
+                                                         const Tensor& lse0, const Mask& m, bool want_dq, bool want_dkdv,
                                                          bool want_dbias) {
   Args a;
   fill(a, q0, k0, v0, m);
   TORCH_CHECK(o0.sizes() == q0.sizes() && do0.sizes() == q0.sizes() && o0.scalar_type() == at::kBFloat16 &&
                   do0.scalar_type() == at::kBFloat16 && o0.device() == q0.device() && do0.device() == q0.device(),
               "o and do must be bf16 tensors like q");
+  TORCH_CHECK(!lo0.defined() || (lo0.sizes() == q0.sizes() && lo0.scalar_type() == at::kBFloat16 &&
+                                 lo0.device() == q0.device()),
+              "o_lo must be a bf16 tensor like q");
   TORCH_CHECK(lse0.scalar_type() == at::kFloat && lse0.numel() == q0.size(0) * q0.size(1) * q0.size(2) &&
                   lse0.device() == q0.device(),
               "lse must be the fp32 [B, H, S] of the forward");
   const c10::cuda::CUDAGuard guard(q0.device());
   const Tensor q = prep(q0), k = prep(k0), v = prep(v0), o = prep(o0), dout = prep(do0), lse = lse0.contiguous();
+  const Tensor o_lo = lo0.defined() ? prep(lo0) : Tensor();
   Tensor dq, dk, dv, dbias;
   if (want_dq || want_dbias) dq = output_like(q);  // the kernel of dbias computes dq too
   if (want_dkdv) {
@@ -172,8 +179,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> backward_impl(const Tensor& q0, const
   const Tensor ws = workspace(bytes, "ffa_gen_bwd_workspace", q);
   auto maybe = [](const Tensor& t) { return t.defined() ? tensor(t) : ffa_gen_tensor{}; };
   const ffa_gen_tensor tq = tensor(q), tk = tensor(k), tv = tensor(v), to = tensor(o), tdo = tensor(dout);
-  const ffa_gen_tensor tdq = maybe(dq), tdk = maybe(dk), tdv = maybe(dv);
-  check(ffa_gen_bwd(&a.p, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), dq.defined() ? &tdq : nullptr,
+  const ffa_gen_tensor tlo = maybe(o_lo), tdq = maybe(dq), tdk = maybe(dk), tdv = maybe(dv);
+  check(ffa_gen_bwd(&a.p, &tq, &tk, &tv, &to, o_lo.defined() ? &tlo : nullptr, &tdo, lse.data_ptr<float>(), dq.defined() ? &tdq : nullptr,
                     dk.defined() ? &tdk : nullptr, dk.defined() ? &tdv : nullptr, data(dbias), data(ws), bytes,
                     stream_of(q)),
         "ffa_gen_bwd");
@@ -184,29 +191,34 @@ Tensor general_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTe
                   const OptTensor& key_lengths, const OptTensor& query_offsets, int64_t query_offset,
                   at::IntArrayRef borders, bool both, bool causal, c10::optional<double> scale) {
   const Mask m{bias, key_lengths, query_offsets, query_offset, borders.vec(), both, causal, scale};
-  return std::get<0>(forward_impl(q, k, v, m, false));
+  return std::get<0>(forward_impl(q, k, v, m, false, false));
 }
 
-std::tuple<Tensor, Tensor> general_lse_op(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
-                                          const OptTensor& key_lengths, const OptTensor& query_offsets,
-                                          int64_t query_offset, at::IntArrayRef borders, bool both, bool causal,
-                                          c10::optional<double> scale) {
+Tensor some(const Tensor& t, const Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
+
+std::tuple<Tensor, Tensor, Tensor> general_lse_op(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                  const OptTensor& bias, const OptTensor& key_lengths,
+                                                  const OptTensor& query_offsets, int64_t query_offset,
+                                                  at::IntArrayRef borders, bool both, bool causal,
+                                                  c10::optional<double> scale, bool with_lo) {
   const Mask m{bias, key_lengths, query_offsets, query_offset, borders.vec(), both, causal, scale};
-  return forward_impl(q, k, v, m, true);
+  auto [o, lo, lse] = forward_impl(q, k, v, m, true, with_lo);
+  return {o, some(lo, q), lse};
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> general_backward_op(
-    const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& dout, const Tensor& lse,
-    const OptTensor& bias, const OptTensor& key_lengths, const OptTensor& query_offsets, int64_t query_offset,
+    const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const OptTensor& o_lo, const Tensor& dout,
+    const Tensor& lse, const OptTensor& bias, const OptTensor& key_lengths, const OptTensor& query_offsets, int64_t query_offset,
     at::IntArrayRef borders, bool both, bool causal, c10::optional<double> scale, bool want_dq, bool want_dkdv,
     bool want_dbias) {
   const Mask m{bias, key_lengths, query_offsets, query_offset, borders.vec(), both, causal, scale};
-  auto [dq, dk, dv, db] = backward_impl(q, k, v, o, dout, lse, m, want_dq, want_dkdv, want_dbias);
-  auto some = [&](const Tensor& t) { return t.defined() ? t : at::empty({0}, q.options()); };
-  return {some(dq), some(dk), some(dv), some(db)};
+  auto [dq, dk, dv, db] =
+      backward_impl(q, k, v, o, o_lo.value_or(Tensor()), dout, lse, m, want_dq, want_dkdv, want_dbias);
+  return {some(dq, q), some(dk, q), some(dv, q), some(db, q)};
 }
 
-// The autograd node of ffa_b200::general_attention.  It saves q, k, v, o, the LSE and the
+// The autograd node of ffa_b200::general_attention.  It saves q, k, v, o (and its remainder,
+// where the bias wants a gradient), the LSE and the
 // mask's tensors, and computes the gradients that are wanted.
 class GeneralAttention : public torch::autograd::Function<GeneralAttention> {
  public:
@@ -215,8 +227,8 @@ class GeneralAttention : public torch::autograd::Function<GeneralAttention> {
                         int64_t query_offset, std::vector<int64_t> borders, bool both, bool causal,
                         c10::optional<double> scale) {
     const Mask m{bias, key_lengths, query_offsets, query_offset, borders, both, causal, scale};
-    auto [o, lse] = forward_impl(q, k, v, m, true);
-    ctx->save_for_backward({q, k, v, o, lse, bias.value_or(Tensor()), key_lengths.value_or(Tensor()),
+    auto [o, lo, lse] = forward_impl(q, k, v, m, true, bias.has_value() && bias->requires_grad());
+    ctx->save_for_backward({q, k, v, o, lo, lse, bias.value_or(Tensor()), key_lengths.value_or(Tensor()),
                             query_offsets.value_or(Tensor())});
     ctx->saved_data["query_offset"] = query_offset;
     ctx->saved_data["borders"] = borders;
@@ -232,9 +244,9 @@ class GeneralAttention : public torch::autograd::Function<GeneralAttention> {
     const auto s = ctx->get_saved_variables();
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     auto& d = ctx->saved_data;
-    Mask m{opt(s[5]),
-           opt(s[6]),
+    Mask m{opt(s[6]),
            opt(s[7]),
+           opt(s[8]),
            d["query_offset"].toInt(),
            d["borders"].toIntVector(),
            d["both"].toBool(),
@@ -245,7 +257,7 @@ class GeneralAttention : public torch::autograd::Function<GeneralAttention> {
     torch::autograd::tensor_list r(11);
     {
       const at::AutoGradMode off(false);
-      auto [dq, dk, dv, db] = backward_impl(s[0], s[1], s[2], s[3], grads[0], s[4], m, want_dq, want_dkdv, want_dbias);
+      auto [dq, dk, dv, db] = backward_impl(s[0], s[1], s[2], s[3], s[4], grads[0], s[5], m, want_dq, want_dkdv, want_dbias);
       if (want_dq) r[0] = dq;
       r[1] = dk;
       r[2] = dv;
@@ -279,8 +291,8 @@ Tensor general_attention_op(const Tensor& q, const Tensor& k, const Tensor& v, c
 
 TORCH_LIBRARY_FRAGMENT(ffa_b200, m) {
   m.def("general(Tensor q, Tensor k, Tensor v, " FFA_MASK_ARGS ") -> Tensor");
-  m.def("general_lse(Tensor q, Tensor k, Tensor v, " FFA_MASK_ARGS ") -> (Tensor, Tensor)");
-  m.def("general_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor dout, Tensor lse, " FFA_MASK_ARGS
+  m.def("general_lse(Tensor q, Tensor k, Tensor v, " FFA_MASK_ARGS ", bool with_lo) -> (Tensor, Tensor, Tensor)");
+  m.def("general_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor? o_lo, Tensor dout, Tensor lse, " FFA_MASK_ARGS
         ", bool want_dq, bool want_dkdv, bool want_dbias) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("general_attention(Tensor q, Tensor k, Tensor v, " FFA_MASK_ARGS ") -> Tensor");
 }

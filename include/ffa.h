@@ -160,19 +160,24 @@ typedef struct ffa_gen_problem {
 
 /* Bytes of workspace that ffa_gen_fwd / ffa_gen_bwd need on this problem (0: none), or -1
  * (ffa_last_error says why).  The workspace holds nothing between calls. */
-long long ffa_gen_fwd_workspace(const ffa_gen_problem* p);
+long long ffa_gen_fwd_workspace(const ffa_gen_problem* p, int with_o_lo);
 long long ffa_gen_bwd_workspace(const ffa_gen_problem* p);
 
-/* Forward.  lse: [batch, q_heads, q_len] fp32 base-2 log-sum-exp, or NULL. */
+/* Forward.  lse: [batch, q_heads, q_len] fp32 base-2 log-sum-exp, or NULL.
+ * o_lo: a tensor like o for the remainder of O behind its rounding to bf16, or NULL; only with
+ * a bias.  With it P is multiplied in two parts as well, and o + o_lo is O to 16 bits: what
+ * the backward needs for the bias's gradient, whose sums cancel (about a fifth slower). */
 int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
-                const ffa_gen_tensor* o, float* lse, void* workspace, long long workspace_bytes, void* stream);
+                const ffa_gen_tensor* o, const ffa_gen_tensor* o_lo, float* lse, void* workspace,
+                long long workspace_bytes, void* stream);
 
 /* Deterministic backward (no atomics, fixed orders of summation).  dq may be NULL, and dk
  * with dv.  dbias: bf16 [buckets, q_heads] gradient of the bias, or NULL; it needs dq.
+ * o_lo: the forward's, or NULL (then delta is that of the rounded O).
  * Gradients are written whole: rows without a visible counterpart are 0. */
 int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
-                const ffa_gen_tensor* o, const ffa_gen_tensor* dout, const float* lse, const ffa_gen_tensor* dq,
-                const ffa_gen_tensor* dk, const ffa_gen_tensor* dv, void* dbias, void* workspace,
+                const ffa_gen_tensor* o, const ffa_gen_tensor* o_lo, const ffa_gen_tensor* dout, const float* lse,
+                const ffa_gen_tensor* dq, const ffa_gen_tensor* dk, const ffa_gen_tensor* dv, void* dbias, void* workspace,
                 long long workspace_bytes, void* stream);
 
 /* Most recent error message of the calling thread ("" if none). Copies at most n-1
