@@ -154,9 +154,9 @@ inline long long split_steps(long long ctas, long long slots, long long units, d
 
 struct FwdPlan {
   bool step;  // ffa_gen_step_kernel (few query rows for each key head), else ffa_gen_fwd_kernel
-  // step: groups of 16 rows of an item, items of a key head, CTAs, one item for each CTA
-  int rg, row_tiles, grid;
-  bool single;
+  // step: groups of 16 rows of an item, items of a key head, CTAs, and of those for each item
+  // (0: equal shares of all keys)
+  int rg, row_tiles, grid, cluster;
   // else: splits of the keys and their steps
   int n_split, per_split, keys_per_split;
   // workspace, offsets in floats (tables) and of the parts: O, LSE, entries (bytes)
@@ -177,11 +177,22 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias, bool exact) 
     const long long items = static_cast<long long>(p->batch) * p->kv_heads * f.row_tiles;
     const long long units = std::max<long long>(1, ceil_div(p->k_len, small_d ? 128 : 64));  // tiles of an item, at most
     const long long slots = kSMs * (f.rg == 1 ? 2 : 1);
-    // Equal shares, unless one item a CTA does: short items in one wave, where the join would
-    // cost more than the last tiles, and sequences too many to look through.
-    f.single = units == 1 || p->batch > 1024 || (items <= slots && items * units <= slots + 3 * items);
-    f.grid = static_cast<int>(f.single ? items : std::min(slots, items * units / 2));
-    f.join = !f.single;
+    // Few items: clusters of up to 16 CTAs (8 with 32 rows, whose CTAs fill an SM: a GPU holds
+    // too few clusters of 16 SMs), as many as fit, at least two tiles for each CTA.  Many: equal
+    // shares, unless the items have one or two tiles or there are too many sequences to look
+    // through.  Between them the estimate of time decides: 0.7 us for a tile of a CTA, and 11
+    // us more for shares and their join (B2 H32 over 4 heads D128, 16384 keys: 20 us against
+    // 33; 24 rows on 65536 keys: 111 against 68).
+    f.cluster = 1;
+    const int most = f.rg == 1 ? 16 : 8;
+    while (f.cluster < most && items * f.cluster * 2 <= slots && units >= f.cluster * 4) f.cluster *= 2;
+    const long long share_ctas = std::max<long long>(1, std::min(slots, items * units / 2));
+    const double mean = p->batch > 1 && p->key_lengths ? 0.67 : 1.0;
+    const double by_cluster = 0.7 * units / f.cluster * ceil_div(items * f.cluster, slots);
+    const double by_share = 0.7 * mean * items * units / share_ctas + 11.0;
+    if (units > 2 && p->batch <= 1024 && by_share < by_cluster) f.cluster = 0;
+    f.grid = static_cast<int>(f.cluster ? items * f.cluster : std::min(slots, items * units / 2));
+    f.join = f.cluster == 0;
     if (f.join) {
       const long long rows = 2LL * f.grid * 16 * f.rg;
       f.lse_off = rows * p->head_dim;
@@ -201,8 +212,9 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias, bool exact) 
     const double seen = std::min<double>(p->k_len, std::max(0.0, off + 0.5 * p->q_len)) / std::max(1, p->k_len);
     mean = std::max(1.0, mean * seen);
   }
-  // a step of one CTA: four of them share an SM at head dims up to 64
-  f.per_split = static_cast<int>(split_steps(heads * ceil_div(p->q_len, rows), kSMs * (small_d ? 4 : 1), units, mean,
+  // a step of one CTA: up to four of them share an SM at head dims up to 64
+  const long long slots = kSMs * (small_d ? FwdLayout<64>::ctas(exact) : FwdLayout<128>::ctas(exact));
+  f.per_split = static_cast<int>(split_steps(heads * ceil_div(p->q_len, rows), slots, units, mean,
                                              heads * p->q_len, p->head_dim, small_d ? 1.0 : 2.2, small_d ? 5.0 : 2.7,
                                              small_d ? 11.0 : 4.5));
   f.n_split = static_cast<int>(ceil_div(units, f.per_split));
@@ -263,6 +275,18 @@ inline int check_regs_once(const void* kernel, int needed, bool* done) {
   const int rc = check_launch_regs(kernel, needed);
   if (rc == FFA_OK) __atomic_store_n(done, true, __ATOMIC_RELEASE);
   return rc;
+}
+
+// Clusters of 16 CTAs for `kernel`, once for each device.
+inline int allow_clusters_once(const void* kernel, unsigned long long* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return set_error(FFA_ERR_LAUNCH, "cudaGetDevice failed");
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return FFA_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return set_error(FFA_ERR_LAUNCH, "cudaFuncSetAttribute(NonPortableClusterSizeAllowed) failed");
+  __atomic_fetch_or(done, bit, __ATOMIC_ACQ_REL);
+  return FFA_OK;
 }
 
 struct Call {
@@ -355,9 +379,25 @@ static int launch_gen_step_rg(const Call& c, const FwdPlan& f, float* ws) {
   if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
   JoinEntry* entries = ws ? reinterpret_cast<JoinEntry*>(reinterpret_cast<uintptr_t>(ws) + f.entry_off) : nullptr;
   float* part_lse = ws ? ws + f.lse_off : nullptr;
-  kern<<<f.grid, L::THREADS, smem, c.stream>>>(tk, tv, pr, c.bias, c.q, c.o, c.lse, ws, part_lse, entries, f.row_tiles,
-                                               f.single ? 1 : 0);
-  if ((rc = launched()) || !f.join) return rc;
+  if (f.cluster > 8) {
+    static unsigned long long sixteen = 0;
+    if ((rc = allow_clusters_once(reinterpret_cast<const void*>(kern), &sixteen))) return rc;
+  }
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(f.cluster > 1 ? f.cluster : 1);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(f.grid);
+  cfg.blockDim = dim3(L::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = c.stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = f.cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tk, tv, pr, c.bias, c.q, c.o, c.lse, ws, part_lse, entries,
+                                           f.row_tiles, f.cluster);
+  if (e != cudaSuccess) return set_error(FFA_ERR_LAUNCH, cudaGetErrorString(e));
+  if (!f.join) return FFA_OK;
   const int rows = std::min(L::ROWS, pr.G * pr.Sq);
   return launch_early(ffa_gen_step_join_kernel, dim3(f.grid, static_cast<unsigned>(ceil_div(rows, 4))), 128, 0,
                       c.stream, pr, ws, part_lse, entries, c.o, c.lse, f.row_tiles, L::ROWS);

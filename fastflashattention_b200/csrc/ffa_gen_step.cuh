@@ -5,14 +5,16 @@
 // that share a key head (row r = g * Sq + t) form items of 16 MT rows, the M of mma.sync
 // m16n8k16; the tensor cores' rate does not matter here, and a 128-row tcgen05 tile would
 // be empty.  Two CTAs to an SM, each a TMA warp and four warps that compute:
-//   * all keys of all items, laid end to end, are cut into equal shares (Work), one for each
-//     CTA, whatever the lengths of the sequences are.  The TMA warp walks through its share
-//     without a stop: HBM sees no gaps between items;
+//   * few items: a cluster of CTAs shares the keys of each, and joins its results through
+//     distributed shared memory, in the same launch;
+//   * many items: all keys of all items, laid end to end, are cut into equal shares (Work), one
+//     for each CTA, whatever the lengths of the sequences are.  The TMA warp walks through its
+//     share without a stop: HBM sees no gaps between items.  An item that several CTAs share
+//     is joined by ffa_gen_step_join_kernel, launched beside the last CTAs (programmatic
+//     dependent launch), which it waits for;
 //   * each warp takes 16 rows and a quarter of a tile's keys, and keeps its own running max,
 //     sum and O (registers); four warps are joined in shared memory at the end of a segment.  ROWS8: at
-//     most 8 rows, and the softmax of the other 8 is left out;
-//   * an item that several CTAs share is joined by ffa_gen_step_join_kernel, launched beside
-//     the last CTAs (programmatic dependent launch), which it waits for.
+//     most 8 rows, and the softmax of the other 8 is left out.
 #pragma once
 #include "ffa_gen_common.cuh"
 
@@ -39,6 +41,31 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Barrier of all threads of the cluster, with release and acquire of shared memory.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Load from the shared memory of the cluster's CTA `rank`, at this CTA's address `addr`.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
 // ------------------------------------------------------------------------------------
 // Work of a CTA
 // ------------------------------------------------------------------------------------
@@ -46,7 +73,8 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // KEYS keys as the sequence has, at least one (zeros have to be written too).  CTA c of n
 // gets the tiles [U c / n, U (c + 1) / n) of all U.  An item that crosses from one CTA into
 // the next ones is written in parts, in fp32, normalised, with its LSE: by the CTA in which
-// it starts in that CTA's slot 1, by the others in their slot 0.  `single`: one item a CTA.
+// it starts in that CTA's slot 1, by the others in their slot 0.  With `cluster` CTAs for
+// each item (one or more) the CTA of rank r takes the r-th equal part of its item.
 struct Segment {
   int b, item;    // sequence, item of the sequence
   int keys, off;  // the sequence's visible keys and offset
@@ -65,6 +93,7 @@ template <bool CAUSAL, bool OFFSETS>
 struct Work {
   long long left, total, end;  // tiles left to the CTA, all tiles, the tile behind the last segment
   int b, item, t, keys, off, tiles;
+  bool shares;
 
   __device__ __forceinline__ static int tiles_of(int keys, int tile) { return max(1, (keys + tile - 1) / tile); }
   __device__ __forceinline__ void enter(const Problem& pr, int seq, int tile) {
@@ -73,13 +102,14 @@ struct Work {
     keys = pr.keys(seq, off, CAUSAL);
     tiles = tiles_of(keys, tile);
   }
-  __device__ void start(const Problem& pr, int per_seq, int tile, bool single) {
-    if (single) {
-      enter(pr, blockIdx.x / per_seq, tile);
-      item = blockIdx.x % per_seq;
-      t = 0;
-      left = total = tiles;
-      end = 0;
+  __device__ void start(const Problem& pr, int per_seq, int tile, int cluster) {
+    shares = cluster == 0;
+    if (!shares) {
+      const int at = blockIdx.x / cluster, rank = blockIdx.x % cluster;
+      enter(pr, at / per_seq, tile);
+      item = at % per_seq;
+      t = static_cast<int>(static_cast<long long>(tiles) * rank / cluster);
+      left = static_cast<long long>(tiles) * (rank + 1) / cluster - t;
       return;
     }
     // tiles of each sequence: a warp takes 32 sequences at a time
@@ -135,7 +165,7 @@ struct Work {
         item = 0;
         enter(pr, b + 1, tile);
       }
-    } else if (s.t0 == 0 && s.nt < s.tiles) {
+    } else if (shares && s.t0 == 0 && s.nt < s.tiles) {
       // the CTAs up to the one that holds the item's last tile
       const long long last_tile = end + s.tiles - s.nt - 1;
       int last = static_cast<int>(((last_tile + 1) * gridDim.x - 1) / total);
@@ -168,8 +198,10 @@ struct StepLayout {
   static constexpr int SEG_OFF = ML_OFF + 2 * WARPS * 16 * 4;
   static constexpr int BAR_OFF = SEG_OFF + SEGS * 32;  // full[], empty[], seg_full[], seg_empty[]
   static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 2 * SEGS) * 8;
+  static constexpr int RES_OFF = MISC_OFF + 16;  // LSE of the CTA's rows, for its cluster
+  static_assert(ROWS * D * 4 <= RING, "the CTA's O for its cluster fits in the ring");
   // bias: bucket by position, then entries
-  static constexpr int LUT_OFF = MISC_OFF + 16;
+  static constexpr int LUT_OFF = RES_OFF + ROWS * 4;
   // bytes of the bias part for `heads` heads
   static int bias_bytes(const Bias& bias, int heads) { return lut_size(bias) * 2 + bias.buckets * heads * 4; }
 };
@@ -185,7 +217,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     ffa_gen_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ Problem pr, const __grid_constant__ Bias bias, const View q,
                         const View o, float* __restrict__ LSE, float* __restrict__ part, float* __restrict__ part_lse,
-                        JoinEntry* __restrict__ entries, int row_tiles, int single) {
+                        JoinEntry* __restrict__ entries, int row_tiles, int cluster) {
   using L = StepLayout<D, RG>;
   constexpr int KS = D / 16;          // K-steps of Q K^T
   constexpr int NG = L::WKEYS / 16;   // groups of 16 keys of a warp
@@ -223,10 +255,10 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
   if (warp == L::WARPS) {
     // ------------------------------------------------------------------ producer
     Work<CAUSAL, CAUSAL || BIAS> work;
-    work.start(pr, per_seq, L::KEYS, single != 0);
+    work.start(pr, per_seq, L::KEYS, cluster);
     if (lane == 0) {
       const uint64_t once = policy_evict_first();
-      JoinEntry shared{0, 0, 0, work.left > 0 && work.t > 0};
+      JoinEntry shared{0, 0, 0, work.shares && work.left > 0 && work.t > 0};
       bool ok = true;
       int it = 0;
       for (int n = 0; ok; ++n) {
@@ -255,6 +287,11 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
       if (*abort_flag)
         for (int x = max(0, it - STAGES); x < it; ++x) mbar_wait_drain(full(x), (x / STAGES) & 1);
     }
+    __syncwarp();
+    if (cluster > 1) {  // the compute warps' two barriers
+      cluster_barrier();
+      cluster_barrier();
+    }
     return;
   }
 
@@ -264,6 +301,10 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
   if (BIAS)
     for (int t = threadIdx.x; t <= bias.left + bias.right; t += NC)
       lut[t] = static_cast<unsigned short>(bias.bucket(t - bias.left));
+  // cluster: this CTA's O (the ring's room, once it is read) and LSE, -inf without keys
+  float* res = reinterpret_cast<float*>(smem);
+  float* res_lse = reinterpret_cast<float*>(smem + L::RES_OFF);
+  if (cluster > 1 && threadIdx.x < ROWS) res_lse[threadIdx.x] = -INFINITY;
   bool ok = true;
   int it = 0;  // tile of the CTA
   for (int n = 0;; ++n) {
@@ -481,7 +522,9 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
         a.w = fmaf(f[w], y.w, a.w);
       }
       const int col = round * JOIN + c4;
-      if (ok && col < pr.D) {
+      if (ok && cluster > 1) {
+        *reinterpret_cast<float4*>(res + r * D + col) = a;
+      } else if (ok && col < pr.D) {
         if (sg.whole())
           *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + col) =
               make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
@@ -491,12 +534,52 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     }
     if (ok && valid && c4 == 0) {
       const float lse = total == 0.f ? -INFINITY : m + __log2f(total);
-      if (!sg.whole())
+      if (cluster > 1)
+        res_lse[r] = lse;
+      else if (!sg.whole())
         part_lse[prow] = lse;
       else if (LSE != nullptr)
         LSE[(b * static_cast<long long>(pr.Hq) + h) * pr.Sq + t] = lse;
     }
   }
+
+  if (cluster <= 1) return;
+  // -------------------------------------------------------------------- join the cluster
+  // Each CTA takes every `cluster`-th group of four columns from all the others' results,
+  // weighed with 2^(LSE - max LSE).
+  cluster_barrier();
+  const int rank = blockIdx.x % cluster, at = blockIdx.x / cluster;
+  const int b = at / per_seq, item = at % per_seq;
+  const int hk = item / row_tiles, row0 = item % row_tiles * ROWS, n_rows = min(ROWS, rows - row0);
+  const int groups = pr.D / 4;
+  for (int x = rank * NC + threadIdx.x; x < n_rows * groups; x += cluster * NC) {
+    const int r = x / groups, c = x % groups * 4;
+    const uint32_t o_at = smem_u32(res + r * D + c), lse_at = smem_u32(res_lse + r);
+    float m = -INFINITY, total = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < cluster; ++p) {  // the loads of four CTAs do not wait for one another
+      const float lse = ld_cluster(lse_at, p);
+      const float4 y = ld_cluster4(o_at, p);
+      const float m_new = fmaxf(m, lse), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float f = fast_exp2(m - m_safe), w = lse == -INFINITY ? 0.f : fast_exp2(lse - m_safe);
+      m = m_new;
+      total = fmaf(total, f, w);
+      // a CTA without keys has left the ring's contents here
+      a.x = fmaf(a.x, f, w == 0.f ? 0.f : w * y.x);
+      a.y = fmaf(a.y, f, w == 0.f ? 0.f : w * y.y);
+      a.z = fmaf(a.z, f, w == 0.f ? 0.f : w * y.z);
+      a.w = fmaf(a.w, f, w == 0.f ? 0.f : w * y.w);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const long long h = hk * pr.G + (row0 + r) / pr.Sq;
+    const int t = (row0 + r) % pr.Sq;
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(o.p) + b * o.sb + h * o.sh + t * o.ss + c) =
+        make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+    if (c == 0 && LSE != nullptr)
+      LSE[(b * static_cast<long long>(pr.Hq) + h) * pr.Sq + t] = total == 0.f ? -INFINITY : m + __log2f(total);
+  }
+  cluster_barrier();  // nobody leaves while another reads its shared memory
 }
 
 // Join the parts of the items that cross CTAs: O = sum_p w_p O_p / sum_p w_p with
