@@ -33,33 +33,53 @@ def _rows_problem(name, t, batch, device):
     return None
 
 
+def _inside(query, key, value, enable_gqa):
+    """Whether the three tensors meet the contract: the checks of ``_shape_reason`` without its
+    messages, for calls whose kernels take less time than the checks' bookkeeping."""
+    t, bf16 = torch.Tensor, torch.bfloat16
+    if not (isinstance(query, t) and isinstance(key, t) and isinstance(value, t)):
+        return False
+    qs, ks = query.shape, key.shape
+    if len(qs) != 4 or len(ks) != 4 or value.shape != ks:
+        return False
+    batch, heads, rows, dim = qs
+    kv_heads, keys = ks[1], ks[2]
+    return (batch == ks[0] and dim == ks[3] and dim % 8 == 0 and 8 <= dim <= 128
+            and (heads == kv_heads or (enable_gqa and kv_heads > 0 and heads % kv_heads == 0))
+            and rows < _MAX_LEN and keys < _MAX_LEN
+            and query.dtype is bf16 and key.dtype is bf16 and value.dtype is bf16
+            and query.is_cuda and key.is_cuda and value.is_cuda
+            and query.get_device() == key.get_device() == value.get_device())
+
+
 def _shape_reason(query, key, value, key_lengths, scale, enable_gqa):
     """Why the tensors are outside the contract of general attention, or ``None``."""
-    from . import _tensor_problem
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        problem = _tensor_problem(name, t)
-        if problem is not None:
-            return problem
-        if t.device != query.device:
-            return f"{name} is on device '{t.device}'; it must be on '{query.device}' with the query"
-    qs, ks, vs = (tuple(t.shape) for t in (query, key, value))
-    if ks != vs:
-        return f"shapes of key {ks} and value {vs} differ"
-    if qs[0] != ks[0] or qs[3] != ks[3]:
-        return f"query {qs} and key {ks} must have the same batch and head_dim"
-    if qs[3] % 8 != 0 or not 8 <= qs[3] <= 128:
-        return f"head_dim={qs[3]}; must be a multiple of 8, at most 128"
-    if qs[1] != ks[1]:
-        if not enable_gqa:
-            return f"query has {qs[1]} heads and key {ks[1]}; pass enable_gqa=True to share key heads"
-        if ks[1] == 0 or qs[1] % ks[1] != 0:
-            return f"query heads ({qs[1]}) must be a multiple of key heads ({ks[1]})"
-    if max(qs[2], ks[2]) >= _MAX_LEN:
-        return f"lengths {qs[2]} and {ks[2]}; must be below 2^29"
+    if not _inside(query, key, value, enable_gqa):
+        from . import _tensor_problem
+        for name, t in (("query", query), ("key", key), ("value", value)):
+            problem = _tensor_problem(name, t)
+            if problem is not None:
+                return problem
+            if t.device != query.device:
+                return f"{name} is on device '{t.device}'; it must be on '{query.device}' with the query"
+        qs, ks, vs = (tuple(t.shape) for t in (query, key, value))
+        if ks != vs:
+            return f"shapes of key {ks} and value {vs} differ"
+        if qs[0] != ks[0] or qs[3] != ks[3]:
+            return f"query {qs} and key {ks} must have the same batch and head_dim"
+        if qs[3] % 8 != 0 or not 8 <= qs[3] <= 128:
+            return f"head_dim={qs[3]}; must be a multiple of 8, at most 128"
+        if qs[1] != ks[1]:
+            if not enable_gqa:
+                return f"query has {qs[1]} heads and key {ks[1]}; pass enable_gqa=True to share key heads"
+            if ks[1] == 0 or qs[1] % ks[1] != 0:
+                return f"query heads ({qs[1]}) must be a multiple of key heads ({ks[1]})"
+        if max(qs[2], ks[2]) >= _MAX_LEN:
+            return f"lengths {qs[2]} and {ks[2]}; must be below 2^29"
     if scale is not None and not math.isfinite(scale):
         return f"scale={scale}; must be finite"
     if key_lengths is not None:
-        return _rows_problem("key_lengths", key_lengths, qs[0], query.device)
+        return _rows_problem("key_lengths", key_lengths, query.shape[0], query.device)
     return None
 
 
@@ -111,8 +131,22 @@ def bucket_borders(side: int, max_distance: int) -> tuple:
     return tuple(out)
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+_operators = None
+
+
+def _op(wants_grad):
+    """The operator of ``torch.ops.ffa_b200`` for a call with or without gradients (the
+    overload itself: finding it by name costs a microsecond a call)."""
+    global _operators
+    if _operators is None:
+        ops = _lib.ops()
+        _operators = (ops.general.default, ops.general_attention.default)
+    return _operators[wants_grad]
+
+
+def _refuse(reason):
+    from . import UnsupportedConfig
+    raise UnsupportedConfig(reason)
 
 
 def cross_attention(query, key, value, key_lengths=None, scale=None, enable_gqa=False):
@@ -132,13 +166,11 @@ def cross_attention(query, key, value, key_lengths=None, scale=None, enable_gqa=
     The backward is deterministic.  A few queries (Hq / Hkv * Sq up to 64, a decoding step)
     take one pass over the keys that is split over the SMs.
     """
-    from . import UnsupportedConfig
     reason = _shape_reason(query, key, value, key_lengths, scale, enable_gqa)
     if reason is not None:
-        raise UnsupportedConfig(reason)
-    ops = _lib.ops()
-    op = ops.general_attention if _wants_grad(query, key, value) else ops.general
-    return op(query, key, value, None, key_lengths, None, 0, (), False, False, scale)
+        _refuse(reason)
+    grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)
+    return _op(grad)(query, key, value, None, key_lengths, None, 0, (), False, False, scale)
 
 
 def relative_attention(query, key, value, bias, max_distance=128, bidirectional=None, is_causal=False,
@@ -161,15 +193,14 @@ def relative_attention(query, key, value, bias, max_distance=128, bidirectional=
     0 for a sequence that attends to itself, ``length - Sq`` for the newest Sq tokens over a
     cache of ``length`` keys.  A tensor may change between the replays of a captured graph.
     """
-    from . import UnsupportedConfig
     reason = _shape_reason(query, key, value, key_lengths, scale, enable_gqa)
     if reason is None:
         reason = _bias_reason(query, bias, max_distance, bidirectional, is_causal, query_offset)
     if reason is not None:
-        raise UnsupportedConfig(reason)
+        _refuse(reason)
     both = (not is_causal) if bidirectional is None else bool(bidirectional)
     borders = bucket_borders(bias.shape[0] // 2 if both else bias.shape[0], max_distance)
     offsets, offset = (query_offset, 0) if isinstance(query_offset, torch.Tensor) else (None, query_offset)
-    ops = _lib.ops()
-    op = ops.general_attention if _wants_grad(query, key, value, bias) else ops.general
-    return op(query, key, value, bias, key_lengths, offsets, offset, borders, both, bool(is_causal), scale)
+    grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad
+                                        or bias.requires_grad)
+    return _op(grad)(query, key, value, bias, key_lengths, offsets, offset, borders, both, bool(is_causal), scale)
