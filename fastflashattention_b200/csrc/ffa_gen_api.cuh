@@ -294,6 +294,7 @@ struct Call {
   Bias bias;
   View q, k, v, o, o_lo, dout, dq, dk, dv;
   float* lse;
+  bool want_dbias;
   cudaStream_t stream;
 };
 
@@ -428,8 +429,7 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   }
   auto kern = ffa_gen_dkdv_kernel<D, CAUSAL, BIAS>;
   static unsigned long long configured = 0;
-  constexpr int most = L::TAB_OFF + (BIAS ? kTableMax * 4 : 0);
-  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), most, &configured))) return rc;
+  if ((rc = set_smem_once(reinterpret_cast<const void*>(kern), L::MOST, &configured))) return rc;
   if constexpr (D == 128) {
     static bool configured_regs = false;
     if ((rc = check_regs_once(reinterpret_cast<const void*>(kern), bwd::LAUNCH_REGS_NEEDED, &configured_regs)))
@@ -474,11 +474,12 @@ static int launch_gen_dq(const Call& c, const BwdPlan& w, float* ws) {
   const float* tables = ws + w.table_off;
   const unsigned short* lut = reinterpret_cast<const unsigned short*>(ws + w.lut_off);
   const float* lse = c.lse;
+  float* bias_part = c.want_dbias ? ws + w.bias_off : nullptr;
   if (BIAS)
     return launch_early(kern, grid, W::THREADS, smem, c.stream, tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.o_lo, c.dout,
-                        lse, ws, ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split, group);
+                        lse, ws, ws + w.stat_floats, ws + w.dq_off, bias_part, w.dq_split, group);
   kern<<<grid, W::THREADS, smem, c.stream>>>(tk, tv, tdq, pr, c.bias, tables, lut, c.q, c.o, c.o_lo, c.dout, lse, ws,
-                                             ws + w.stat_floats, ws + w.dq_off, ws + w.bias_off, w.dq_split, group);
+                                             ws + w.stat_floats, ws + w.dq_off, bias_part, w.dq_split, group);
   return launched();
 }
 
@@ -626,6 +627,7 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
   };
   if (want_dq && queries) {
     c.dq = view(dq);
+    c.want_dbias = dbias != nullptr;
     if ((rc = dispatch<RunDq>(c, p->causal, w, ws))) return rc;
   }
   if (want_dkdv && keys) {

@@ -206,8 +206,7 @@ struct DkdvLayout {
   static constexpr int STEP = BwdShape<D>::STEP;
   static constexpr int KV_TILE = 128 * D * 2;   // K, V (resident)
   static constexpr int TILE = STEP * D * 2;     // Q, dO (streamed)
-  // three Q slots, as in the plain kernel; at D = 128 the bias table takes the third's room
-  static constexpr int Q_STAGES = (BIAS && D == 128) ? 2 : 3;
+  static constexpr int Q_STAGES = 3;
   static constexpr int DO_STAGES = 2;
   static constexpr int K_OFF = 0;
   static constexpr int V_OFF = KV_TILE;
@@ -222,9 +221,14 @@ struct DkdvLayout {
   // ds_ready, final, drain, s_free
   static constexpr int NBARS = 1 + 2 * Q_STAGES + 2 * DO_STAGES + 7;
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
+  // At D = 128 there is room for the bias table or for a third Q slot.  The slot is worth
+  // more, and the steps near the diagonal read the table from L2 (B2 H16 S4096 causal: 257 us
+  // against 281 with the table; with all steps near, distance 1024, XX against 285).
+  static constexpr bool TAB_SHARED = BIAS && D == 64;
   static constexpr int TAB_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
+  static constexpr int MOST = TAB_OFF + (TAB_SHARED ? kTableMax * 4 : 0);
   // no alignment slack (see bwd::DkdvLayout)
-  static int smem_bytes(const Bias& bias) { return TAB_OFF + (BIAS ? table_size(bias) * 4 : 0); }
+  static int smem_bytes(const Bias& bias) { return TAB_OFF + (TAB_SHARED ? table_size(bias) * 4 : 0); }
 };
 
 template <int D, bool CAUSAL, bool BIAS, int EMU = bwd_emu(BIAS)>
@@ -262,7 +266,6 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
   const uint32_t s_free = s_full + 48;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
-  float* tab = reinterpret_cast<float*>(smem + L::TAB_OFF);
   auto q_addr = [&](int i) { return sbase + L::Q_OFF + (i % QS) * L::TILE; };
   auto do_addr = [&](int i) { return sbase + L::DO_OFF + (i % DS) * L::DO_STAGE_BYTES; };
   auto lse_smem = [&](int i) {
@@ -493,11 +496,18 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     for (int hg = ns > 0 ? st0 / nqb : 0; i < ns || !ok; ++hg) {
       if (!ok && hg * nqb >= st0 + ns) break;
       float bias_l = 0.f, bias_r = 0.f;
+      const float* tab = nullptr;  // the head's table
       if (BIAS) {
         asm volatile("griddepcontrol.wait;" ::: "memory");  // the tables are written
-        ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table
-        copy_table(tab, tables, hk * pr.G + hg, bias, threadIdx.x, 256);
-        ok = named_barrier_and(2, 256, ok);
+        if constexpr (L::TAB_SHARED) {
+          float* room = reinterpret_cast<float*>(smem + L::TAB_OFF);
+          ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table
+          copy_table(room, tables, hk * pr.G + hg, bias, threadIdx.x, 256);
+          ok = named_barrier_and(2, 256, ok);
+          tab = room;
+        } else {
+          tab = tables + static_cast<long long>(hk * pr.G + hg) * table_size(bias);
+        }
         bias_l = tab[0];
         bias_r = tab[table_last(bias)];
       }
@@ -1074,7 +1084,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(ds_ready);
-      if (BIAS) {
+      if (BIAS && bias_part != nullptr) {
         // this step's share of dbias, while the tensor core is at dQ(j)
         if (near) {
           add_near_block<CW>(p, kc - (off + qw), bias, lut, sums, diag, lane);
@@ -1096,7 +1106,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     const bool empty = nk <= 0;
     const bool done = ok && (empty || mbar_wait(final_bar, 0, abort_flag, kErrGenDqCompute));
     tc_fence_after();
-    if (BIAS) {
+    if (BIAS && bias_part != nullptr) {
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) {
         sum_l += __shfl_xor_sync(0xffffffffu, sum_l, x);
