@@ -223,7 +223,8 @@ struct DkdvLayout {
   static constexpr int MISC_OFF = BAR_OFF + NBARS * 8;
   // At D = 128 there is room for the bias table or for a third Q slot.  The slot is worth
   // more, and the steps near the diagonal read the table from L2 (B2 H16 S4096 causal: 257 us
-  // against 281 with the table; with all steps near, distance 1024, XX against 285).
+  // against 281 with the table; with all steps near, distance 1024, 262
+  // against 284).
   static constexpr bool TAB_SHARED = BIAS && D == 64;
   static constexpr int TAB_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
   static constexpr int MOST = TAB_OFF + (TAB_SHARED ? kTableMax * 4 : 0);
@@ -636,6 +637,10 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
 // ====================================================================================
 // dQ and dbias
 // ====================================================================================
+// Floats of scratch of a warp for add_near_block: 47 diagonals of each chain.
+template <int CW>
+constexpr int kDiagFloats = CW / 16 * 48;
+
 template <int D, bool BIAS>
 struct DqLayout {
   static constexpr int STEP = BwdShape<D>::STEP;
@@ -655,7 +660,7 @@ struct DqLayout {
   // bias: diagonal scratch of each warp, table (fp32 by position), buckets by position,
   // per-warp sums
   static constexpr int DIAG_OFF = DELTA_OFF + 512;
-  static constexpr int TAB_OFF = DIAG_OFF + (BIAS ? 8 * 96 * 4 : 0);
+  static constexpr int TAB_OFF = DIAG_OFF + (BIAS ? 8 * kDiagFloats<BwdShape<D>::CW> * 4 : 0);
   static int smem_bytes(const Bias& bias) {
     return TAB_OFF + (BIAS ? table_size(bias) * 4 + lut_size(bias) * 2 + 8 * bias.buckets * 4 : 0) + 1024;
   }
@@ -733,42 +738,67 @@ __device__ __forceinline__ float row_dot_to_tmem(const __nv_bfloat16* __restrict
 
 // Add the diagonal sums of a warp's 32 x CW block of dS (lane = row, ds[e] = column e) to
 // the warp's sums by bucket.  `r0`: relative position of lane 0, column 0; `lut`: bucket of
-// position r at r + left; `diag`: 96 floats of scratch of this warp.
+// position r at r + left; `diag`: scratch of this warp.
+//
+// A chain takes 16 columns.  Before its column e, lane l holds the sum of diagonal e - l over
+// the lanes below it; after it lane 31's diagonal e - 31 is complete, and comes round to
+// lane 0.  The chains are independent: one over all columns would wait for 64 shuffles in
+// turn.  For the same reason the chunks of diagonals are summed by bucket side by side.  (dQ of
+// B2 H16 S4096 D128 causal, distance 256 and 1024: 289 and 365 us with one chain and one
+// chunk after another, 267 and 315 so.  Chains of 8 columns: 268 and 317.  As a product with a
+// selection matrix, mma.sync, beside the kernel's own: 327 and 370.)
 template <int CW>
 __device__ __forceinline__ void add_near_block(const float (&ds)[CW], int r0, const Bias& bias,
                                                const unsigned short* lut, float* sums, float* diag, int lane) {
-  // before column e, lane l holds the sum of diagonal e - l over the lanes below it; after
-  // it lane 31's diagonal e - 31 is complete, and comes round to lane 0
-  float a = 0.f;
+  constexpr int CHAINS = CW / 16;
+  float a[CHAINS] = {};
 #pragma unroll
-  for (int e = 0; e < CW; ++e) {
-    if (e > 0) {
-      a = __shfl_sync(0xffffffffu, a, (lane + 31) & 31);
-      if (lane == 0) {
-        diag[e - 1] = a;  // diagonal e - 32, kept 31 places on
-        a = 0.f;
+  for (int e = 0; e < 16; ++e) {
+#pragma unroll
+    for (int q = 0; q < CHAINS; ++q) {
+      if (e > 0) {
+        a[q] = __shfl_sync(0xffffffffu, a[q], (lane + 31) & 31);
+        if (lane == 0) {
+          diag[q * 48 + e - 1] = a[q];  // diagonal e - 32, kept 31 places on
+          a[q] = 0.f;
+        }
       }
+      a[q] += ds[q * 16 + e];
     }
-    a += ds[e];
   }
-  diag[CW + 30 - lane] = a;  // diagonal CW - 1 - l
-  __syncwarp();
-#pragma unroll 1
-  for (int c = 0; c < CW + 32; c += 32) {
-    const int x = c + lane;  // CW + 31 diagonals; the last lane of the last chunk has none
-    float v = x < CW + 31 ? diag[x] : 0.f;
-    const int r = min(max(r0 + x - 31, -bias.left), bias.right);
-    const int u = lut[r + bias.left];
-    // positions of one bucket are neighbours: sums of runs of equal buckets
-    const int prev = __shfl_up_sync(0xffffffffu, u, 1);
-    const uint32_t heads = __ballot_sync(0xffffffffu, lane == 0 || prev != u);
-    const int head = 31 - __clz(heads & (0xffffffffu >> (31 - lane)));
 #pragma unroll
-    for (int k = 1; k < 32; k <<= 1) {
-      const float y = __shfl_up_sync(0xffffffffu, v, k);
-      if (lane - k >= head) v += y;
+  for (int q = 0; q < CHAINS; ++q) diag[q * 48 + 46 - lane] = a[q];  // diagonal 15 - l
+  __syncwarp();
+  constexpr int NC = CW / 32 + 1;  // chunks of 32 of the CW + 31 diagonals; the last lane of the last one has none
+  float v[NC];
+  int u[NC], head[NC];
+  bool last[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int x = c * 32 + lane;
+    v[c] = 0.f;
+#pragma unroll
+    for (int q = 0; q < CHAINS; ++q)
+      if (x >= q * 16 && x < q * 16 + 47) v[c] += diag[q * 48 + x - q * 16];
+    const int r = min(max(r0 + x - 31, -bias.left), bias.right);
+    u[c] = lut[r + bias.left];
+    // positions of one bucket are neighbours: sums of runs of equal buckets
+    const int prev = __shfl_up_sync(0xffffffffu, u[c], 1);
+    const uint32_t heads = __ballot_sync(0xffffffffu, lane == 0 || prev != u[c]);
+    head[c] = 31 - __clz(heads & (0xffffffffu >> (31 - lane)));
+    last[c] = lane == 31 || ((heads >> (lane + 1)) & 1u);  // the run's last lane
+  }
+#pragma unroll
+  for (int k = 1; k < 32; k <<= 1) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float y = __shfl_up_sync(0xffffffffu, v[c], k);
+      if (lane - k >= head[c]) v[c] += y;
     }
-    if (lane == 31 || ((heads >> (lane + 1)) & 1u)) sums[u] += v;  // the run's last lane; runs differ in bucket
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {  // a chunk's runs differ in bucket, those of two chunks need not
+    if (last[c]) sums[u[c]] += v[c];
     __syncwarp();
   }
 }
@@ -1011,7 +1041,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     const uint32_t t_s = tmem + lane_off + CW * g;
     const uint32_t t_dp = tmem + lane_off + L::DP + CW * g;
     float* sums = sums_all + warp * bias.buckets;
-    float* diag = reinterpret_cast<float*>(smem + L::DIAG_OFF) + warp * 96;
+    float* diag = reinterpret_cast<float*>(smem + L::DIAG_OFF) + warp * kDiagFloats<CW>;
     float bias_l = 0.f, bias_r = 0.f, sum_l = 0.f, sum_r = 0.f;
     if (BIAS) {
       bias_l = tab[0];
