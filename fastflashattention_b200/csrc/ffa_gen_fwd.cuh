@@ -58,17 +58,24 @@ struct FwdLayout {
   static int smem_bytes(const Bias& bias) { return TAB_OFF + (bias.table ? table_size(bias) * 4 : 0) + 1024; }
 };
 
+// max(a, b, c), NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Row max of 64 scores (16 chains of three-input maxima, then a short tree).
 __device__ __forceinline__ float row_max64(const uint32_t (&a)[32], const uint32_t (&b)[32]) {
   float x[16];
 #pragma unroll
   for (int u = 0; u < 16; ++u)
-    x[u] = fmax3(__uint_as_float(a[u]), __uint_as_float(a[16 + u]), __uint_as_float(b[u]));
+    x[u] = max3_nan(__uint_as_float(a[u]), __uint_as_float(a[16 + u]), __uint_as_float(b[u]));
 #pragma unroll
-  for (int u = 0; u < 16; u += 2) x[u] = fmax3(x[u], __uint_as_float(b[16 + u]), __uint_as_float(b[17 + u]));
-  const float y0 = fmax3(x[0], x[1], x[2]), y1 = fmax3(x[3], x[4], x[5]), y2 = fmax3(x[6], x[7], x[8]);
-  const float y3 = fmax3(x[9], x[10], x[11]), y4 = fmax3(x[12], x[13], x[14]);
-  return fmax3(fmax3(y0, y1, y2), fmax3(y3, y4, x[15]), y0);
+  for (int u = 0; u < 16; u += 2) x[u] = max3_nan(x[u], __uint_as_float(b[16 + u]), __uint_as_float(b[17 + u]));
+  const float y0 = max3_nan(x[0], x[1], x[2]), y1 = max3_nan(x[3], x[4], x[5]), y2 = max3_nan(x[6], x[7], x[8]);
+  const float y3 = max3_nan(x[9], x[10], x[11]), y4 = max3_nan(x[12], x[13], x[14]);
+  return max3_nan(max3_nan(y0, y1, y2), max3_nan(y3, y4, x[15]), y0);
 }
 
 template <int D, bool CAUSAL, bool BIAS, bool EXACT, int EMU = D == 64 ? 2 : 0>
@@ -329,9 +336,11 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
         tmem_ld32(t_s + 64 * hf, sa);
         tmem_ld32(t_s + 64 * hf + 32, sb);
         tmem_ld_wait();
-        tmax = fmaxf(tmax, row_max64(sa, sb));
+        tmax = max3_nan(tmax, tmax, row_max64(sa, sb));
       }
       tmax = BIAS ? fmaf(tmax, c, fb) : tmax * c;
+      // a visible score that is NaN or +inf makes the row NaN (exp2_fma2 would lose it)
+      if (!(tmax < INFINITY)) l = __int_as_float(0x7fffffff);
       const float m_new = fmaxf(m_used, tmax);
       const bool need = m_new > m_used + fwd::RESCALE_THRESHOLD;
       if (__any_sync(0xffffffffu, need)) {
@@ -395,12 +404,12 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       }
     }
     // Epilogue.  Every thread of the warpgroup reaches the barrier, finished or not.  A row
-    // without keys (no max) is 0: the sum holds what the polynomial makes of 2^-inf, and
-    // tensor memory may hold anything.  Its Q tile, where the output is staged, may still be
+    // without keys (no max, and none of them NaN) is 0: the sum holds what the polynomial
+    // makes of 2^-inf, and tensor memory may hold anything.  Its Q tile, where the output is staged, may still be
     // on its way when the other tile has keys.
     const bool done = ok && (n_kv == 0 || mbar_wait(cnt > 0 ? o_final(i) : q_full, 0, abort_flag, kErrGenFwdSoftmax));
     tc_fence_after();
-    const bool valid = done && grow < pr.Sq, none = m_used == -INFINITY;
+    const bool valid = done && grow < pr.Sq, none = m_used == -INFINITY && l == l;
     const float inv_l = none ? 0.f : 1.f / l;
     const float lse = none ? -INFINITY : m_used + __log2f(l);
     const uint32_t o_tile = sbase + L::Q_OFF + i * L::Q_TILE;

@@ -593,36 +593,60 @@ __global__ void __launch_bounds__(128)
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * 4 + (threadIdx.x >> 5);  // of the item
   asm volatile("griddepcontrol.wait;" ::: "memory");    // the parts are written
-  const JoinEntry e = entries[blockIdx.x];
-  if (e.parts == 0) return;
-  const int r = e.item % row_tiles * rows + row;
-  if (r >= pr.G * pr.Sq) return;
-  const int h = e.item / row_tiles * pr.G + r / pr.Sq, t = r % pr.Sq;
-  // row of part p: slot 1 of the first CTA, slot 0 of the next ones
+  // Row of part p: slot 1 of the first CTA, slot 0 of the next ones.  A lane takes the LSE of
+  // one part of 32; its loads do not wait for one another (a slot that was not written is
+  // inside the workspace, and its value is dropped), nor do those of the parts themselves.
   auto at = [&](int p) { return (2LL * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * rows + row; };
-  auto lse_of = [&](int p) { return p == 0 || entries[blockIdx.x + p].slot0 ? part_lse[at(p)] : -INFINITY; };
-  float m = -INFINITY;
-  for (int p = lane; p < e.parts; p += 32) m = fmaxf(m, lse_of(p));
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  float total = 0.f;
+  const int left = gridDim.x - blockIdx.x;  // parts there can be
+  const JoinEntry e = entries[blockIdx.x];
+  const int item_row = e.item % row_tiles * rows + row;
+  float m = -INFINITY, total = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   const int c = lane * 4;
-  if (m > -INFINITY) {
-#pragma unroll 8
-    for (int p = 0; p < e.parts; ++p) {
-      const float lse = lse_of(p);
-      const float w = exp2f(lse - m);
-      total += w;
-      if (c < pr.D && lse > -INFINITY) {
-        const float4 x = *reinterpret_cast<const float4*>(part + at(p) * pr.D + c);
-        a.x = fmaf(w, x.x, a.x);
-        a.y = fmaf(w, x.y, a.y);
-        a.z = fmaf(w, x.z, a.z);
-        a.w = fmaf(w, x.w, a.w);
+  for (int p0 = 0; p0 < left; p0 += 32) {
+    float lse = -INFINITY;
+    if (p0 + lane < left) {
+      const bool written = p0 + lane == 0 || entries[blockIdx.x + p0 + lane].slot0;
+      const float y = part_lse[at(p0 + lane)];
+      if (written && p0 + lane < e.parts) lse = y;
+    }
+    if (p0 >= e.parts || item_row >= pr.G * pr.Sq) break;  // the same for the whole warp
+    const float m_old = m;
+    float top = lse;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    m = fmaxf(m_old, top);
+    const float m_safe = m == -INFINITY ? 0.f : m;
+    const float f = exp2f(m_old - m_safe), w = exp2f(lse - m_safe);  // NaN where the part is
+    float sum = w;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    total = fmaf(total, f, sum);
+    a.x *= f;
+    a.y *= f;
+    a.z *= f;
+    a.w *= f;
+    const int n = min(32, e.parts - p0);
+    for (int q0 = 0; q0 < n; q0 += 8) {
+      float4 x[8];
+      float wq[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        wq[q] = __shfl_sync(0xffffffffu, w, q0 + q);  // 0 for a part that there is not
+        x[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (wq[q] > 0.f && c < pr.D) x[q] = *reinterpret_cast<const float4*>(part + at(p0 + q0 + q) * pr.D + c);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        a.x = fmaf(wq[q], x[q].x, a.x);
+        a.y = fmaf(wq[q], x[q].y, a.y);
+        a.z = fmaf(wq[q], x[q].z, a.z);
+        a.w = fmaf(wq[q], x[q].w, a.w);
       }
     }
   }
+  if (e.parts == 0 || item_row >= pr.G * pr.Sq) return;
+  const int h = e.item / row_tiles * pr.G + item_row / pr.Sq, t = item_row % pr.Sq;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   if (c < pr.D) {
     __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(o.p) + e.b * o.sb + h * o.sh + t * o.ss + c;

@@ -320,6 +320,42 @@ def test_bias_gradient_against_differences():
     assert abs((g.double() * u).sum() - slope) <= (bound * u.abs()).sum() + 1e-4
 
 
+# ---- values that are not finite -------------------------------------------------------------
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("B, H, Sq, Sk, D", [
+    (1, 2, 1, 40, 64), (2, 2, 2, 5000, 128), (2, 16, 3, 20001, 128), (40, 16, 1, 700, 64),  # cluster, shares
+    (2, 2, 130, 300, 64), (2, 2, 130, 300, 128), (1, 2, 130, 9000, 64), (1, 2, 260, 5000, 128),  # whole, split keys
+])
+def test_values_that_are_not_finite_are_seen(B, H, Sq, Sk, D, biased):
+    """A visible query, key or value that is not finite makes the rows that see it NaN, and
+    changes no other row."""
+    q, k, v, _ = inputs(B, H, H, Sq, Sk, D)
+    call = lambda q, k, v: relative_attention(q, k, v, table(32, H)) if biased else cross_attention(q, k, v)  # noqa: E731
+    clean = call(q, k, v)
+
+    def hit(o, rows):
+        assert torch.isnan(o[0, 0, rows]).all()
+        o = o.clone()
+        o[0, 0, rows] = clean[0, 0, rows]
+        assert torch.equal(o, clean)
+
+    for x in (math.nan, math.inf):
+        q2 = q.clone()
+        q2[0, 0, Sq - 1, 3] = x
+        hit(call(q2, k, v), slice(Sq - 1, Sq))
+    for key in [*range(18), Sk // 2, Sk - 1]:  # all places in a group of columns
+        k2 = k.clone()
+        k2[0, 0, key, 5] = math.nan
+        hit(call(q, k2, v), slice(None))
+    k2 = k.clone()
+    k2[0, 0, 17] = q[0, 0, 0].float().sign().to(torch.bfloat16) * math.inf  # a score of +inf in row 0
+    assert torch.isnan(call(q, k2, v)[0, 0, 0]).all()
+    v2 = v.clone()
+    v2[0, 0, Sk - 1] = math.nan
+    hit(call(q, k, v2), slice(None))
+
+
 # ---- gradients that are wanted, determinism, graphs ---------------------------------------
 
 @pytest.mark.parametrize("wanted", ["q", "k", "v", "b", "qk", "kb", "qb"])
