@@ -177,19 +177,31 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias, bool exact) 
     const long long items = static_cast<long long>(p->batch) * p->kv_heads * f.row_tiles;
     const long long units = std::max<long long>(1, ceil_div(p->k_len, small_d ? 128 : 64));  // tiles of an item, at most
     const long long slots = kSMs * (f.rg == 1 ? 2 : 1);
-    // Few items: clusters of up to 16 CTAs (8 with 32 rows, whose CTAs fill an SM: a GPU holds
-    // too few clusters of 16 SMs), as many as fit, at least two tiles for each CTA.  Many: equal
-    // shares, unless the items have one or two tiles or there are too many sequences to look
-    // through.  Between them the estimate of time decides: 0.7 us for a tile of a CTA, and 11
-    // us more for shares and their join (B2 H32 over 4 heads D128, 16384 keys: 20 us against
-    // 33; 24 rows on 65536 keys: 111 against 68).
+    // Clusters of up to 16 CTAs for each item, as many as fit at once, at least two tiles for
+    // each CTA (many items: one CTA each), or equal shares of all items' tiles and a join.
+    // The estimate of time decides: all tiles (32 KB) through HBM, or a CTA's tiles at 0.7 us
+    // (0.85 with 32 rows), and 12 us more for shares and their join.  Shares win where few
+    // items leave SMs without work, or sequences of different lengths do (B2 H32 over 4 heads,
+    // 3 tokens on 50001 keys, D128: 58 us against 89; B2 H32 over 4 heads, 1 token on 50001
+    // keys: 54 against 46; B64 H16, 1 token on 375 to 1500 keys, D64: 60 against 53).  With
+    // very many sequences shares would look through them for too long.
+    // A cluster lies inside one GPC, whose SMs it may not fill: `fit` holds how many clusters
+    // of 1, 2, .. 16 CTAs run at once (a B200 with 148 SMs says 296, 148, 71, 33, 14 with two
+    // CTAs to an SM and 148, 74, 33, 15, 7 with one; a little less here, as a GPU's SMs may lie
+    // in other GPCs).  One cluster too many costs a second wave (B1 H16, 1 token on 4000 keys,
+    // D64: 20 us with clusters of 16, 15 with clusters of 8).
+    constexpr int fit[2][5] = {{296, 148, 64, 32, 12}, {148, 74, 32, 14, 6}};
     f.cluster = 1;
-    const int most = f.rg == 1 ? 16 : 8;
-    while (f.cluster < most && items * f.cluster * 2 <= slots && units >= f.cluster * 4) f.cluster *= 2;
+    int at_once = fit[f.rg - 1][0];
+    for (int x = 1; x < 5 && items <= fit[f.rg - 1][x] && units >= f.cluster * 4; ++x) {
+      f.cluster *= 2;
+      at_once = fit[f.rg - 1][x];
+    }
     const long long share_ctas = std::max<long long>(1, std::min(slots, items * units / 2));
     const double mean = p->batch > 1 && p->key_lengths ? 0.67 : 1.0;
-    const double by_cluster = 0.7 * units / f.cluster * ceil_div(items * f.cluster, slots);
-    const double by_share = 0.7 * mean * items * units / share_ctas + 11.0;
+    const double tile_us = f.rg == 1 ? 0.7 : 0.85, hbm = 0.005 * mean * items * units;
+    const double by_cluster = std::max(tile_us * units / f.cluster * std::max(1.0, mean * items / at_once), hbm);
+    const double by_share = std::max(tile_us * mean * items * units / share_ctas, hbm) + 12.0;
     if (units > 2 && p->batch <= 1024 && by_share < by_cluster) f.cluster = 0;
     f.grid = static_cast<int>(f.cluster ? items * f.cluster : std::min(slots, items * units / 2));
     f.join = f.cluster == 0;

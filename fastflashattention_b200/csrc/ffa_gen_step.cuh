@@ -5,10 +5,10 @@
 // that share a key head (row r = g * Sq + t) form items of 16 MT rows, the M of mma.sync
 // m16n8k16; the tensor cores' rate does not matter here, and a 128-row tcgen05 tile would
 // be empty.  Two CTAs to an SM, each a TMA warp and four warps that compute:
-//   * few items: a cluster of CTAs shares the keys of each, and joins its results through
-//     distributed shared memory, in the same launch;
-//   * many items: all keys of all items, laid end to end, are cut into equal shares (Work), one
-//     for each CTA, whatever the lengths of the sequences are.  The TMA warp walks through its
+//   * a CTA takes an item, or, where items are few, a cluster of CTAs shares its keys, and
+//     joins its results through distributed shared memory, in the same launch;
+//   * few long sequences, or very different ones: all keys of all items, laid end to end, are
+//     cut into equal shares (Work), one for each CTA, whatever the lengths of the sequences are.  The TMA warp walks through its
 //     share without a stop: HBM sees no gaps between items.  An item that several CTAs share
 //     is joined by ffa_gen_step_join_kernel, launched beside the last CTAs (programmatic
 //     dependent launch), which it waits for;
