@@ -164,11 +164,6 @@ __device__ __forceinline__ void store_staged(bool staged, const CUtensorMap* con
 // ====================================================================================
 // dK / dV
 // ====================================================================================
-// Of every 4 groups of 4 exponentials, how many go to the FMA pipe instead of MUFU.EX2.  None
-// is best without a bias (B4 H16 S4096 D128: 1471 us against 1535), one with it (1816 us
-// against 1915, and 208 against 214 at B8 H12 S1024 D64).
-constexpr int bwd_emu(bool bias) { return bias ? 1 : 0; }
-
 // Shape of a CTA: two compute warpgroups, each with CW columns of a step (thread = TMEM lane
 // = row), then the control warps.  At D = 128 setmaxnreg moves registers from those to the
 // compute warpgroups (see ffa_bwd.cuh); at D = 64 all threads have the same.
@@ -232,7 +227,7 @@ struct DkdvLayout {
   static int smem_bytes(const Bias& bias) { return TAB_OFF + (TAB_SHARED ? table_size(bias) * 4 : 0); }
 };
 
-template <int D, bool CAUSAL, bool BIAS, int EMU = bwd_emu(BIAS)>
+template <int D, bool CAUSAL, bool BIAS>
 __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     ffa_gen_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
@@ -552,18 +547,11 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
             }
             const float2 xa = fma2(make_float2(p[e], p[e + 1]), cc, la);
             const float2 xb = fma2(make_float2(p[e + 2], p[e + 3]), cc, lb);
-            if ((e >> 2 & 3) < EMU) {  // this group of 4 on the FMA pipe
-              const float2 ea = exp2_fma2(xa), eb = exp2_fma2(xb);
-              p[e + 0] = ea.x;
-              p[e + 1] = ea.y;
-              p[e + 2] = eb.x;
-              p[e + 3] = eb.y;
-            } else {
-              p[e + 0] = fast_exp2(xa.x);
-              p[e + 1] = fast_exp2(xa.y);
-              p[e + 2] = fast_exp2(xb.x);
-              p[e + 3] = fast_exp2(xb.y);
-            }
+            // (a quarter on the FMA pipe, exp2_fma2, changes the time by less than 1 %)
+            p[e + 0] = fast_exp2(xa.x);
+            p[e + 1] = fast_exp2(xa.y);
+            p[e + 2] = fast_exp2(xb.x);
+            p[e + 3] = fast_exp2(xb.y);
           }
           if (masked) {  // apart from the loop, so that other steps branch around it
             const int first = q_first - min(qc, 1 << 30);  // column of the first query that sees the key
@@ -803,7 +791,7 @@ __device__ __forceinline__ void add_near_block(const float (&ds)[CW], int r0, co
   }
 }
 
-template <int D, bool CAUSAL, bool BIAS, int EMU = bwd_emu(BIAS)>
+template <int D, bool CAUSAL, bool BIAS>
 __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     ffa_gen_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ Problem pr,
@@ -1076,17 +1064,8 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
 #pragma unroll
       for (int e = 0; e < CW; e += 2) {
         const float2 x = fma2(make_float2(p[e], p[e + 1]), c2, l2);
-        float p0, p1;
-        if ((e >> 2 & 3) < EMU) {  // this pair on the FMA pipe
-          const float2 ex = exp2_fma2(x);
-          p0 = ex.x;
-          p1 = ex.y;
-        } else {
-          p0 = fast_exp2(x.x);
-          p1 = fast_exp2(x.y);
-        }
-        p[e] = p0;
-        p[e + 1] = p1;
+        p[e] = fast_exp2(x.x);
+        p[e + 1] = fast_exp2(x.y);
       }
       if (masked) {  // apart from the loop, so that other steps branch around it
         const int last = lim - kc;

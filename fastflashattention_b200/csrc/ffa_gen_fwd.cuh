@@ -14,7 +14,7 @@
 //   * the loop bodies are 64 scores long and the same for every kind of tile; a mask, a bias
 //     for each score or a negative scale is applied in tensor memory first (a rolled loop).
 //     A short launch spends much of its time fetching instructions that it runs for the first
-//     time (B8 H12 S1024 D64: 91 us with bodies of 128 scores for each kind, 58 so);
+//     time (B8 H12 S1024 D64 without a bias: 91 us with bodies of 128 scores for each kind, 59 so);
 //   * a tile whose relative positions all lie in the last bucket of a side has one bias: it
 //     joins the row max and the exponent's constant for free;
 //   * EXACT, for a training step that wants the bias's gradient: P goes to the product as two
