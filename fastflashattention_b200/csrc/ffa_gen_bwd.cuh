@@ -323,6 +323,9 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // LSE and delta are written.  Each warp waits for that itself before its first wait that
+  // depends on them: the time limit of a wait on a barrier is for this kernel's own work.
+  auto wait_stats = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   if (warp >= 8) {
     if constexpr (D == 128) setmaxnreg_dec<bwd::REGS_CONTROL>();
     const uint64_t keep = policy_evict_last();
@@ -347,7 +350,6 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
       bulk_load(do_addr(it) + L::TILE + STEP * 4, DELTA + r, STEP * 4, do_full(s));
       return true;
     };
-    auto wait_stats = [&]() { asm volatile("griddepcontrol.wait;" ::: "memory"); };  // LSE and delta are written
     if (warp == W::PRODUCER) {
       // -------------------------------------------------------------- producer: K, V, Q ring
       if (lane == 0) {
@@ -361,6 +363,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
         }
         bool ok = true;
         for (int it = 0; it < ns && ok; ++it) {
+          if (W::DO_PRODUCER >= 0 && it == QS) wait_stats();
           if ((ok = load_q(it))) ++n_q;
           if (W::DO_PRODUCER < 0 && ok) {
             if (it == 0) wait_stats();
@@ -451,7 +454,9 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
           zero_tail(sbase + L::K_OFF, SLABS, n_keys - n0, lane);
           zero_tail(sbase + L::V_OFF, SLABS, n_keys - n0, lane);
         }
-        ok = ok && issue_s(0) && issue_dp(0);
+        ok = ok && issue_s(0);
+        wait_stats();
+        ok = ok && issue_dp(0);
       }
       // S(i+1) as soon as the warpgroups have copied S(i) into registers, then dV(i), dK(i)
       // and dP(i+1): P(i) and dS(i) live in the dP columns.
@@ -488,13 +493,13 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     const float2 c2 = make_float2(pr.scale_log2, pr.scale_log2);
     bool ok = true;
     int i = 0;
+    wait_stats();  // and the bias tables
     // heads of the group; all compute threads pass the barriers of every head
     for (int hg = ns > 0 ? st0 / nqb : 0; i < ns || !ok; ++hg) {
       if (!ok && hg * nqb >= st0 + ns) break;
       float bias_l = 0.f, bias_r = 0.f;
       const float* tab = nullptr;  // the head's table
       if (BIAS) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // the tables are written
         if constexpr (L::TAB_SHARED) {
           float* room = reinterpret_cast<float*>(smem + L::TAB_OFF);
           ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table

@@ -4,6 +4,7 @@ Every value of every output is held to the bound that the oracle derives from th
 roundings (oracle/general_oracle.py), and every output to the package's gate of 5e-3
 relative L2 (typical errors are far below the bound, which adds up worst cases).
 """
+import ctypes
 import math
 import threading
 
@@ -121,6 +122,50 @@ def test_few_rows_shares(B, Hkv, Sk, D):
     check(q, k, v, None, train=False)
     lens = torch.randint(0, Sk + 1, (B,), device="cuda", generator=gen, dtype=torch.int32)
     check(q, k, v, None, train=False, key_lengths=lens)
+
+
+def step_lengths(B, Sk):
+    """Lengths of a padded batch: the longest, none, one, and others between."""
+    return torch.tensor([(Sk, 0, 1, Sk // 3, Sk - 5, Sk // 2)[b % 6] for b in range(B)], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("items", [12, 13, 32, 33, 64, 65, 148, 149, 296, 297])
+@pytest.mark.parametrize("rows, D", [(1, 64), (9, 128)])
+def test_clusters_of_ctas(items, rows, D):
+    """As many items as clusters of 16, 8, 4, 2 and 1 CTAs fit at once, and one more."""
+    Sk = 4200 if D == 64 else 2100
+    q, k, v, _ = inputs(1, items, items, rows, Sk, D)
+    check(q, k, v, None, train=False)
+    q, k, v, _ = inputs(items, 1, 1, rows, Sk, D)
+    check(q, k, v, None, train=False, key_lengths=step_lengths(items, Sk))
+
+
+@pytest.mark.parametrize("items", [6, 14, 15, 32, 33, 74, 75, 148, 149])
+@pytest.mark.parametrize("D", [64, 128])
+def test_clusters_of_ctas_with_32_rows(items, D):
+    q, k, v, _ = inputs(1, 4 * items, items, 6, 1500, D)
+    check(q, k, v, None, train=False)
+    check(q, k, v, None, table(32, 4 * items), train=False, is_causal=True, query_offset=1400)
+
+
+@pytest.mark.parametrize("B, Hkv, G, Sq, Sk, D, ragged, shares", [
+    (2, 4, 8, 3, 20000, 128, False, True), (4, 4, 4, 8, 20000, 64, True, True),  # 32 rows
+    (10, 10, 3, 7, 2560, 128, False, False), (10, 10, 3, 7, 6000, 128, False, True),
+    (1, 13, 1, 1, 50000, 128, False, True), (1, 13, 9, 1, 100000, 64, False, True),  # 16 rows
+    (11, 3, 1, 1, 20000, 128, True, True),
+])
+def test_shares(B, Hkv, G, Sq, Sk, D, ragged, shares):
+    """Equal shares of all keys, whose parts a second kernel joins (one shape that the estimate
+    of time gives to single CTAs, 35.0 against 34.0)."""
+    q, k, v, _ = inputs(B, G * Hkv, Hkv, Sq, Sk, D)
+    lens = step_lengths(B, Sk) if ragged else None
+    p = _lib.GenProblem(batch=B, q_heads=G * Hkv, kv_heads=Hkv, q_len=Sq, k_len=Sk, head_dim=D, scale=1.0)
+    if ragged:
+        p.key_lengths = lens.data_ptr()
+    assert (_lib.load().ffa_gen_fwd_workspace(ctypes.byref(p), 0) > 0) == shares  # room for the parts
+    check(q, k, v, None, train=False, key_lengths=lens)
+    where = {"key_lengths": lens, "query_offset": lens - Sq} if ragged else {"query_offset": Sk - Sq}
+    check(q, k, v, None, table(32, G * Hkv), train=False, is_causal=True, **where)
 
 
 @pytest.mark.parametrize("Sq, Sk, D", [(100, 4000, 64), (100, 4000, 128), (4000, 100, 64), (4000, 100, 128)])
