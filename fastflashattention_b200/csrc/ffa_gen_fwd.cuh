@@ -3,18 +3,22 @@
 //   O_i = sum_j softmax_j(S_ij) v_j,   LSE_i = base-2 log-sum-exp of S_i (-inf: no key)
 //
 // The plan of the plain forward (ffa_fwd.cuh): a softmax warpgroup for each 128-row query
-// tile (thread = row), a TMA warp and an MMA warp; S and O in tensor memory, P handed back
+// tile (thread = row), and warps that load and issue MMAs; S and O in tensor memory, P handed back
 // through it over S; the running max is rescaled lazily.  What differs:
 //   * operands are 4-D tensor maps, so any strides of batch, head and row do, and the key
 //     head of a query head is found by division;
 //   * head dims up to 64: the softmax bounds the kernel, and one warp of a scheduler waits
 //     for its own loads and MMAs most of the time.  So a CTA has one tile and walks 64 keys
-//     a step: 128 columns of tensor memory and 80 registers a thread, four CTAs to an SM;
+//     a step, 128 columns of tensor memory, four CTAs to an SM.  One warp loads and issues
+//     MMAs, whose commits free the slots that it loads: with five warps a thread has 96
+//     registers, with six 80 and spills (B8 H16 S4096: 749 us with six, 684 so; with a bias 857
+//     and 732);
 //   * head dims up to 128: two tiles and 128 keys a step, one CTA to an SM;
 //   * the loop bodies are 64 scores long and the same for every kind of tile; a mask, a bias
-//     for each score or a negative scale is applied in tensor memory first (a rolled loop).
-//     A short launch spends much of its time fetching instructions that it runs for the first
-//     time (B8 H12 S1024 D64 without a bias: 91 us with bodies of 128 scores for each kind, 59 so);
+//     for each score or a negative scale is applied first, in registers where a step has 64
+//     keys, else in tensor memory (a rolled loop).  A short launch spends much of its time
+//     fetching instructions that it runs for the first time (B8 H12 S1024 D64 without a bias:
+//     91 us with bodies of 128 scores for each kind, 59 with these);
 //   * a tile whose relative positions all lie in the last bucket of a side has one bias: it
 //     joins the row max and the exponent's constant for free;
 //   * EXACT, for a training step that wants the bias's gradient: P goes to the product as two
@@ -37,13 +41,13 @@ template <int D>
 struct FwdLayout {
   static constexpr int NT = D == 64 ? 1 : 2;        // 128-row tiles (softmax warpgroups) of a CTA
   // CTAs of an SM.  EXACT holds 32 registers more: three CTAs without spills beat four (B8 H16
-  // S4096 D64: 1107 us against 1406)
+  // S4096 D64: 998 us against 1047)
   static constexpr int ctas(bool exact) { return D == 64 ? (exact ? 3 : 4) : 1; }
   static constexpr int KEYS = D == 64 ? 64 : 128;   // keys of a step
   static constexpr int HALVES = KEYS / 64;          // P is handed over 64 keys at a time
   static constexpr int ROWS = 128 * NT;
   // D = 128 moves registers between warpgroups (setmaxnreg), so the control warps fill one up
-  static constexpr int THREADS = D == 64 ? 192 : 384;
+  static constexpr int THREADS = D == 64 ? 160 : 384;
   static constexpr int TMEM = D == 64 ? 128 : 512;  // S [0, KEYS) of each tile, then O
   static constexpr uint32_t O_COL = KEYS * NT;
   static constexpr int Q_TILE = 128 * D * 2, TILE = KEYS * D * 2;
@@ -78,7 +82,10 @@ __device__ __forceinline__ float row_max64(const uint32_t (&a)[32], const uint32
   return max3_nan(max3_nan(y0, y1, y2), max3_nan(y3, y4, x[15]), y0);
 }
 
-template <int D, bool CAUSAL, bool BIAS, bool EXACT, int EMU = D == 64 ? 2 : 0>
+// EMU of every 8 column pairs take their exponentials on the FMA pipe.  At D = 64 one is best
+// with a bias (B8 H16 S4096: 740 us, 767 with two, 777 with none) and as good as two without;
+// at D = 128 it changes nothing.
+template <int D, bool CAUSAL, bool BIAS, bool EXACT, int EMU = D == 64 ? 1 : 0>
 __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXACT))
     ffa_gen_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -87,7 +94,9 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
                        float* __restrict__ part_lse, int n_split, int per_split, int group) {
   using L = FwdLayout<D>;
   constexpr int SLABS = D / 64, STAGES = L::STAGES, NT = L::NT, KEYS = L::KEYS;
-  constexpr int PRODUCER = 4 * NT, MMA = 4 * NT + 1;  // warps
+  constexpr int HALVES = L::HALVES;
+  constexpr bool ONE = NT == 1;  // one warp loads and issues MMAs
+  constexpr int PRODUCER = 4 * NT, MMA = ONE ? PRODUCER : PRODUCER + 1;  // warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -162,39 +171,61 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
 
   if (warp >= 4 * NT) {
     if constexpr (D == 128) setmaxnreg_dec<fwd::REGS_CONTROL>();
-    if (warp == PRODUCER) {
+    const uint64_t keep = policy_evict_last();
+    auto load_q = [&]() {
+      mbar_arrive_expect_tx(q_full, NT * L::Q_TILE);
+      for (int i = 0; i < NT; ++i)
+        for (int sl = 0; sl < SLABS; ++sl)
+          tma_load_4d(sbase + L::Q_OFF + i * L::Q_TILE + sl * 16384, &tm_q, q_full, sl * 64, m0 + i * 128, h, b, keep);
+    };
+    auto load_kv = [&](int n) {  // K_0, V_0, K_1, V_1, ..
+      mbar_arrive_expect_tx(kv_full(n), L::TILE);
+      for (int sl = 0; sl < SLABS; ++sl)
+        tma_load_4d(sbase + L::KV_OFF + (n % STAGES) * L::TILE + sl * (KEYS * 128), (n & 1) ? &tm_v : &tm_k, kv_full(n),
+                    sl * 64, (t0 + (n >> 1)) * KEYS, hk, b, keep);
+    };
+    auto slot_free = [&](int n) {
+      return mbar_wait(kv_empty(n), ((n / STAGES) & 1) ^ 1, abort_flag, kErrGenFwdProducer);
+    };
+    // the table, once its kernel has written it (this one may start before that ends)
+    auto load_table = [&]() {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      const int bytes = table_size(bias) * 4;
+      mbar_arrive_expect_tx(tab_full, bytes);
+      bulk_load(smem_u32(tab), tables + static_cast<long long>(h) * table_size(bias), bytes, tab_full);
+    };
+    // let the copies in flight, of the first n tiles, land before the CTA's shared memory goes away
+    auto drain_loads = [&](int n) {
+      if (!*abort_flag) return;
+      for (int x = max(0, n - STAGES); x < n; ++x) mbar_wait_drain(kv_full(x), (x / STAGES) & 1);
+      mbar_wait_drain(q_full, 0);
+      if (BIAS && n > 0) mbar_wait_drain(tab_full, 0);
+    };
+    // without tiles nobody waits for the tables: the launch ends after theirs all the same
+    if (BIAS && warp == PRODUCER && n_kv == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!ONE && warp == PRODUCER) {
       // ---------------------------------------------------------------- producer
-      if (BIAS && n_kv == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // as below: the launch ends after the tables'
       if (lane == 0 && n_kv > 0) {
-        const uint64_t keep = policy_evict_last();
-        mbar_arrive_expect_tx(q_full, NT * L::Q_TILE);
-        for (int i = 0; i < NT; ++i)
-          for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(sbase + L::Q_OFF + i * L::Q_TILE + sl * 16384, &tm_q, q_full, sl * 64, m0 + i * 128, h, b, keep);
+        load_q();
         int n = 0;
-        for (; n < 2 * n_kv; ++n) {
-          if (!mbar_wait(kv_empty(n), ((n / STAGES) & 1) ^ 1, abort_flag, kErrGenFwdProducer)) break;
-          mbar_arrive_expect_tx(kv_full(n), L::TILE);
-          for (int sl = 0; sl < SLABS; ++sl)
-            tma_load_4d(sbase + L::KV_OFF + (n % STAGES) * L::TILE + sl * (KEYS * 128), (n & 1) ? &tm_v : &tm_k,
-                        kv_full(n), sl * 64, (t0 + (n >> 1)) * KEYS, hk, b, keep);
-          if (BIAS && n == 0) {
-            // the table, once its kernel has written it (this one may start before that ends)
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            const int bytes = table_size(bias) * 4;
-            mbar_arrive_expect_tx(tab_full, bytes);
-            bulk_load(smem_u32(tab), tables + static_cast<long long>(h) * table_size(bias), bytes, tab_full);
-          }
+        for (; n < 2 * n_kv && slot_free(n); ++n) {
+          load_kv(n);
+          if (BIAS && n == 0) load_table();
         }
-        if (*abort_flag) {
-          // let in-flight copies land before the CTA's shared memory goes away
-          for (int x = max(0, n - STAGES); x < n; ++x) mbar_wait_drain(kv_full(x), (x / STAGES) & 1);
-          mbar_wait_drain(q_full, 0);
-          if (BIAS && n > 0) mbar_wait_drain(tab_full, 0);
-        }
+        drain_loads(n);
       }
     } else if (warp == MMA) {
       // ---------------------------------------------------------------- MMA issuer
+      int loaded = 0;  // tiles (ONE)
+      if (ONE && n_kv > 0) {
+        loaded = min(STAGES, 2 * n_kv);
+        if (lane == 0) {
+          load_q();
+          for (int n = 0; n < loaded; ++n) load_kv(n);
+          if (BIAS) load_table();
+        }
+        __syncwarp();
+      }
       constexpr uint32_t IDESC_QK = idesc_bf16(128, KEYS, false, false);
       constexpr uint32_t IDESC_PV = idesc_bf16(128, D, false, true);
       bool ok = n_kv > 0 && mbar_wait(q_full, 0, abort_flag, kErrGenFwdMma);
@@ -225,7 +256,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
         const uint64_t vd = mnmajor_desc(kv_addr(n), KEYS, 0);
         const uint32_t d = tmem + L::O_COL + i * 128, a = tmem + i * KEYS;
 #pragma unroll 1
-        for (int half = 0; half < L::HALVES; ++half) {
+        for (int half = 0; half < HALVES; ++half) {
           if (!mbar_wait(p_ready(i, half), j & 1, abort_flag, kErrGenFwdMma)) return false;
           tc_fence_after();
           if (elect_one()) {
@@ -246,6 +277,15 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       }
       for (int j = 0; j < n_kv && ok; ++j) {
         const int nv = 2 * j + 1, nk = 2 * j + 2;  // V_j and K_{j+1}
+        if (ONE) {
+          // S_j is there: the slots of V_{j-1} and K_j are free, or will be at once
+          for (; loaded <= nk + 2 && loaded < 2 * n_kv; ++loaded) {
+            if (!(ok = slot_free(loaded))) break;
+            if (lane == 0) load_kv(loaded);
+          }
+          __syncwarp();
+          if (!ok) break;
+        }
         if (!(ok = kv_wait(nv))) break;
         const int tail = n_keys - (t0 + j) * KEYS;
         if (tail < KEYS && n_keys < pr.Sk) zero_tail<KEYS>(kv_addr(nv), SLABS, tail, lane);
@@ -269,6 +309,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       // every issued MMA has finished before TMEM is released
       commit(drain_bar);
       mbar_wait_drain(drain_bar, 0);
+      if (ONE && n_kv > 0) drain_loads(loaded);
     }
   } else {
     if constexpr (D == 128) setmaxnreg_inc<fwd::REGS_SOFTMAX>();
@@ -302,42 +343,54 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
         near = r_min < bias.right && r_max > -bias.left;
         fb = tab[r_min >= bias.right ? table_last(bias) : 0];
       }
-      // With a bias for each score or a scale that does not keep the order, the scores in
-      // tensor memory become scaled scores; masked ones become -inf.
+      // With a bias for each score or a scale that does not keep the order, the scores become
+      // scaled scores; masked ones become -inf.  In registers, where a step's scores fit, else
+      // in tensor memory.
       const bool scaled = near || scale_log2 <= 0.f;
       const float c = scaled ? 1.f : scale_log2;  // what the scores still have to be multiplied with
-      if (scaled || masked) {
-#pragma unroll 1
-        for (int x = 0; x < KEYS; x += 32) {
-          uint32_t r[32];
-          tmem_ld32(t_s + x, r);
-          tmem_ld_wait();
-          if (scaled) {
-            const float* tp = tab + (n0 + x - off - grow + bias.left + kPad);
+      const int last = lim - n0;  // last column that this row sees
+      const float* tp = tab + (n0 - off - grow + bias.left + kPad);
+      auto adjust = [&](uint32_t (&r)[32], int x) {  // columns x .. x + 31
+        if (scaled) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), scale_log2, BIAS && near ? tp[e] : fb));
-          }
-          if (masked) {
-            const int last = lim - n0 - x;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (e > last) r[e] = 0xff800000u;
-          }
-          tmem_st32(t_s + x, r);
+          for (int e = 0; e < 32; ++e)
+            r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), scale_log2, BIAS && near ? tp[x + e] : fb));
         }
-        tmem_st_wait();
-      }
-      if (scaled) fb = 0.f;
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (x + e > last) r[e] = 0xff800000u;
+        }
+      };
       uint32_t sa[32], sb[32];  // 64 scores
       float tmax = -INFINITY;
-#pragma unroll 1
-      for (int hf = L::HALVES - 1; hf >= 0; --hf) {
-        tmem_ld32(t_s + 64 * hf, sa);
-        tmem_ld32(t_s + 64 * hf + 32, sb);
+      if constexpr (HALVES == 1) {
+        tmem_ld32(t_s, sa);
+        tmem_ld32(t_s + 32, sb);
         tmem_ld_wait();
-        tmax = max3_nan(tmax, tmax, row_max64(sa, sb));
+        adjust(sa, 0);
+        adjust(sb, 32);
+        tmax = row_max64(sa, sb);
+      } else {
+        if (scaled || masked) {
+#pragma unroll 1
+          for (int x = 0; x < KEYS; x += 32) {
+            tmem_ld32(t_s + x, sa);
+            tmem_ld_wait();
+            adjust(sa, x);
+            tmem_st32(t_s + x, sa);
+          }
+          tmem_st_wait();
+        }
+#pragma unroll 1
+        for (int hf = HALVES - 1; hf >= 0; --hf) {
+          tmem_ld32(t_s + 64 * hf, sa);
+          tmem_ld32(t_s + 64 * hf + 32, sb);
+          tmem_ld_wait();
+          tmax = max3_nan(tmax, tmax, row_max64(sa, sb));
+        }
       }
+      if (scaled) fb = 0.f;
       tmax = BIAS ? fmaf(tmax, c, fb) : tmax * c;
       // a visible score that is NaN or +inf makes the row NaN (exp2_fma2 would lose it)
       if (!(tmax < INFINITY)) l = __int_as_float(0x7fffffff);
@@ -367,7 +420,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       // 64 scores -> P -> 32 columns over these scores, and 32 of remainders behind them (the
       // first half's scores are still in registers)
 #pragma unroll 1
-      for (int hf = 0; hf < L::HALVES; ++hf) {
+      for (int hf = 0; hf < HALVES; ++hf) {
         if (hf > 0) {
           tmem_ld32(t_s + 64 * hf, sa);
           tmem_ld32(t_s + 64 * hf + 32, sb);
