@@ -15,8 +15,8 @@
 //     and 732);
 //   * head dims up to 128: two tiles and 128 keys a step, one CTA to an SM;
 //   * the loop bodies are 64 scores long and the same for every kind of tile; a mask, a bias
-//     for each score or a negative scale is applied first, in registers where a step has 64
-//     keys, else in tensor memory (a rolled loop).  A short launch spends much of its time
+//     for each score or a negative scale is applied where the scores come into registers for
+//     their maximum.  A short launch spends much of its time
 //     fetching instructions that it runs for the first time (B8 H12 S1024 D64 without a bias:
 //     91 us with bodies of 128 scores for each kind, 59 with these);
 //   * a tile whose relative positions all lie in the last bucket of a side has one bias: it
@@ -344,51 +344,58 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
         fb = tab[r_min >= bias.right ? table_last(bias) : 0];
       }
       // With a bias for each score or a scale that does not keep the order, the scores become
-      // scaled scores; masked ones become -inf.  In registers, where a step's scores fit, else
-      // in tensor memory.
+      // scaled scores; masked ones become -inf.  Those that do not stay in registers (the second
+      // half of 128) go back to tensor memory.  Without a bias this is rare, and at D = 128 a
+      // loop apart keeps the others' shorter (B2 H16 S4096 D128: 273 us against 283).
       const bool scaled = near || scale_log2 <= 0.f;
       const float c = scaled ? 1.f : scale_log2;  // what the scores still have to be multiplied with
-      const int last = lim - n0;  // last column that this row sees
-      const float* tp = tab + (n0 - off - grow + bias.left + kPad);
-      auto adjust = [&](uint32_t (&r)[32], int x) {  // columns x .. x + 31
+      uint32_t sa[32], sb[32];  // 64 scores
+      auto adjust = [&](int x) {  // columns x .. x + 63 of the step
         if (scaled) {
+          const float* tp = tab + (n0 + x - off - grow + bias.left + kPad);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), scale_log2, BIAS && near ? tp[x + e] : fb));
+          for (int e = 0; e < 32; ++e) {
+            sa[e] = __float_as_uint(fmaf(__uint_as_float(sa[e]), scale_log2, BIAS && near ? tp[e] : fb));
+            sb[e] = __float_as_uint(fmaf(__uint_as_float(sb[e]), scale_log2, BIAS && near ? tp[32 + e] : fb));
+          }
         }
         if (masked) {
+          const int last = lim - n0 - x;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (x + e > last) r[e] = 0xff800000u;
+          for (int e = 0; e < 32; ++e) {
+            if (e > last) sa[e] = 0xff800000u;
+            if (32 + e > last) sb[e] = 0xff800000u;
+          }
         }
       };
-      uint32_t sa[32], sb[32];  // 64 scores
-      float tmax = -INFINITY;
-      if constexpr (HALVES == 1) {
-        tmem_ld32(t_s, sa);
-        tmem_ld32(t_s + 32, sb);
+      auto load = [&](int hf) {
+        tmem_ld32(t_s + 64 * hf, sa);
+        tmem_ld32(t_s + 64 * hf + 32, sb);
         tmem_ld_wait();
-        adjust(sa, 0);
-        adjust(sb, 32);
-        tmax = row_max64(sa, sb);
-      } else {
-        if (scaled || masked) {
+      };
+      auto store = [&](int hf) {
+        tmem_st32(t_s + 64 * hf, sa);
+        tmem_st32(t_s + 64 * hf + 32, sb);
+        tmem_st_wait();
+      };
+      constexpr bool APART = HALVES > 1 && !BIAS;
+      if (APART && (scaled || masked)) {
 #pragma unroll 1
-          for (int x = 0; x < KEYS; x += 32) {
-            tmem_ld32(t_s + x, sa);
-            tmem_ld_wait();
-            adjust(sa, x);
-            tmem_st32(t_s + x, sa);
-          }
-          tmem_st_wait();
+        for (int hf = 0; hf < HALVES; ++hf) {
+          load(hf);
+          adjust(64 * hf);
+          store(hf);
         }
+      }
+      float tmax = -INFINITY;
 #pragma unroll 1
-        for (int hf = HALVES - 1; hf >= 0; --hf) {
-          tmem_ld32(t_s + 64 * hf, sa);
-          tmem_ld32(t_s + 64 * hf + 32, sb);
-          tmem_ld_wait();
-          tmax = max3_nan(tmax, tmax, row_max64(sa, sb));
+      for (int hf = HALVES - 1; hf >= 0; --hf) {
+        load(hf);
+        if (!APART) {
+          adjust(64 * hf);
+          if (hf > 0 && (scaled || masked)) store(hf);
         }
+        tmax = max3_nan(tmax, tmax, row_max64(sa, sb));
       }
       if (scaled) fb = 0.f;
       tmax = BIAS ? fmaf(tmax, c, fb) : tmax * c;
@@ -421,11 +428,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       // first half's scores are still in registers)
 #pragma unroll 1
       for (int hf = 0; hf < HALVES; ++hf) {
-        if (hf > 0) {
-          tmem_ld32(t_s + 64 * hf, sa);
-          tmem_ld32(t_s + 64 * hf + 32, sb);
-          tmem_ld_wait();
-        }
+        if (hf > 0) load(hf);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t hi[32], lo[EXACT ? 32 : 1];
 #pragma unroll
