@@ -631,11 +631,12 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
           c.o, c.dout, lse, ws, ws + w.stat_floats, p->q_heads, p->q_len, p->head_dim);
     if ((rc = launched())) return rc;
   }
-  auto sum = [&](const float* part, const View& out, int n_split, int H, int S) {
+  // `n` (one or two) gradients of the same shape from their splits, behind the kernel that wrote them
+  auto sum = [&](int n, const float* part0, const View& out0, const float* part1, const View& out1, int n_split, int H,
+                 int S) {
     const long long chunks = static_cast<long long>(p->batch) * H * S * (p->head_dim / 8);
-    ffa_gen_sum_kernel<<<static_cast<unsigned>(ceil_div(chunks, 256)), 256, 0, c.stream>>>(
-        part, out, n_split, p->batch, H, S, p->head_dim);
-    return launched();
+    return launch_early(ffa_gen_sum_kernel, dim3(static_cast<unsigned>(ceil_div(chunks, 256)), n), 256, 0, c.stream, part0,
+                        part1, out0, out1, n_split, p->batch, H, S, p->head_dim);
   };
   if (want_dq && queries) {
     c.dq = view(dq);
@@ -646,12 +647,12 @@ int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen
     c.dk = view(dk);
     c.dv = view(dv);
     if ((rc = dispatch<RunDkdv>(c, p->causal, w, ws))) return rc;
-    if (w.dkdv_split > 1 && ((rc = sum(ws + w.dk_off, c.dk, w.dkdv_split, p->kv_heads, p->k_len)) ||
-                             (rc = sum(ws + w.dv_off, c.dv, w.dkdv_split, p->kv_heads, p->k_len))))
+    if (w.dkdv_split > 1 &&
+        (rc = sum(2, ws + w.dk_off, c.dk, ws + w.dv_off, c.dv, w.dkdv_split, p->kv_heads, p->k_len)))
       return rc;
   }
   if (want_dq && queries && w.dq_split > 1 &&
-      (rc = sum(ws + w.dq_off, c.dq, w.dq_split, p->q_heads, p->q_len)))
+      (rc = sum(1, ws + w.dq_off, c.dq, ws + w.dq_off, c.dq, w.dq_split, p->q_heads, p->q_len)))
     return rc;
   if (dbias && p->q_heads > 0) {
     const int blocks = queries ? static_cast<int>(ceil_div(p->q_len, 128)) * w.dq_split : 0;

@@ -73,9 +73,14 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Sum of the splits' fp32 gradients [n_split][B][H][S][D] into a bf16 view; 8 columns a thread.
-__global__ void __launch_bounds__(256) ffa_gen_sum_kernel(const float* __restrict__ part, const View out, int n_split,
-                                                          int B, int H, int S, int D) {
+// Sum of the splits' fp32 gradients [n_split][B][H][S][D] into a bf16 view; 8 columns a
+// thread.  blockIdx.y: the first or the second pair of parts and view (dK and dV).
+__global__ void __launch_bounds__(256)
+    ffa_gen_sum_kernel(const float* __restrict__ part0, const float* __restrict__ part1, const View out0,
+                       const View out1, int n_split, int B, int H, int S, int D) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits have written
+  const float* part = blockIdx.y == 0 ? part0 : part1;
+  const View out = blockIdx.y == 0 ? out0 : out1;
   const long long chunks = static_cast<long long>(B) * H * S * (D / 8);
   const long long c = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (c >= chunks) return;

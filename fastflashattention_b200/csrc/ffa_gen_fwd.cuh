@@ -51,7 +51,7 @@ struct FwdLayout {
   static constexpr int TMEM = D == 64 ? 128 : 512;  // S [0, KEYS) of each tile, then O
   static constexpr uint32_t O_COL = KEYS * NT;
   static constexpr int Q_TILE = 128 * D * 2, TILE = KEYS * D * 2;
-  static constexpr int STAGES = D == 64 ? 4 : 4;
+  static constexpr int STAGES = 4;
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = NT * Q_TILE;
   // q_full, kv_full[], kv_empty[], tab_full; for each tile s_full, o_final, p_ready[2]; drain
