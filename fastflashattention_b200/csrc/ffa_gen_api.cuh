@@ -311,7 +311,9 @@ struct Call {
 };
 
 // A launch that may start before the kernel in front of it ends (it waits itself, where it
-// needs that kernel's results), so that its launch costs nothing.
+// needs that kernel's results), so that its launch costs nothing.  What the kernel in front
+// writes is not constant while this one runs: its pointers are not `const __restrict__`, which
+// would let the compiler take the loads for constant ones and move them above the wait.
 template <typename... P, typename... A>
 static int launch_early(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, A... args) {
   cudaLaunchAttribute attr{};

@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(256)
 // Sum of the splits' fp32 gradients [n_split][B][H][S][D] into a bf16 view; 8 columns a
 // thread.  blockIdx.y: the first or the second pair of parts and view (dK and dV).
 __global__ void __launch_bounds__(256)
-    ffa_gen_sum_kernel(const float* __restrict__ part0, const float* __restrict__ part1, const View out0,
-                       const View out1, int n_split, int B, int H, int S, int D) {
+    ffa_gen_sum_kernel(const float* part0, const float* part1, const View out0, const View out1, int n_split, int B,
+                       int H, int S, int D) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits have written
   const float* part = blockIdx.y == 0 ? part0 : part1;
   const View out = blockIdx.y == 0 ? out0 : out1;
@@ -238,8 +238,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
                         const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                         const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                         const __grid_constant__ Problem pr, const __grid_constant__ Bias bias,
-                        const float* __restrict__ tables, const float* __restrict__ LSE,
-                        const float* __restrict__ DELTA, float* __restrict__ dk_part,
+                        const float* tables, const float* LSE, const float* DELTA, float* __restrict__ dk_part,
                         float* __restrict__ dv_part, int n_split, int group) {
   using L = DkdvLayout<D, BIAS>;
   using W = BwdShape<D>;
@@ -805,10 +804,9 @@ template <int D, bool CAUSAL, bool BIAS>
 __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
     ffa_gen_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ Problem pr,
-                      const __grid_constant__ Bias bias, const float* __restrict__ tables,
-                      const unsigned short* __restrict__ lut_g, const View q, const View o, const View o_lo, const View dout,
-                      const float* __restrict__ LSE, float* __restrict__ lse_out, float* __restrict__ delta_out,
-                      float* __restrict__ dq_part, float* __restrict__ bias_part,
+                      const __grid_constant__ Bias bias, const float* tables, const unsigned short* lut_g, const View q,
+                      const View o, const View o_lo, const View dout, const float* LSE, float* __restrict__ lse_out,
+                      float* __restrict__ delta_out, float* __restrict__ dq_part, float* __restrict__ bias_part,
                       int n_split, int group) {
   using L = DqLayout<D, BIAS>;
   using W = BwdShape<D>;

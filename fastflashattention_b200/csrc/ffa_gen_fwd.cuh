@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
     ffa_gen_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                        const __grid_constant__ CUtensorMap tm_lo, const __grid_constant__ Problem pr, const __grid_constant__ Bias bias,
-                       const float* __restrict__ tables, float* __restrict__ LSE, float* __restrict__ part,
+                       const float* tables, float* __restrict__ LSE, float* __restrict__ part,
                        float* __restrict__ part_lse, int n_split, int per_split, int group) {
   using L = FwdLayout<D>;
   constexpr int SLABS = D / 64, STAGES = L::STAGES, NT = L::NT, KEYS = L::KEYS;
@@ -534,9 +534,8 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
 // keys fill; a split whose keys the row does not see (LSE = -inf) weighs nothing.
 template <int LANES>
 __global__ void __launch_bounds__(256)
-    ffa_gen_join_kernel(const __grid_constant__ Problem pr, const float* __restrict__ part,
-                        const float* __restrict__ part_lse, const View o, const View o_lo, float* __restrict__ LSE,
-                        int keys_per_split, int causal) {
+    ffa_gen_join_kernel(const __grid_constant__ Problem pr, const float* part, const float* part_lse, const View o,
+                        const View o_lo, float* __restrict__ LSE, int keys_per_split, int causal) {
   const long long rows = static_cast<long long>(pr.B) * pr.Hq * pr.Sq;
   const long long r = static_cast<long long>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
   const int c = threadIdx.x % LANES * 4;

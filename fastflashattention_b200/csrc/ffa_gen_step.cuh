@@ -590,9 +590,8 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
 // row, four columns a lane.  A part whose keys the row does not see (LSE = -inf) is not read,
 // nor is the slot of a CTA that has none.
 __global__ void __launch_bounds__(128)
-    ffa_gen_step_join_kernel(const __grid_constant__ Problem pr, const float* __restrict__ part,
-                             const float* __restrict__ part_lse, const JoinEntry* __restrict__ entries, const View o,
-                             float* __restrict__ LSE, int row_tiles, int rows) {
+    ffa_gen_step_join_kernel(const __grid_constant__ Problem pr, const float* part, const float* part_lse,
+                             const JoinEntry* entries, const View o, float* __restrict__ LSE, int row_tiles, int rows) {
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * 4 + (threadIdx.x >> 5);  // of the item
   asm volatile("griddepcontrol.wait;" ::: "memory");    // the parts are written
