@@ -131,6 +131,7 @@ template <int D>
 __device__ __forceinline__ void give_acc(uint32_t t_acc, int g, uint32_t tile, int row, float* part, int true_d,
                                          bool done, int rows, bool empty, float mul) {
   if (!done) return;
+  __syncwarp();  // tensor memory is loaded by whole warps
 #pragma unroll 1
   for (int c = g * (D / 2); c < (g + 1) * (D / 2); c += 32) {
     uint32_t r[32];
@@ -154,7 +155,7 @@ template <int D, int NT>
 __device__ __forceinline__ void store_staged(bool staged, const CUtensorMap* const (&maps)[NT], uint32_t first_tile,
                                              int row0, int h, int b) {
   fence_proxy_async_smem();
-  const bool all = named_barrier_and(1, 256, staged);
+  const bool all = whole_barrier_and(1, 256, staged);
   if (all && threadIdx.x == 0) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -506,9 +507,9 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
       if (BIAS) {
         if constexpr (L::TAB_SHARED) {
           float* room = reinterpret_cast<float*>(smem + L::TAB_OFF);
-          ok = named_barrier_and(2, 256, ok);  // everyone is done with the last head's table
+          ok = whole_barrier_and(2, 256, ok);  // everyone is done with the last head's table
           copy_table(room, tables, hk * pr.G + hg, bias, threadIdx.x, 256);
-          ok = named_barrier_and(2, 256, ok);
+          ok = whole_barrier_and(2, 256, ok);
           tab = room;
         } else {
           tab = tables + static_cast<long long>(hk * pr.G + hg) * table_size(bias);
@@ -1031,7 +1032,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
       for (int t = threadIdx.x; t < lut_size(bias) / 2; t += 256)
         reinterpret_cast<uint32_t*>(lut)[t] = reinterpret_cast<const uint32_t*>(lut_g)[t];
     }
-    named_barrier_and(2, 256, true);
+    whole_barrier_and(2, 256, true);
     dl = delta_s[row];
     const int lim = CAUSAL ? min(n_keys - 1, qg + off) : n_keys - 1;  // last visible key
     const uint32_t t_s = tmem + lane_off + CW * g;
@@ -1133,7 +1134,7 @@ __global__ void __launch_bounds__(BwdShape<D>::THREADS, BwdShape<D>::CTAS)
         sums[lut[0]] += sum_l;
         sums[lut[bias.left + bias.right]] += sum_r;
       }
-      if (named_barrier_and(2, 256, done)) {
+      if (whole_barrier_and(2, 256, done)) {
         float* dst = bias_part + (static_cast<long long>(bh) * nblk * n_split + cw.rank) * bias.buckets;
         for (int u = threadIdx.x; u < bias.buckets; u += 256) {
           float a = 0.f;

@@ -155,6 +155,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
+// named_barrier_and, for warps whose lanes may have come apart (loops and branches by lane in
+// front of it): the hardware barrier is an aligned one, which wants each warp whole.
+__device__ __forceinline__ bool whole_barrier_and(int id, int n, bool pred) {
+  __syncwarp();
+  return named_barrier_and(id, n, pred);
+}
+
 // Zero the rows from `row` on of a tile of ROWS rows in shared memory (64-column slabs, 128
 // bytes a row; the swizzle moves nothing between rows).  The whole warp calls it,
 // before it issues MMAs that read the tile.  A probability of 0 does not undo a NaN in the

@@ -477,6 +477,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       else if (LSE != nullptr)
         LSE[ridx] = lse;
     }
+    __syncwarp();  // tensor memory is loaded by whole warps
     // O, then (EXACT) its remainder, over the Q tile, which is free once every MMA has finished
 #pragma unroll 1
     for (int rem = 0; rem < (EXACT && n_split == 1 ? 2 : 1); ++rem) {
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
       }
       if (n_split == 1) {  // the store leaves out rows from Sq on
         fence_proxy_async_smem();
-        const bool store = named_barrier_and(1 + i, 128, done);
+        const bool store = whole_barrier_and(1 + i, 128, done);
         if (row == 0 && store && mi < pr.Sq) {
 #pragma unroll
           for (int sl = 0; sl < SLABS; ++sl)
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXAC
           bulk_commit_group();
           bulk_wait_read();
         }
-        if (EXACT) named_barrier_and(1 + i, 128, true);  // the tile has been read
+        if (EXACT) whole_barrier_and(1 + i, 128, true);  // the tile has been read
       }
     }
   }

@@ -44,8 +44,10 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Barrier of all threads of the cluster, with release and acquire of shared memory.
+// Barrier of all threads of the cluster, with release and acquire of shared memory.  Like the
+// barriers of a CTA it wants each warp whole.
 __device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Load from the shared memory of the cluster's CTA `rank`, at this CTA's address `addr`.
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     if (ok) sg = *seg_slot(n);
     __syncwarp();
     if (lane == 0) mbar_arrive(seg_empty(n));
-    ok = named_barrier_and(1, NC, ok);
+    ok = whole_barrier_and(1, NC, ok);
     if (!ok || sg.tiles == 0) break;
     const int b = sg.b, n_keys = sg.keys;
     const int hk = sg.item / row_tiles, row0 = sg.item % row_tiles * ROWS;
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
         const int g = g0 + t / bias.buckets;
         entry[t] = g < pr.G ? bias.entry(t % bias.buckets, hk * pr.G + g, pr.Hq) : 0.f;
       }
-      named_barrier_and(1, NC, true);
+      whole_barrier_and(1, NC, true);
     }
 
     float acc[D / 8][4];
@@ -494,14 +496,14 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     float f[4] = {}, m = -INFINITY, total = 0.f;
 #pragma unroll
     for (int round = 0; round < D / JOIN; ++round) {
-      if (round > 0) named_barrier_and(1, NC, true);  // the last round has been read
+      if (round > 0) whole_barrier_and(1, NC, true);  // the last round has been read
 #pragma unroll
         for (int d = 0; d < JOIN / 8; ++d)
 #pragma unroll
           for (int x = 0; x < NX; ++x)
             *reinterpret_cast<float2*>(so + (warp * 16 + x * 8 + quad) * JOIN + 8 * d + 2 * qlane) =
                 make_float2(acc[round * (JOIN / 8) + d][2 * x], acc[round * (JOIN / 8) + d][2 * x + 1]);
-      ok = named_barrier_and(1, NC, ok);
+      ok = whole_barrier_and(1, NC, ok);
       if (!valid) continue;
       if (round == 0) {  // the warps' weights, normalised
 #pragma unroll

@@ -41,3 +41,22 @@ def test_early_kernels_take_no_constant_pointers(name):
     parameters, body = KERNELS[name]
     if "griddepcontrol.wait" in body:
         assert not re.search(r"const\s+[\w ]+\*\s*__restrict__", parameters)
+
+
+def functions_with(needle):
+    """Bodies of the device functions that contain `needle`."""
+    for path in SOURCES:
+        text = re.sub(r"//[^\n]*", "", path.read_text())
+        for m in re.finditer(r"__device__ __forceinline__ \w+ (\w+)\([^)]*\) \{\n(.*?)\n\}", text, re.S):
+            if needle in m.group(2):
+                yield m.group(1), m.group(2)
+
+
+def test_aligned_barriers_find_their_warps_whole():
+    """bar.red and barrier.cluster.arrive.aligned want all lanes of a warp at once, and lanes come
+    apart in loops and branches by lane: each stands in one function, behind a __syncwarp()."""
+    for needle, name in (("named_barrier_and(", "whole_barrier_and"), ("barrier.cluster.arrive", "cluster_barrier")):
+        assert sum(p.read_text().count(needle) for p in SOURCES) == 1, needle
+        found = dict(functions_with(needle))
+        assert list(found) == [name]
+        assert found[name].index("__syncwarp();") < found[name].index(needle)
