@@ -436,8 +436,9 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   if ((rc = make_map(&tv, c.v, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
   if ((rc = make_map(&tdk, c.dk, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
   if ((rc = make_map(&tdv, c.dv, pr.B, pr.Hkv, pr.Sk, pr.D))) return rc;
+  const bool queries = pr.Hq > 0 && pr.Sq > 0;
   tq = tdo = tk;  // without queries nothing is loaded through them
-  if (pr.Sq > 0) {
+  if (queries) {
     if ((rc = make_map(&tq, c.q, pr.B, pr.Hq, pr.Sq, pr.D, W::STEP))) return rc;
     if ((rc = make_map(&tdo, c.dout, pr.B, pr.Hq, pr.Sq, pr.D, W::STEP))) return rc;
   }
@@ -454,7 +455,7 @@ static int launch_gen_dkdv(const Call& c, const BwdPlan& w, float* ws) {
   const float* tables = ws + w.table_off;
   const float *lse = ws, *delta = ws + w.stat_floats;
   const int smem = L::smem_bytes(c.bias), group = work_group(pr.B * pr.Hkv, rows, pr.D, CAUSAL);
-  if (pr.Sq > 0)  // behind the kernel that writes delta
+  if (queries)  // behind the kernel that writes delta
     return launch_early(kern, grid, W::THREADS, smem, c.stream, tk, tv, tq, tdo, tdk, tdv, pr, c.bias, tables, lse,
                         delta, ws + w.dk_off, ws + w.dv_off, w.dkdv_split, group);
   kern<<<grid, W::THREADS, smem, c.stream>>>(tk, tv, tq, tdo, tdk, tdv, pr, c.bias, tables, lse, delta, ws + w.dk_off,

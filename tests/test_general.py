@@ -264,6 +264,23 @@ def test_empty(B, Hq, Hkv, Sq, Sk):
             assert g.shape == t.shape and (g == 0).all()
 
 
+@pytest.mark.parametrize("Hkv", [0, 2])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [4, 300])
+def test_no_query_heads(Hkv, Sq, D):
+    """No query heads, over key heads too: an empty output, and zeros for every key and value."""
+    q, k, v = (torch.randn(2, h, s, D, device="cuda").to(torch.bfloat16).requires_grad_(True)
+               for h, s in ((0, Sq), (Hkv, 200), (Hkv, 200)))
+    bias = torch.zeros(32, 0, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    calls = [(cross_attention(q, k, v, enable_gqa=True), (q, k, v))]
+    calls.append((relative_attention(q, k, v, bias, enable_gqa=True), (q, k, v, bias)))
+    for o, leaves in calls:
+        assert o.shape == (2, 0, Sq, D)
+        for g, t in zip(torch.autograd.grad(o, leaves, torch.ones_like(o)), leaves):
+            assert g.shape == t.shape and (g == 0).all()
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
 # ---- relative position bias --------------------------------------------------------------
 
 def table(buckets, H, seed=11, size=2.0):
