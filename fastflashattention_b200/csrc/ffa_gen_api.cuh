@@ -42,7 +42,7 @@ inline int check_problem(const ffa_gen_problem* p) {
   if (p->query_offset > kOffsetLimit || p->query_offset < -kOffsetLimit)
     return set_error(FFA_ERR_UNSUPPORTED, "query_offset must be within +-2^29");
   if (!std::isfinite(p->scale)) return set_error(FFA_ERR_INVALID, "scale must be finite");
-  if (p->causal && !p->bias)
+  if (p->causal && !p->bias && p->q_heads > 0)  // (the bias of no heads has no data)
     return set_error(FFA_ERR_UNSUPPORTED, "general attention is causal only with a position bias (see ffa_fwd)");
   if (p->bias) {
     if (p->buckets < 1 || p->buckets > kMaxBuckets || (p->both && p->buckets % 2 != 0) || !p->borders)

@@ -273,11 +273,14 @@ def test_no_query_heads(Hkv, Sq, D):
                for h, s in ((0, Sq), (Hkv, 200), (Hkv, 200)))
     bias = torch.zeros(32, 0, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     calls = [(cross_attention(q, k, v, enable_gqa=True), (q, k, v))]
-    calls.append((relative_attention(q, k, v, bias, enable_gqa=True), (q, k, v, bias)))
+    for causal in (False, True):
+        calls.append((relative_attention(q, k, v, bias, is_causal=causal, enable_gqa=True), (q, k, v, bias)))
     for o, leaves in calls:
         assert o.shape == (2, 0, Sq, D)
         for g, t in zip(torch.autograd.grad(o, leaves, torch.ones_like(o)), leaves):
             assert g.shape == t.shape and (g == 0).all()
+    with torch.no_grad():
+        assert relative_attention(q, k, v, bias, is_causal=True, enable_gqa=True).shape == (2, 0, Sq, D)
     assert _lib.device_status() == (0, 0, 0, 0)
 
 

@@ -247,6 +247,16 @@ def test_c_abi_nothing_to_do():
         assert lib.ffa_gen_fwd(ctypes.byref(p), t, t, t, t, None, None, None, 0, None) == _lib.FFA_OK
 
 
+@pytest.mark.parametrize("causal", [0, 1])
+def test_c_abi_no_query_heads_over_key_heads(causal):
+    """A table of no heads has no data: a null bias is then no refusal."""
+    lib = _lib.load()
+    t = ctypes.byref(_lib.GenTensor(16, 64, 64, 64))
+    p = problem(q_heads=0, causal=causal)
+    assert lib.ffa_gen_fwd(ctypes.byref(p), t, t, t, t, None, None, None, 0, None) == _lib.FFA_OK
+    assert lib.ffa_gen_bwd_workspace(ctypes.byref(p)) >= 0
+
+
 def test_operators_are_registered():
     ops = _lib.ops()
     for name in ("general", "general_lse", "general_backward", "general_attention"):
