@@ -12,6 +12,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -30,6 +31,14 @@ def _rows_problem(name, t, batch, device):
         return f"{name} dtype is {t.dtype}; only int32 is supported"
     if tuple(t.shape) != (batch,) or not t.is_contiguous():
         return f"{name} must be a contiguous tensor of shape ({batch},), one entry for each sequence"
+    return None
+
+
+def _tangent_problem(*tensors):
+    """Why forward-mode derivatives rule out the tensors, or ``None``: the kernels know none, and
+    a tangent that is dropped would be a derivative of zero."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return "forward-mode derivatives (dual tensors, torch.func.jvp) are not supported"
     return None
 
 
@@ -79,8 +88,10 @@ def _shape_reason(query, key, value, key_lengths, scale, enable_gqa):
     if scale is not None and not math.isfinite(scale):
         return f"scale={scale}; must be finite"
     if key_lengths is not None:
-        return _rows_problem("key_lengths", key_lengths, query.shape[0], query.device)
-    return None
+        problem = _rows_problem("key_lengths", key_lengths, query.shape[0], query.device)
+        if problem is not None:
+            return problem
+    return _tangent_problem(query, key, value)
 
 
 def _bias_reason(query, bias, max_distance, bidirectional, is_causal, query_offset):
@@ -103,12 +114,14 @@ def _bias_reason(query, bias, max_distance, bidirectional, is_causal, query_offs
         return (f"max_distance={max_distance}; must be an integer above the {first} distances that have a bucket of "
                 f"their own, at most {_MAX_DISTANCE}")
     if isinstance(query_offset, torch.Tensor):
-        return _rows_problem("query_offset", query_offset, query.shape[0], query.device)
-    if isinstance(query_offset, bool) or not isinstance(query_offset, int):
+        problem = _rows_problem("query_offset", query_offset, query.shape[0], query.device)
+        if problem is not None:
+            return problem
+    elif isinstance(query_offset, bool) or not isinstance(query_offset, int):
         return "query_offset is neither an integer nor a torch.Tensor"
-    if abs(query_offset) > _MAX_LEN:
+    elif abs(query_offset) > _MAX_LEN:
         return f"query_offset={query_offset}; must be within +-2^29"
-    return None
+    return _tangent_problem(bias)
 
 
 @functools.lru_cache(maxsize=64)
@@ -163,7 +176,7 @@ def cross_attention(query, key, value, key_lengths=None, scale=None, enable_gqa=
     ``enable_gqa``: Hq may be a multiple of Hkv; query head h reads key head h // (Hq / Hkv).
     ``scale`` defaults to ``1/sqrt(D)``.
 
-    The backward is deterministic.  A few queries (Hq / Hkv * Sq up to 64, a decoding step)
+    The backward is deterministic; second and forward-mode derivatives are refused.  A few queries (Hq / Hkv * Sq up to 64, a decoding step)
     take one pass over the keys that is split over the SMs.
     """
     reason = _shape_reason(query, key, value, key_lengths, scale, enable_gqa)

@@ -15,6 +15,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/autograd.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
@@ -241,6 +242,8 @@ class GeneralAttention : public torch::autograd::Function<GeneralAttention> {
 
   static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx,
                                                torch::autograd::tensor_list grads) {
+    TORCH_CHECK(!grads[0]._fw_grad(0).defined(),
+                "the backward of general attention does not support forward-mode derivatives of the output's gradient");
     const auto s = ctx->get_saved_variables();
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     auto& d = ctx->saved_data;
@@ -304,4 +307,10 @@ TORCH_LIBRARY_IMPL(ffa_b200, CUDA, m) {
   m.impl("general_attention", general_op);  // reached only where autograd is off (inference mode)
 }
 
-TORCH_LIBRARY_IMPL(ffa_b200, Autograd, m) { m.impl("general_attention", general_attention_op); }
+// Without a kernel of their own the other operators would drop tangents (forward-mode
+// derivatives) without a word; this one refuses them, and a backward through their outputs.
+TORCH_LIBRARY_IMPL(ffa_b200, Autograd, m) {
+  m.impl("general_attention", general_attention_op);
+  for (const char* name : {"general", "general_lse", "general_backward"})
+    m.impl(name, torch::autograd::autogradNotImplementedFallback());
+}

@@ -10,8 +10,11 @@ import threading
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from fastflashattention_b200 import RelativeFlashAttention, _lib, cross_attention, fast_attention, relative_attention
+from fastflashattention_b200 import (RelativeFlashAttention, UnsupportedConfig, _lib, cross_attention, fast_attention,
+                                     relative_attention)
+from fastflashattention_b200._general import bucket_borders
 from oracle.general_oracle import attend
 
 pytestmark = pytest.mark.gpu
@@ -458,6 +461,43 @@ def test_second_derivatives_are_refused():
     near(g, attend(q, k, v, do)["dq"], "dq")
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
         g.sum().backward()
+
+
+FORWARD_MODE = "forward-mode|forward AD"
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("Sq", [2, 100])
+def test_forward_mode_derivatives_are_refused(Sq, grad):
+    """Dual tensors, torch.func.jvp, a tangent of the output's gradient, and the registered operators."""
+    q, k, v, do = inputs(1, 2, 2, Sq, 120, 64)
+    bias = table(32, 2)
+    general = torch.ops.ffa_b200.general
+    calls = {
+        "cross": lambda q, k, v, b: cross_attention(q, k, v),
+        "relative": relative_attention,
+        "general": lambda q, k, v, b: general(q, k, v, b, None, None, 0, list(bucket_borders(16, 128)), True, False, None),
+        "lse": lambda q, k, v, b: torch.ops.ffa_b200.general_lse(q, k, v, None, None, None, 0, [], False, False, None,
+                                                                 False)[0],
+    }
+    if grad:
+        q.requires_grad_(True)
+    for name, call in calls.items():
+        for at in range(4 if name in ("relative", "general") else 3):
+            args = [q, k, v, bias]
+            def one(x):
+                return call(*args[:at], x, *args[at + 1:])
+            with pytest.raises((UnsupportedConfig, RuntimeError), match=FORWARD_MODE):
+                torch.func.jvp(one, (args[at].detach(),), (torch.ones_like(args[at]),))
+            with forward_ad.dual_level(), pytest.raises((UnsupportedConfig, RuntimeError), match=FORWARD_MODE):
+                one(forward_ad.make_dual(args[at], torch.ones_like(args[at])))
+    q2 = q.detach().clone().requires_grad_(True)
+    o = cross_attention(q2, k, v)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(o, [q2], forward_ad.make_dual(do, torch.ones_like(do)), retain_graph=True)
+        near(cross_attention(q, k, v), attend(q, k, v)["o"], "o")  # a level without tangents is no matter
+    near(torch.autograd.grad(o, [q2], do)[0], attend(q, k, v, do)["dq"], "dq")
 
 
 @pytest.mark.parametrize("D", [64, 128])

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from fastflashattention_b200 import (RelativeFlashAttention, UnsupportedConfig, _lib, cross_attention,
                                      relative_attention)
@@ -93,6 +94,52 @@ def test_bias_outside_the_contract(bias, extra, needle):
     q = fake(2, 4, 3, 64)
     with pytest.raises(UnsupportedConfig, match=needle):
         relative_attention(q, q, q, bias, **extra)
+
+
+@pytest.mark.parametrize("dual", ["query", "key", "value", "bias"])
+def test_forward_mode_derivatives_are_refused(dual):
+    """The kernels know no tangents: a derivative of zero without a word would be wrong."""
+    shapes = {"query": (1, 2, 3, 64), "key": (1, 2, 5, 64), "value": (1, 2, 5, 64), "bias": (32, 2)}
+    with forward_ad.dual_level():
+        t = {n: fake(*s) for n, s in shapes.items()}
+        assert _shape_reason(t["query"], t["key"], t["value"], None, None, False) is None
+        assert _bias_reason(t["query"], t["bias"], 128, None, False, 0) is None
+        plain = torch.zeros(*shapes[dual], dtype=torch.bfloat16)
+        t[dual] = forward_ad.make_dual(plain, torch.ones_like(plain)).as_subclass(Cuda)
+        assert forward_ad.unpack_dual(t[dual]).tangent is not None
+        with pytest.raises(UnsupportedConfig, match="forward-mode"):
+            relative_attention(t["query"], t["key"], t["value"], t["bias"])
+        if dual != "bias":
+            with pytest.raises(UnsupportedConfig, match="forward-mode"):
+                cross_attention(t["query"], t["key"], t["value"])
+
+
+def test_registered_operators_refuse_tangents():
+    """The operators themselves, with a stand-in for the kernel: dual tensors and torch.func.jvp
+    raise, a level without tangents and a disabled forward mode do not, and backward raises."""
+    ops = _lib.ops()
+    stand_in = torch.library.Library("ffa_b200", "IMPL")
+    try:
+        stand_in.impl("general", lambda q, *_: q * 2, "CPU")
+        q = torch.ones(1, 1, 2, 8)
+        call = lambda q, bias=None: ops.general(q, q, q, bias, None, None, 0, [], False, False, None)  # noqa: E731
+        with pytest.raises(NotImplementedError, match="forward AD"):
+            torch.func.jvp(call, (q,), (q,))
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(q, q)
+            for args in ((dual,), (q, dual)):
+                with pytest.raises(NotImplementedError, match="forward AD"):
+                    call(*args)
+            assert torch.equal(call(q), q * 2)
+            with forward_ad._set_fwd_grad_enabled(False):
+                assert torch.equal(call(dual), q * 2)
+        leaf = q.clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="not implemented"):
+            call(leaf).sum().backward()
+        with torch.no_grad():
+            assert not call(leaf).requires_grad
+    finally:
+        stand_in._destroy()
 
 
 def test_smallest_tables_are_inside_the_contract():
