@@ -29,7 +29,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ._general import cross_attention, relative_attention
+from ._general import _tangent_problem, cross_attention, relative_attention
 from ._kernel import attention_train, fastflash_attn, fastflash_attn_train, FastFlashAttn, LOG2E  # noqa: F401
 
 __all__ = [
@@ -73,7 +73,8 @@ def _reason(query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gq
     """Why the input is unsupported (a message), or ``None`` if it is supported.
 
     Checks run in the reference order (``__init__.py:56-80``): mask, dropout, GQA flag,
-    then per-tensor type / device / dtype / rank, then equal shapes, then head_dim.
+    then per-tensor type / device / dtype / rank, then equal shapes, then head_dim; behind
+    them, forward-mode derivatives.
     """
     if attn_mask is not None:
         return "attn_mask is not supported (strict policy); pass attn_mask=None and use is_causal"
@@ -92,7 +93,7 @@ def _reason(query, key, value, attn_mask, dropout_p, is_causal, scale, enable_gq
     head_dim = shapes[0][-1]
     if head_dim not in _HEAD_DIMS:
         return f"head_dim={head_dim}; must be a power of two <= 128"
-    return None
+    return _tangent_problem(query, key, value)
 
 
 def is_eligible(query, key, value, attn_mask=None, dropout_p=0.0,

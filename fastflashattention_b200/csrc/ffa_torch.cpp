@@ -22,6 +22,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/autograd.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -122,6 +123,8 @@ class Attention : public torch::autograd::Function<Attention> {
 
   static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx,
                                                torch::autograd::tensor_list grads) {
+    TORCH_CHECK(!grads[0]._fw_grad(0).defined(),
+                "the backward of attention does not support forward-mode derivatives of the output's gradient");
     const auto saved = ctx->get_saved_variables();
     const bool causal = ctx->saved_data["causal"].toBool();
     c10::optional<double> scale;
@@ -152,4 +155,10 @@ TORCH_LIBRARY_IMPL(ffa_b200, CUDA, m) {
   m.impl("backward", backward_op);
 }
 
-TORCH_LIBRARY_IMPL(ffa_b200, Autograd, m) { m.impl("attention", attention_op); }
+// Without a kernel of their own the other operators would drop tangents (forward-mode
+// derivatives) without a word; this one refuses them, and a backward through their outputs.
+TORCH_LIBRARY_IMPL(ffa_b200, Autograd, m) {
+  m.impl("attention", attention_op);
+  for (const char* name : {"forward", "forward_lse", "backward"})
+    m.impl(name, torch::autograd::autogradNotImplementedFallback());
+}
