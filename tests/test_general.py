@@ -472,12 +472,12 @@ def test_forward_mode_derivatives_are_refused(Sq, grad):
     """Dual tensors, torch.func.jvp, a tangent of the output's gradient, and the registered operators."""
     q, k, v, do = inputs(1, 2, 2, Sq, 120, 64)
     bias = table(32, 2)
-    general = torch.ops.ffa_b200.general
+    general = _lib.ops().general
     calls = {
         "cross": lambda q, k, v, b: cross_attention(q, k, v),
         "relative": relative_attention,
         "general": lambda q, k, v, b: general(q, k, v, b, None, None, 0, list(bucket_borders(16, 128)), True, False, None),
-        "lse": lambda q, k, v, b: torch.ops.ffa_b200.general_lse(q, k, v, None, None, None, 0, [], False, False, None,
+        "lse": lambda q, k, v, b: _lib.ops().general_lse(q, k, v, None, None, None, 0, [], False, False, None,
                                                                  False)[0],
     }
     if grad:
