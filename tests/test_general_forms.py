@@ -1,0 +1,185 @@
+"""GPU: the LSE of every form of general attention's forward, gradients through each of them, and
+the registered operators that give both.
+
+The LSE (base 2, -inf without a key) is what the backward recomputes probabilities from.  Which
+form a call takes - one CTA, a cluster of CTAs or equal shares for a few rows, whole or split
+keys for many - depends on its sizes; each is held to the 64-bit oracle's bounds.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from fastflashattention_b200 import _lib, cross_attention, relative_attention
+from fastflashattention_b200._general import bucket_borders
+from oracle.general_oracle import FINE, HALF, PAIR, attend
+
+pytestmark = pytest.mark.gpu
+
+TOL = 5e-3
+
+
+def rnd(gen, *shape, size=1.0):
+    return (torch.randn(*shape, device="cuda", generator=gen) * size).to(torch.bfloat16)
+
+
+def inputs(B, Hq, Hkv, Sq, Sk, D, seed=0, size=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (rnd(gen, B, Hq, Sq, D, size=size), rnd(gen, B, Hkv, Sk, D), rnd(gen, B, Hkv, Sk, D), rnd(gen, B, Hq, Sq, D))
+
+
+def table(H, buckets=32, seed=11):
+    return rnd(torch.Generator(device="cuda").manual_seed(seed), buckets, H, size=2.0)
+
+
+def step_lengths(B, Sk):
+    """Lengths of a padded batch: the longest, none, one, and others between."""
+    return torch.tensor([(Sk, 0, 1, Sk // 3, Sk - 5, Sk // 2)[b % 6] for b in range(B)], dtype=torch.int32, device="cuda")
+
+
+def mask_args(bias=None, causal=False, lengths=None, offsets=0, distance=128):
+    """The operators' <mask> arguments and the oracle's, of the same mask."""
+    borders = list(bucket_borders(bias.shape[0] // (1 if causal else 2), distance)) if bias is not None else []
+    tensor = isinstance(offsets, torch.Tensor)
+    both = bias is not None and not causal
+    op = (bias, lengths, offsets if tensor else None, 0 if tensor else offsets, borders, both, causal, None)
+    return op, dict(bias=bias, causal=causal, both=both, lengths=lengths, offsets=offsets, max_distance=distance)
+
+
+def inside(got, want, name, gate=TOL):
+    value, bound = want
+    got = got.detach().double()
+    assert got.shape == value.shape and torch.isfinite(got).all(), name
+    assert ((got - value).abs() - bound).max() <= 0, f"{name}: {float(((got - value).abs() - bound).max())} over the bound"
+    if gate is not None and value.norm() > 0:
+        assert (got - value).norm() <= gate * value.norm(), name
+
+
+def lse_inside(got, want):
+    """-inf exactly where no key is seen, and everywhere else inside the oracle's bound."""
+    value, bound = want
+    none = value == -math.inf
+    assert got.dtype == torch.float32 and got.shape == value.shape
+    assert torch.equal(got == -math.inf, none)
+    far = torch.where(none, 0.0, (got.double() - value).abs() - bound)
+    assert not torch.isnan(far).any() and far.max() <= 0, f"LSE: {float(far.max())} over the bound"
+
+
+def check(q, k, v, do, grads=True, **mask):
+    """o and LSE of general_lse, and what general_backward makes of them."""
+    ops = _lib.ops()
+    op, oracle = mask_args(**mask)
+    want = attend(q, k, v, do if grads else None, exact=False, **oracle)
+    o, lo, lse = ops.general_lse(q, k, v, *op, False)
+    assert lo.numel() == 0
+    inside(o, want["o"], "o")
+    lse_inside(lse, want["lse"])
+    if grads:
+        dq, dk, dv, db = ops.general_backward(q, k, v, o, None, do, lse, *op, True, True, False)
+        assert db.numel() == 0
+        for name, g in (("dq", dq), ("dk", dk), ("dv", dv)):
+            inside(g, want[name], name)
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+# ---- a few rows ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("items, rows, Sk, D", [
+    (297, 1, 300, 64), (160, 1, 300, 128),                                        # one CTA for each item
+    (148, 1, 600, 64), (64, 1, 1100, 64), (32, 1, 2100, 64), (12, 1, 4200, 64),   # clusters of 2, 4, 8, 16 CTAs
+    (148, 9, 300, 128), (64, 9, 600, 128), (32, 9, 1100, 128), (12, 9, 2100, 128),
+])
+def test_lse_of_clusters(items, rows, Sk, D):
+    check(*inputs(1, items, items, rows, Sk, D))
+    check(*inputs(items, 1, 1, rows, Sk, D), lengths=step_lengths(items, Sk))
+    lens = step_lengths(items, Sk)  # sequences that are shorter than their new tokens, too
+    check(*inputs(items, 1, 1, rows, Sk, D), bias=table(1), causal=True, lengths=lens, offsets=lens - rows)
+
+
+@pytest.mark.parametrize("items, Sk, D", [(148, 300, 64), (74, 600, 64), (32, 1100, 128), (14, 1100, 128), (6, 1100, 64)])
+def test_lse_of_clusters_with_32_rows(items, Sk, D):
+    check(*inputs(1, 4 * items, items, 6, Sk, D))
+    check(*inputs(1, 4 * items, items, 6, Sk, D), bias=table(4 * items), offsets=Sk - 6, causal=True)
+
+
+@pytest.mark.parametrize("B, Hkv, G, Sq, Sk, D, ragged", [
+    (2, 4, 8, 3, 20000, 128, False), (4, 4, 4, 8, 20000, 64, True), (10, 10, 3, 7, 6000, 128, False),  # 32 rows
+    (1, 13, 1, 1, 50000, 128, False), (1, 13, 9, 1, 100000, 64, False), (11, 3, 1, 1, 20000, 128, True),  # 16 rows
+])
+def test_lse_of_shares(B, Hkv, G, Sq, Sk, D, ragged):
+    q, k, v, do = inputs(B, G * Hkv, Hkv, Sq, Sk, D)
+    lens = step_lengths(B, Sk) if ragged else None
+    p = _lib.GenProblem(batch=B, q_heads=G * Hkv, kv_heads=Hkv, q_len=Sq, k_len=Sk, head_dim=D, scale=1.0)
+    if ragged:
+        p.key_lengths = lens.data_ptr()
+    assert _lib.load().ffa_gen_fwd_workspace(ctypes.byref(p), 0) > 0  # room for the parts
+    check(q, k, v, do, lengths=lens)
+    check(q, k, v, do, bias=table(G * Hkv), causal=True, lengths=lens, offsets=lens - Sq if ragged else Sk - Sq)
+
+
+@pytest.mark.parametrize("B, Hkv, G, Sq, Sk, D", [
+    (1, 12, 1, 1, 4200, 64), (40, 8, 1, 1, 300, 64), (1, 13, 1, 2, 50000, 128), (2, 4, 8, 3, 20000, 64),
+])
+def test_gradients_through_a_few_rows(B, Hkv, G, Sq, Sk, D):
+    """The public calls: keys and values that want gradients, and a table that does not."""
+    q, k, v, do = inputs(B, G * Hkv, Hkv, Sq, Sk, D)
+    lens = step_lengths(B, Sk) if B > 1 else None
+    bias = table(G * Hkv)
+    for frozen in (None, bias):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        if frozen is None:
+            o = cross_attention(*leaves, key_lengths=lens, enable_gqa=G > 1)
+            want = attend(q, k, v, do, lengths=lens)
+        else:
+            o = relative_attention(*leaves, frozen, key_lengths=lens, query_offset=Sk // 2, enable_gqa=G > 1)
+            want = attend(q, k, v, do, bias=frozen, both=True, lengths=lens, offsets=Sk // 2, exact=False)
+        inside(o, want["o"], "o")
+        for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)):
+            inside(g, want[name], name)
+
+
+# ---- many rows ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("Sq, Sk", [(100, 4000), (300, 300), (1000, 77), (130, 0)])
+def test_lse_of_whole_and_split_keys(Sq, Sk, D):
+    check(*inputs(2, 2, 1, Sq, Sk, D), grads=Sk > 0)
+    if Sk:
+        lens = torch.tensor([Sk // 3, 0], dtype=torch.int32, device="cuda")
+        check(*inputs(2, 2, 1, Sq, Sk, D), lengths=lens)
+        check(*inputs(2, 2, 1, Sq, Sk, D), bias=table(2), causal=True, offsets=-70)  # rows without a key
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq, Sk", [(100, 4000), (300, 300)])
+def test_remainder_of_o(Sq, Sk, D):
+    """o + o_lo is O to 16 bits, whole and split, and the LSE beside it is the same contract's."""
+    q, k, v, _ = inputs(2, 2, 1, Sq, Sk, D)
+    op, oracle = mask_args(bias=table(2))
+    want = attend(q, k, v, exact=True, **oracle)
+    value, bound = want["o"]
+    weighed = (bound - 1e-7 - HALF * value.abs()) / (HALF + FINE)  # P |V|
+    o, lo, lse = _lib.ops().general_lse(q, k, v, *op, True)
+    # what rounding O to nearest leaves is at most half a step.  (o + lo need not round to o: a
+    # remainder just below half a step rounds to half a step, and o + lo is then a tie.)
+    assert (lo.double().abs() <= HALF * o.double().abs()).all()
+    fine = PAIR * value.abs() + (PAIR + FINE) * weighed + 1e-7
+    inside(o.double() + lo.double(), (value, fine), "o + o_lo", gate=None)
+    lse_inside(lse, want["lse"])
+
+
+@pytest.mark.parametrize("want_dq, want_dkdv, want_db", [(True, False, False), (False, True, False), (True, True, True),
+                                                         (False, False, True), (True, False, True), (False, True, True)])
+def test_backward_operator_gives_what_is_wanted(want_dq, want_dkdv, want_db):
+    q, k, v, do = inputs(2, 4, 2, 150, 170, 64)
+    op, oracle = mask_args(bias=table(4))
+    # the remainder is read with dQ, which dbias comes with
+    want = attend(q, k, v, do, exact=want_dq or want_db, **oracle)
+    o, lo, lse = _lib.ops().general_lse(q, k, v, *op, True)
+    got = _lib.ops().general_backward(q, k, v, o, lo, do, lse, *op, want_dq, want_dkdv, want_db)
+    for name, g, wanted in zip(("dq", "dk", "dv", "dbias"), got, (want_dq or want_db, want_dkdv, want_dkdv, want_db)):
+        if wanted:
+            inside(g, want[name], name, gate=None if name == "dbias" else TOL)
+        else:
+            assert g.numel() == 0
