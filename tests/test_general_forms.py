@@ -13,7 +13,7 @@ import torch
 
 from fastflashattention_b200 import _lib, cross_attention, relative_attention
 from fastflashattention_b200._general import bucket_borders
-from oracle.general_oracle import FINE, HALF, PAIR, attend
+from oracle.general_oracle import FINE, HALF, PAIR, attend, bucket_of
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,72 @@ def test_backward_operator_gives_what_is_wanted(want_dq, want_dkdv, want_db):
             inside(g, want[name], name, gate=None if name == "dbias" else TOL)
         else:
             assert g.numel() == 0
+
+
+# ---- the bias's gradient -------------------------------------------------------------------
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D, seed", [(64, 1), (128, 0)])
+def test_remainder_of_o_is_what_the_bias_gradient_needs(D, seed, causal):
+    """dbias adds dS over whole rows, whose sum is 0, so an error of delta = O . dO, common to a
+    row, stays where dS cancels.  Values with a common mean leave dS as it is and enlarge that
+    error.  With the remainder dbias is off by its own rounding to bf16, at most 2^-8 of each
+    entry and so of the norm, and little else; without it, or without the forward that
+    computes it, by 1.9 to 40 % of the norm (the same inputs in 64 bits with O, or P and O,
+    rounded to bf16).  5e-3 lies between them."""
+    gen = torch.Generator().manual_seed(seed)
+    one = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16)  # noqa: E731
+    B, H, S = 1, 2, 1485
+    q, k = (one(B, H, S, D).float() * D ** -0.5).to(torch.bfloat16).cuda(), one(B, H, S, D).cuda()
+    v, do = (one(B, H, S, D).float() + 4).to(torch.bfloat16).cuda(), one(B, H, S, D).cuda()
+    bias = (torch.randn(16, H, generator=gen) * 2).to(torch.bfloat16).cuda()
+    op, oracle = mask_args(bias=bias, causal=causal, distance=64)
+    op = (*op[:-1], 1.0)
+    value = attend(q, k, v, do, scale=1.0, **oracle)["dbias"][0]
+
+    def off(g):
+        return float((g.double() - value).norm() / value.norm())
+
+    leaf = bias.clone().requires_grad_(True)
+    o = relative_attention(q, k, v, leaf, max_distance=64, is_causal=causal, scale=1.0)
+    public = off(torch.autograd.grad(o, [leaf], do)[0])
+    ops = _lib.ops()
+    o, lo, lse = ops.general_lse(q, k, v, *op, True)
+    with_lo = off(ops.general_backward(q, k, v, o, lo, do, lse, *op, True, False, True)[3])
+    dropped = off(ops.general_backward(q, k, v, o, None, do, lse, *op, True, False, True)[3])
+    o, _, lse = ops.general_lse(q, k, v, *op, False)
+    plain = off(ops.general_backward(q, k, v, o, None, do, lse, *op, True, False, True)[3])
+    print(f"dbias off by {public:.5f} {with_lo:.5f}, without the remainder {dropped:.5f} {plain:.5f}")
+    assert public <= TOL and with_lo <= TOL
+    assert dropped > TOL and plain > TOL
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B, H, S, D, buckets, distance", [
+    (2, 3, 70, 64, 32, 128), (1, 4, 385, 64, 16, 64), (1, 2, 700, 128, 64, 256), (2, 2, 300, 96, 256, 1024),
+    (1, 6, 513, 64, 128, 800),
+])
+def test_bias_gradient_as_a_whole(B, H, S, D, buckets, distance, causal):
+    """The norm of dbias's error where errors of different rows are independent: the rounding of
+    the result, and four times the root of the rows' squared errors.  (The bound of each value
+    adds up worst cases, and a few per cent of error stay inside it.)"""
+    q, k, v, do = inputs(B, H, H, S, S, D, size=D ** -0.5)
+    bias = table(H, buckets)
+    _, oracle = mask_args(bias=bias, causal=causal, distance=distance)
+    value, _ = attend(q, k, v, do, scale=1.0, **oracle)["dbias"]
+    leaf = bias.clone().requires_grad_(True)
+    o = relative_attention(q, k, v, leaf, max_distance=distance, is_causal=causal, scale=1.0)
+    (g,) = torch.autograd.grad(o, [leaf], do)
+    # a row's error: 2^-12 (exponentials, 32-bit sums) of its terms in each bucket
+    qd, kd, vd, dd = (t.double() for t in (q, k, v, do))
+    r = torch.arange(S, device="cuda")[None, :] - torch.arange(S, device="cuda")[:, None]
+    bucket = bucket_of(r, buckets, distance, not causal)
+    s = qd @ kd.transpose(-1, -2) + bias.double()[bucket].permute(2, 0, 1)
+    if causal:
+        s = s.masked_fill(r > 0, -math.inf)
+    p, dp = torch.softmax(s, -1), dd @ vd.transpose(-1, -2)
+    terms = p * (dp.abs() + (p * dp).sum(-1, keepdim=True).abs())
+    rows = torch.zeros(B, H, S, buckets, device="cuda", dtype=torch.float64)
+    rows.scatter_add_(3, bucket.expand(B, H, S, S), terms)
+    assert (g.double() - value).norm() <= HALF * value.norm() + 4 * FINE * rows.norm()
+
