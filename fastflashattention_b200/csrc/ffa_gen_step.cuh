@@ -328,25 +328,27 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     int lim[NX], pos[NX], head[NX];
     const int g0 = row0 / pr.Sq;  // the item's first head of the group
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = row0 + rg * 16 + x * 8 + quad;
-        const bool valid = x < NX && r < rows;
-        const int g = valid ? r / pr.Sq : g0, t = valid ? r % pr.Sq : 0;
-        if (x < NX) {
-          pos[x] = t + sg.off;
-          lim[x] = valid ? (CAUSAL ? min(n_keys - 1, t + sg.off) : n_keys - 1) : -1;
-          head[x] = (g - g0) * bias.buckets;
+    for (int x = 0; x < NX; ++x) {
+      const int r = row0 + rg * 16 + x * 8 + quad;
+      const bool valid = r < rows;
+      const int g = valid ? r / pr.Sq : g0, t = valid ? r % pr.Sq : 0;
+      pos[x] = t + sg.off;
+      lim[x] = valid ? (CAUSAL ? min(n_keys - 1, t + sg.off) : n_keys - 1) : -1;
+      head[x] = (g - g0) * bias.buckets;
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(q.p) + b * q.sb +
+                                 static_cast<long long>(hk * pr.G + g) * q.sh + t * q.ss;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int col = ks * 16 + y * 8 + qlane * 2;
+          qf[ks][x + 2 * y] = (valid && col < pr.D) ? *reinterpret_cast<const uint32_t*>(src + col) : 0u;
         }
-        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(q.p) + b * q.sb +
-                                   static_cast<long long>(hk * pr.G + g) * q.sh + t * q.ss;
+    }
+    if constexpr (ROWS8) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int col = ks * 16 + y * 8 + qlane * 2;
-            qf[ks][x + 2 * y] = (valid && col < pr.D) ? *reinterpret_cast<const uint32_t*>(src + col) : 0u;
-          }
-      }
+      for (int ks = 0; ks < KS; ++ks) qf[ks][1] = qf[ks][3] = 0u;
+    }
     if (BIAS) {
       const int heads = step_heads(ROWS, pr.Sq, pr.G);
       for (int t = threadIdx.x; t < heads * bias.buckets; t += NC) {
@@ -356,18 +358,12 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
       whole_barrier_and(1, NC, true);
     }
 
-    float acc[D / 8][4];
+    float acc[D / 8][4] = {};
     float mx[NX], sum[NX];
-    {
 #pragma unroll
-      for (int x = 0; x < NX; ++x) {
-        mx[x] = -INFINITY;
-        sum[x] = 0.f;
-      }
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[d][e] = 0.f;
+    for (int x = 0; x < NX; ++x) {
+      mx[x] = -INFINITY;
+      sum[x] = 0.f;
     }
     const int w0 = (warp & 3) * L::WKEYS;  // the warp's first key of a tile
     for (int j = 0; j < sg.nt; ++j, ++it) {
@@ -375,11 +371,7 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
       const uint32_t kt = sbase + (it % STAGES) * 2 * L::TILE, vt = kt + L::TILE;
       const int key0 = (sg.t0 + j) * L::KEYS + w0;
       if (key0 < n_keys) {
-        float s[2 * NG][4];
-#pragma unroll
-          for (int nt = 0; nt < 2 * NG; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        float s[2 * NG][4] = {};
 #pragma unroll
         for (int gk = 0; gk < NG; ++gk) {
           const int row = w0 + 16 * gk + (lane & 7) + ((lane >> 4) << 3);
@@ -388,10 +380,8 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
             uint32_t kf[4];
             ldmatrix4(kf, kt + (ks >> 2) * (L::KEYS * 128) + row * 128 +
                               (((2 * (ks & 3) + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
-    {
-              mma_16816(s[2 * gk], qf[ks], kf[0], kf[1]);
-              mma_16816(s[2 * gk + 1], qf[ks], kf[2], kf[3]);
-            }
+            mma_16816(s[2 * gk], qf[ks], kf[0], kf[1]);
+            mma_16816(s[2 * gk + 1], qf[ks], kf[2], kf[3]);
           }
         }
         if (key0 + L::WKEYS > n_keys) {
@@ -405,53 +395,50 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
           __syncwarp();
         }
         uint32_t pf[NG][4];
+        if constexpr (ROWS8) {  // rows 8 to 15: P = 0
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (x >= NX) {  // rows 8 to 15: P = 0
+          for (int gk = 0; gk < NG; ++gk) pf[gk][1] = pf[gk][3] = 0u;
+        }
 #pragma unroll
-              for (int gk = 0; gk < NG; ++gk) pf[gk][x] = pf[gk][2 + x] = 0u;
-              continue;
-            }
-            constexpr int X = NX - 1;  // (keeps the index below NX for the compiler)
-            const int xx = x < NX ? x : X;
-            // the row's scores of this thread: keys key0 + 8 nt + 2 qlane + {0, 1}
-            float m = -INFINITY;
+        for (int x = 0; x < NX; ++x) {
+          // the row's scores of this thread: keys key0 + 8 nt + 2 qlane + {0, 1}
+          float m = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < 2 * NG; ++nt)
+          for (int nt = 0; nt < 2 * NG; ++nt)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int key = key0 + 8 * nt + 2 * qlane + e;
-                float& y = s[nt][2 * x + e];
-                y *= pr.scale_log2;
-                if (BIAS) {
-                  const int r = min(max(key - pos[xx], -bias.left), bias.right);
-                  y += entry[head[xx] + lut[r + bias.left]];
-                }
-                if (key > lim[xx]) y = -INFINITY;
-                m = fmaxf(m, y);
+            for (int e = 0; e < 2; ++e) {
+              const int key = key0 + 8 * nt + 2 * qlane + e;
+              float& y = s[nt][2 * x + e];
+              y *= pr.scale_log2;
+              if (BIAS) {
+                const int r = min(max(key - pos[x], -bias.left), bias.right);
+                y += entry[head[x] + lut[r + bias.left]];
               }
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float old = mx[xx], m_new = fmaxf(old, m);
-            const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-            if (__any_sync(0xffffffffu, m_new > old)) {
-              const float alpha = fast_exp2(old - m_safe);
-              mx[xx] = m_new;
-              sum[xx] *= alpha;
-#pragma unroll
-              for (int d = 0; d < D / 8; ++d) {
-                acc[d][2 * x] *= alpha;
-                acc[d][2 * x + 1] *= alpha;
-              }
+              if (key > lim[x]) y = -INFINITY;
+              m = fmaxf(m, y);
             }
-            // P goes to the product in bf16, as in the other kernels; its sum stays fp32
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const float old = mx[x], m_new = fmaxf(old, m);
+          const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+          if (__any_sync(0xffffffffu, m_new > old)) {
+            const float alpha = fast_exp2(old - m_safe);
+            mx[x] = m_new;
+            sum[x] *= alpha;
 #pragma unroll
-            for (int nt = 0; nt < 2 * NG; ++nt) {
-              const float p0 = fast_exp2(s[nt][2 * x] - m_safe), p1 = fast_exp2(s[nt][2 * x + 1] - m_safe);
-              sum[xx] += p0 + p1;
-              pf[nt >> 1][x + 2 * (nt & 1)] = pack_bf16x2(p0, p1);
+            for (int d = 0; d < D / 8; ++d) {
+              acc[d][2 * x] *= alpha;
+              acc[d][2 * x + 1] *= alpha;
             }
           }
+          // P goes to the product in bf16, as in the other kernels; its sum stays fp32
+#pragma unroll
+          for (int nt = 0; nt < 2 * NG; ++nt) {
+            const float p0 = fast_exp2(s[nt][2 * x] - m_safe), p1 = fast_exp2(s[nt][2 * x + 1] - m_safe);
+            sum[x] += p0 + p1;
+            pf[nt >> 1][x + 2 * (nt & 1)] = pack_bf16x2(p0, p1);
+          }
+        }
 #pragma unroll
         for (int gk = 0; gk < NG; ++gk) {
           const int row = w0 + 16 * gk + (lane & 15);
@@ -460,10 +447,8 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
             uint32_t vf[4];
             ldmatrix4_trans(vf, vt + (d >> 2) * (L::KEYS * 128) + row * 128 +
                                     (((2 * (d & 3) + (lane >> 4)) ^ (row & 7)) << 4));
-    {
-              mma_16816(acc[2 * d], pf[gk], vf[0], vf[1]);
-              mma_16816(acc[2 * d + 1], pf[gk], vf[2], vf[3]);
-            }
+            mma_16816(acc[2 * d], pf[gk], vf[0], vf[1]);
+            mma_16816(acc[2 * d + 1], pf[gk], vf[2], vf[3]);
           }
         }
       }
@@ -476,15 +461,15 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     float* sm = reinterpret_cast<float*>(smem + L::ML_OFF);
     float* sl = sm + L::WARPS * 16;
 #pragma unroll
-      for (int x = 0; x < NX; ++x) {
-        float t = sum[x];
-        t += __shfl_xor_sync(0xffffffffu, t, 1);
-        t += __shfl_xor_sync(0xffffffffu, t, 2);
-        if (qlane == 0) {
-          sm[warp * 16 + x * 8 + quad] = mx[x];
-          sl[warp * 16 + x * 8 + quad] = t;
-        }
+    for (int x = 0; x < NX; ++x) {
+      float t = sum[x];
+      t += __shfl_xor_sync(0xffffffffu, t, 1);
+      t += __shfl_xor_sync(0xffffffffu, t, 2);
+      if (qlane == 0) {
+        sm[warp * 16 + x * 8 + quad] = mx[x];
+        sl[warp * 16 + x * 8 + quad] = t;
       }
+    }
     // this thread's part of the output: 4 columns of one row in each round; the row's warps
     // are 4 rg .. 4 rg + 3
     const int r = threadIdx.x / (JOIN / 4), c4 = threadIdx.x % (JOIN / 4) * 4;
@@ -498,11 +483,11 @@ __global__ void __launch_bounds__(StepLayout<D, RG>::THREADS, StepLayout<D, RG>:
     for (int round = 0; round < D / JOIN; ++round) {
       if (round > 0) whole_barrier_and(1, NC, true);  // the last round has been read
 #pragma unroll
-        for (int d = 0; d < JOIN / 8; ++d)
+      for (int d = 0; d < JOIN / 8; ++d)
 #pragma unroll
-          for (int x = 0; x < NX; ++x)
-            *reinterpret_cast<float2*>(so + (warp * 16 + x * 8 + quad) * JOIN + 8 * d + 2 * qlane) =
-                make_float2(acc[round * (JOIN / 8) + d][2 * x], acc[round * (JOIN / 8) + d][2 * x + 1]);
+        for (int x = 0; x < NX; ++x)
+          *reinterpret_cast<float2*>(so + (warp * 16 + x * 8 + quad) * JOIN + 8 * d + 2 * qlane) =
+              make_float2(acc[round * (JOIN / 8) + d][2 * x], acc[round * (JOIN / 8) + d][2 * x + 1]);
       ok = whole_barrier_and(1, NC, ok);
       if (!valid) continue;
       if (round == 0) {  // the warps' weights, normalised
