@@ -79,7 +79,7 @@ struct Bias {
     }
     return lo + ((both && r > 0) ? side : 0);
   }
-  // Entry times log2(e).  Entries are clamped to +-2^14 (times log2 e): beyond that one key
+  // Entry times log2(e).  Entries, +inf too, are clamped to +-2^14 (times log2 e): beyond that one key
   // outweighs any other by more than fp32 can hold, and the sum of a score and a bias of
   // the type's lowest value would lose the score.  -inf (the bucket is masked) and NaN stay.
   __device__ __forceinline__ float entry(int u, int h, int Hq) const {

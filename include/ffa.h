@@ -151,8 +151,8 @@ typedef struct ffa_gen_problem {
    * j > i + off fall into the second half of the buckets; without it they count as distance
    * 0.  Bucket u of a side holds the distances [borders[u], borders[u+1]), the last one all
    * from its border on.  borders: host array, one entry for each bucket of a side, ascending
-   * from 0 to at most 1024.  At most 256 buckets.  Finite entries act as if clamped to
-   * +-2^14; -inf masks its bucket. */
+   * from 0 to at most 1024.  At most 256 buckets.  Finite entries and +inf act as if clamped
+   * to +-2^14; -inf masks its bucket. */
   const void* bias;
   int buckets, both;
   const int* borders;
@@ -166,14 +166,14 @@ long long ffa_gen_bwd_workspace(const ffa_gen_problem* p);
 /* Forward.  lse: [batch, q_heads, q_len] fp32 base-2 log-sum-exp, or NULL.
  * o_lo: a tensor like o for the remainder of O behind its rounding to bf16, or NULL; only with
  * a bias.  With it P is multiplied in two parts as well, and o + o_lo is O to 16 bits: what
- * the backward needs for the bias's gradient, whose sums cancel (about a fifth slower). */
+ * the backward needs for the bias's gradient, whose sums cancel (a fifth to a third slower). */
 int ffa_gen_fwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
                 const ffa_gen_tensor* o, const ffa_gen_tensor* o_lo, float* lse, void* workspace,
                 long long workspace_bytes, void* stream);
 
 /* Deterministic backward (no atomics, fixed orders of summation).  dq may be NULL, and dk
  * with dv.  dbias: bf16 [buckets, q_heads] gradient of the bias, or NULL; it needs dq.
- * o_lo: the forward's, or NULL (then delta is that of the rounded O).
+ * o_lo: the forward's, or NULL (then delta is that of the rounded O); read with dq only.
  * Gradients are written whole: rows without a visible counterpart are 0. */
 int ffa_gen_bwd(const ffa_gen_problem* p, const ffa_gen_tensor* q, const ffa_gen_tensor* k, const ffa_gen_tensor* v,
                 const ffa_gen_tensor* o, const ffa_gen_tensor* o_lo, const ffa_gen_tensor* dout, const float* lse,

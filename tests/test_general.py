@@ -372,6 +372,21 @@ def test_lowest_values_act_as_documented():
     assert torch.equal(relative_attention(q, k, v, one), relative_attention(q, k, v, hidden))
 
 
+@pytest.mark.parametrize("n", [2, 200])
+def test_entries_above_the_clamp_act_as_it(n):
+    """+inf and the type's largest value act as 2**14, as documented; NaN does not hide."""
+    q, k, v, _ = inputs(1, 2, 2, 200, 200, 64)
+    top = table(32, 2)
+    top[3] = 2.0 ** 14
+    for x in (math.inf, torch.finfo(torch.bfloat16).max):
+        other = top.clone()
+        other[3] = x
+        assert torch.equal(relative_attention(q[:, :, :n], k, v, other), relative_attention(q[:, :, :n], k, v, top))
+    other[3] = math.nan
+    o = relative_attention(q[:, :, :n], k, v, other)  # distance 3 behind: rows from 3 on see it
+    assert torch.isnan(o[:, :, 3:]).all() and not torch.isnan(o[:, :, :3]).any()
+
+
 def test_bias_gradient_against_differences():
     """The kernel's gradient of the table along a direction against central differences of the
     64-bit forward: their error is of the order of h**2, the bound is the gradient's own."""
