@@ -199,7 +199,14 @@ def relative_attention(query, key, value, bias, max_distance=128, bidirectional=
     logarithm of the distance up to ``max_distance`` (at most 1024), from where the last one
     holds all (:func:`bucket_borders`).  ``bidirectional`` (default: ``not is_causal``) gives
     keys behind the query's position a half of the buckets of their own; otherwise they count
-    as distance 0.  Finite entries act as if clamped to [-2^14, 2^14]; -inf masks its bucket.
+    as distance 0.  Finite entries and +inf act as if clamped to [-2^14, 2^14]; -inf masks its
+    bucket.
+
+    A call whose ``bias`` wants a gradient (``bias.requires_grad`` with gradients enabled) computes
+    its output with probabilities in 16 bits instead of 8, which the gradient's cancelling sums
+    need: its values differ in the last bits from those of other calls, its forward is a fifth to a
+    third slower, and a few queries do not take the single pass of a decoding step.  Decode
+    under ``torch.no_grad()``.
 
     ``is_causal``: key j is visible to query i iff ``j <= p_i``.  ``query_offset`` is an
     integer or an int32 ``[B]`` device tensor: the position of the first query among the keys,

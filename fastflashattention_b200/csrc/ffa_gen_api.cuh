@@ -185,6 +185,10 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias, bool exact) 
     // 3 tokens on 50001 keys, D128: 58 us against 89; B2 H32 over 4 heads, 1 token on 50001
     // keys: 54 against 46; B64 H16, 1 token on 375 to 1500 keys, D64: 60 against 53).  With
     // very many sequences shares would look through them for too long.
+    // The lengths are on the device, so with key_lengths the mean load is a guess, two thirds of
+    // the longest.  Where all are full it costs nothing here (B64 H16, 1 token on 1500 keys, D64:
+    // 65 us with and without the tensor; B8 H32 over 8, 1 on 8192, D128: 44), where all are a
+    // tenth of Sk little (24 against 21 for keys of that shape; 12 against 12).
     // A cluster lies inside one GPC, whose SMs it may not fill: `fit` holds how many clusters
     // of 1, 2, .. 16 CTAs run at once (a B200 with 148 SMs says 296, 148, 71, 33, 14 with two
     // CTAs to an SM and 148, 74, 33, 15, 7 with one; a little less here, as a GPU's SMs may lie
@@ -216,7 +220,10 @@ inline FwdPlan fwd_plan(const ffa_gen_problem* p, const Bias& bias, bool exact) 
   const int rows = small_d ? 128 : 256, keys = small_d ? 64 : 128;
   const long long units = std::max<long long>(1, ceil_div(p->k_len, keys));
   // steps of a block of queries on average: lengths that differ are taken as two thirds of
-  // the longest; under a causal mask the blocks see more and more keys
+  // the longest; under a causal mask the blocks see more and more keys.  The guess serves lengths
+  // that are spread; where all are full it may choose one split too few or too many (B2 H32 over
+  // 8, 500 on 8192, D128: 163 us against 125 without the tensor; B4 H32 over 8, 2048 on 4001: 530
+  // against 462; B16 H20, 224 on 1500, D64: 66 and 66)
   double mean = static_cast<double>(units);
   if (p->batch > 1 && p->key_lengths) mean *= 0.67;
   if (p->causal) {

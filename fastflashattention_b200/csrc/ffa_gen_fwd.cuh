@@ -41,7 +41,7 @@ template <int D>
 struct FwdLayout {
   static constexpr int NT = D == 64 ? 1 : 2;        // 128-row tiles (softmax warpgroups) of a CTA
   // CTAs of an SM.  EXACT holds 32 registers more: three CTAs without spills beat four (B8 H16
-  // S4096 D64: 998 us against 1047)
+  // S4096 D64: 963 us against 995; B8 H12 S1000: 76 against 82)
   static constexpr int ctas(bool exact) { return D == 64 ? (exact ? 3 : 4) : 1; }
   static constexpr int KEYS = D == 64 ? 64 : 128;   // keys of a step
   static constexpr int HALVES = KEYS / 64;          // P is handed over 64 keys at a time
@@ -83,7 +83,7 @@ __device__ __forceinline__ float row_max64(const uint32_t (&a)[32], const uint32
 }
 
 // EMU of every 8 column pairs take their exponentials on the FMA pipe.  At D = 64 one is best
-// with a bias (B8 H16 S4096: 740 us, 767 with two, 777 with none) and as good as two without;
+// (B8 H16 S4096 with a bias: 729 us, 743 with two, 766 with none; without 672, 676 and 698);
 // at D = 128 it changes nothing.
 template <int D, bool CAUSAL, bool BIAS, bool EXACT, int EMU = D == 64 ? 1 : 0>
 __global__ void __launch_bounds__(FwdLayout<D>::THREADS, FwdLayout<D>::ctas(EXACT))
