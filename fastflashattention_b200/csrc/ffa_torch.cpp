@@ -20,6 +20,7 @@
 // raise RuntimeError with the library's message.  The kernels are reached only through the
 // C ABI of libffa_sm100.so (include/ffa.h).
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/autograd.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -123,7 +124,7 @@ class Attention : public torch::autograd::Function<Attention> {
 
   static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx,
                                                torch::autograd::tensor_list grads) {
-    TORCH_CHECK(!grads[0]._fw_grad(0).defined(),
+    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !grads[0]._fw_grad(0).defined(),
                 "the backward of attention does not support forward-mode derivatives of the output's gradient");
     const auto saved = ctx->get_saved_variables();
     const bool causal = ctx->saved_data["causal"].toBool();

@@ -13,6 +13,7 @@
 // the torch caching allocator on the inputs' device, once a call: two calls, or two captured
 // graphs, share none.  Every launch goes on the current stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/autograd.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -242,7 +243,7 @@ class GeneralAttention : public torch::autograd::Function<GeneralAttention> {
 
   static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx,
                                                torch::autograd::tensor_list grads) {
-    TORCH_CHECK(!grads[0]._fw_grad(0).defined(),
+    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !grads[0]._fw_grad(0).defined(),
                 "the backward of general attention does not support forward-mode derivatives of the output's gradient");
     const auto s = ctx->get_saved_variables();
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };

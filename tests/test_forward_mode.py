@@ -62,4 +62,7 @@ def test_on_the_gpu():
         assert torch.equal(fast_attention(q, k, v), want)
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(o, [leaf], forward_ad.make_dual(do, do), retain_graph=True)
+        dual = forward_ad.make_dual(do, do)
+        with forward_ad._set_fwd_grad_enabled(False):  # tangents that nobody wants are no matter
+            assert torch.equal(torch.autograd.grad(o, [leaf], dual, retain_graph=True)[0], g)
     assert torch.equal(torch.autograd.grad(o, [leaf], do)[0], g)

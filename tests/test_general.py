@@ -512,6 +512,9 @@ def test_forward_mode_derivatives_are_refused(Sq, grad):
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(o, [q2], forward_ad.make_dual(do, torch.ones_like(do)), retain_graph=True)
         near(cross_attention(q, k, v), attend(q, k, v)["o"], "o")  # a level without tangents is no matter
+        dual = forward_ad.make_dual(do, torch.ones_like(do))
+        with forward_ad._set_fwd_grad_enabled(False):  # nor are tangents that nobody wants
+            torch.autograd.grad(o, [q2], dual, retain_graph=True)
     near(torch.autograd.grad(o, [q2], do)[0], attend(q, k, v, do)["dq"], "dq")
 
 
