@@ -139,6 +139,41 @@ def test_gradients_through_a_few_rows(B, Hkv, G, Sq, Sk, D):
             inside(g, want[name], name)
 
 
+@pytest.mark.parametrize("B, Hkv, G, Sq, Sk, D", [(2, 4, 8, 3, 20000, 128), (1, 12, 1, 1, 4200, 64)])
+def test_captured_steps_with_gradients(B, Hkv, G, Sq, Sk, D):
+    """Shares with their early join, and clusters of 16, forward and backward in two graphs that are
+    replayed in turn over lengths that change."""
+    q, k, v, do = inputs(B, G * Hkv, Hkv, Sq, Sk, D)
+    bias = table(G * Hkv)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+    def step(lens):
+        a = cross_attention(*leaves, key_lengths=lens, enable_gqa=True)
+        b = relative_attention(*leaves, bias, query_offset=5, key_lengths=lens, enable_gqa=True)
+        return [a.detach(), b.detach(), *torch.autograd.grad(a, leaves, do), *torch.autograd.grad(b, leaves, do)]
+
+    graphs = []
+    for n in range(2):
+        lens = torch.full((B,), Sk - 7 * n, dtype=torch.int32, device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(lens)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(lens)
+        graphs.append((graph, lens, out))
+    for less in (0, 1000, Sk // 2):
+        for graph, lens, _ in graphs:
+            lens -= less
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, lens, out in graphs:
+            for x, y in zip(out, step(lens)):
+                assert torch.equal(x, y)
+
+
 # ---- many rows ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("D", [40, 64, 128])
