@@ -176,8 +176,9 @@ def cross_attention(query, key, value, key_lengths=None, scale=None, enable_gqa=
     ``enable_gqa``: Hq may be a multiple of Hkv; query head h reads key head h // (Hq / Hkv).
     ``scale`` defaults to ``1/sqrt(D)``.
 
-    The backward is deterministic; second and forward-mode derivatives are refused.  A few queries (Hq / Hkv * Sq up to 64, a decoding step)
-    take one pass over the keys that is split over the SMs.
+    The backward is deterministic; second and forward-mode derivatives are refused.  A few
+    queries (Hq / Hkv * Sq up to 64, a decoding step) take one pass over the keys that is
+    split over the SMs.
     """
     reason = _shape_reason(query, key, value, key_lengths, scale, enable_gqa)
     if reason is not None:
